@@ -110,6 +110,63 @@ int ktmi_silu_and_mul(const void* h, int dtype, int64_t R, int64_t N, void* out,
 int ktmi_combine(const void* out, int dtype, const float* w, int64_t T, int64_t top_k, int64_t K,
                  void* res, void* stream);
 
+/* ---- tokens sorted by expert and back -------------------------------------------
+ * For expert products outside ktmi_moe_layer (other weight formats, adapters, training). No
+ * counterpart in the reference, whose sort is part of its layer kernels. Route r = t*top_k + k
+ * goes to expert ids[r]; routes whose id lies outside [0, n_experts) belong to no expert here
+ * and come last. The order is stable: by expert, then by route.
+ *   offsets int32 [n_experts + 1]  expert e's rows are [offsets[e], offsets[e+1])
+ *   perm int32 [tokens*top_k]      perm[p] = the route at place p, ~route past offsets[n_experts]
+ *   pos int32 [tokens, top_k]      pos[r] = the place of route r, ~place for a route of no expert
+ *   rows [tokens*top_k, cols]      x[t] at each of its routes' places, zeros past offsets[n_experts]
+ * x [tokens, cols] in x_dtype with x_stride elements between rows. rows = NULL (x unused): the
+ * order alone. tokens*top_k < 2^31, n_experts <= 2048. Every output is written whole. */
+int64_t ktmi_moe_sort_workspace(int64_t tokens, int64_t top_k, int64_t n_experts);
+int ktmi_moe_sort(const void* x, int x_dtype, int64_t x_stride, int64_t cols, const int32_t* ids, int64_t tokens,
+                  int64_t top_k, int64_t n_experts, void* rows, int32_t* offsets, int32_t* perm, int32_t* pos,
+                  void* workspace, int64_t ws_bytes, void* stream);
+/* y[t] = round( sum_{k ascending} w[t,k] * rows[pos[t,k]] ) over the routes with pos >= 0, in fp32
+ * with one rounding to `dtype`; w = NULL: weights 1, which is the gradient of ktmi_moe_sort with
+ * respect to x. rows [tokens*top_k, cols] with row_stride elements between rows; w fp32; pos as
+ * ktmi_moe_sort writes it (a place past the rows counts as no route). A token without routes gives
+ * zeros. */
+int ktmi_moe_unsort(const void* rows, int dtype, int64_t row_stride, int64_t cols, const float* w, const int32_t* pos,
+                    int64_t tokens, int64_t top_k, void* y, void* stream);
+/* The gradients of ktmi_moe_unsort: drows[pos[t,k]] = w[t,k] * dy[t] (zeros at the places of routes
+ * of no expert, so that every row is written) and dw[t,k] = <dy[t], rows[pos[t,k]]> in fp32 (0 for
+ * those routes). drows = NULL or dw = NULL leaves that one out (rows is read for dw only, w for
+ * drows only); w = NULL: weights 1. */
+int ktmi_moe_unsort_grad(const void* dy, int64_t dy_stride, const void* rows, int64_t row_stride, int dtype,
+                         int64_t cols, const float* w, const int32_t* pos, int64_t tokens, int64_t top_k, void* drows,
+                         float* dw, void* stream);
+
+/* ---- products with 4-bit weights and group scales ---------------------------------
+ * y[r, n] = sum_g scale[e, n, g] * sum_{c in group g} (code[e, n, c] - zero[e, n, g]) * x[r, c], summed
+ * in fp32 and rounded once to x's type. For checkpoints of plain 4-bit codes (no ggml type); no
+ * counterpart in the reference.
+ *   codes uint8 [n_experts, rows, ceil(cols/2)]: byte j of a row holds code 2j in its low and
+ *         2j+1 in its high four bits (codes packed eight to an int32 along cols are the same bytes)
+ *   scales [n_experts, rows, ceil(cols/group)] in scale_dtype; zeros uint8 of that shape, or NULL: 8
+ *   group: 32, 64, a multiple of 128, or at least cols (one group a row)
+ * x rows have x_stride elements between them. Any cols, rows and alignment of codes; scales,
+ * zeros, x and y as their types require. */
+/* dense: y[t] = W x[t], y [tokens, rows] */
+int ktmi_w4_vec(const void* x, int x_dtype, int64_t x_stride, int64_t cols, const void* codes, const void* scales,
+                int scale_dtype, const void* zeros, int64_t group, int64_t rows, int64_t tokens, void* y, void* stream);
+/* by route: y[r] = W[ids[r]] x[r / top_k], y [tokens*top_k, rows]; ids outside [0, n_experts) give
+ * zero rows. The routes of one expert share one read of its weights in decode windows. */
+int64_t ktmi_moe_w4_vec_workspace(int64_t tokens, int64_t top_k, int64_t n_experts);
+int ktmi_moe_w4_vec(const void* x, int x_dtype, int64_t x_stride, int64_t cols, const void* codes, const void* scales,
+                    int scale_dtype, const void* zeros, int64_t group, int64_t rows, int64_t n_experts,
+                    const int32_t* ids, int64_t top_k, int64_t tokens, void* y, void* workspace, int64_t ws_bytes,
+                    void* stream);
+/* rows sorted by expert (ktmi_moe_sort): y[p] = W[e] x[p] for offsets[e] <= p < offsets[e+1],
+ * y [n_rows, rows]; rows past offsets[n_experts] give zero rows. offsets must ascend within
+ * [0, n_rows]; values outside are clamped to it. */
+int ktmi_moe_w4_sorted(const void* x, int x_dtype, int64_t x_stride, int64_t cols, const void* codes,
+                       const void* scales, int scale_dtype, const void* zeros, int64_t group, int64_t rows,
+                       int64_t n_experts, const int32_t* offsets, int64_t n_rows, void* y, void* stream);
+
 /* ---- one hot-expert MoE layer -----------------------------------------------------
  * The GPU half of a layer: routes (t, k) with slot_ids[t*top_k+k] >= 0 run the expert in
  * that slot; y[t] = combine over k of (silu(x_t Wg^T) * (x_t Wu^T)) Wd^T * w[t,k], cold

@@ -61,6 +61,15 @@ SIGNATURES = {
     "ktmi_hot_route": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp]),
     "ktmi_silu_and_mul": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp]),
     "ktmi_combine": (_i32, [_vp, _i32, _vp, _i64, _i64, _i64, _vp, _vp]),
+    "ktmi_moe_sort_workspace": (_i64, [_i64, _i64, _i64]),
+    "ktmi_moe_sort": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "ktmi_moe_unsort": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp]),
+    "ktmi_moe_unsort_grad": (_i32, [_vp, _i64, _vp, _i64, _i32, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _vp]),
+    "ktmi_w4_vec": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _i32, _vp, _i64, _i64, _i64, _vp, _vp]),
+    "ktmi_moe_w4_vec_workspace": (_i64, [_i64, _i64, _i64]),
+    "ktmi_moe_w4_vec": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _i32, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp,
+                               _i64, _vp]),
+    "ktmi_moe_w4_sorted": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _i32, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
     "ktmi_moe_layer_workspace": (_i64, [C.POINTER(ktmi_layer), _i64, _i64, _i32]),
     "ktmi_moe_layer": (_i32, [C.POINTER(ktmi_layer), _vp, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _i32, _vp]),
     "ktmi_moe_layer_mode": (_i32, [C.POINTER(ktmi_layer), _i64, _i64]),
@@ -123,6 +132,18 @@ def stream_ptr(device=None) -> int:
     import torch
 
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def on_device_of(t, fn, *args):
+    """fn(stream handle, *args) with t's device current: the current stream of that device, on which the
+    call's launches and its tensors' allocations are ordered."""
+    import torch
+
+    index = t.get_device()
+    if torch._C._cuda_getDevice() == index:
+        return fn(torch._C._cuda_getCurrentRawStream(index), *args)
+    with torch.cuda.device(index):
+        return fn(torch._C._cuda_getCurrentRawStream(index), *args)
 
 
 def dtype_code(dtype) -> int:

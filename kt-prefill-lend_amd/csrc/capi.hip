@@ -155,6 +155,147 @@ int ktmi_combine(const void* out, int dtype, const float* w, int64_t T, int64_t 
   return launch_combine(out, dtype, w, T, top_k, K, res, (hipStream_t)stream);
 }
 
+// ---- tokens sorted by expert and back
+
+// the shape of a sort's or unsort's routes: the grids take a token a block, the places are int32
+static int check_routes(const char* what, int dtype, int64_t cols, int64_t tokens, int64_t top_k) {
+  KTMI_REQUIRE(dtype_ok(dtype), KTMI_EINVAL, "%s: dtype %d", what, dtype);
+  KTMI_REQUIRE(cols > 0 && cols <= (1 << 24) && tokens >= 0 && top_k > 0, KTMI_EINVAL,
+               "%s: cols %lld (at most 2^24) tokens %lld top_k %lld", what, (long long)cols, (long long)tokens,
+               (long long)top_k);
+  KTMI_REQUIRE(top_k <= 0x7FFFFFFF && tokens <= 0x7FFFFFFF / top_k, KTMI_EINVAL, "%s: %lld tokens x top-%lld routes (below 2^31)",
+               what, (long long)tokens, (long long)top_k);
+  return KTMI_OK;
+}
+
+int64_t ktmi_moe_sort_workspace(int64_t tokens, int64_t top_k, int64_t n_experts) {
+  if (tokens <= 0 || top_k <= 0 || n_experts <= 0 || tokens > 0x7FFFFFFF / top_k) return 0;
+  return moe_sort_chunks(tokens * top_k) * (n_experts + 1) * (int64_t)sizeof(int);
+}
+
+int ktmi_moe_sort(const void* x, int x_dtype, int64_t x_stride, int64_t cols, const int32_t* ids, int64_t tokens,
+                  int64_t top_k, int64_t n_experts, void* rows, int32_t* offsets, int32_t* perm, int32_t* pos,
+                  void* workspace, int64_t ws_bytes, void* stream) {
+  g_err[0] = 0;
+  int rc = check_routes("moe_sort", x_dtype, cols, tokens, top_k);
+  if (rc) return rc;
+  KTMI_REQUIRE(n_experts > 0 && n_experts <= SORT_MAX_EXPERTS, KTMI_EINVAL, "moe_sort: %lld experts (1 to %lld)",
+               (long long)n_experts, (long long)SORT_MAX_EXPERTS);
+  KTMI_REQUIRE(offsets && (tokens == 0 || (ids && perm && pos && (!rows || x))), KTMI_EINVAL, "moe_sort: null pointer");
+  const int es = x_dtype == KTMI_F32 ? 4 : 2;
+  KTMI_REQUIRE(aligned(x, es) && aligned(rows, es), KTMI_EINVAL, "moe_sort: x and rows must be aligned to their type");
+  KTMI_REQUIRE(!rows || x_stride >= cols || tokens <= 1, KTMI_EINVAL, "moe_sort: x_stride %lld below cols %lld",
+               (long long)x_stride, (long long)cols);
+  const int64_t need = ktmi_moe_sort_workspace(tokens, top_k, n_experts);
+  KTMI_REQUIRE(need == 0 || (workspace && ws_bytes >= need && aligned(workspace, 4)), KTMI_ESPACE,
+               "moe_sort: workspace %lld < %lld bytes", (long long)ws_bytes, (long long)need);
+  return launch_moe_sort((const uint8_t*)x, es, x_stride, cols, ids, tokens, top_k, n_experts, (uint8_t*)rows, offsets,
+                         perm, pos, (int*)workspace, (hipStream_t)stream);
+}
+
+int ktmi_moe_unsort(const void* rows, int dtype, int64_t row_stride, int64_t cols, const float* w, const int32_t* pos,
+                    int64_t tokens, int64_t top_k, void* y, void* stream) {
+  g_err[0] = 0;
+  int rc = check_routes("moe_unsort", dtype, cols, tokens, top_k);
+  if (rc) return rc;
+  if (tokens == 0) return KTMI_OK;
+  const int es = dtype == KTMI_F32 ? 4 : 2;
+  KTMI_REQUIRE(rows && pos && y && aligned(rows, es) && aligned(y, es), KTMI_EINVAL,
+               "moe_unsort: null pointer, or one not aligned to its type");
+  KTMI_REQUIRE(row_stride >= cols || tokens * top_k <= 1, KTMI_EINVAL, "moe_unsort: row_stride %lld below cols %lld",
+               (long long)row_stride, (long long)cols);
+  return launch_moe_unsort(rows, dtype, row_stride, cols, w, pos, tokens, top_k, y, (hipStream_t)stream);
+}
+
+int ktmi_moe_unsort_grad(const void* dy, int64_t dy_stride, const void* rows, int64_t row_stride, int dtype,
+                         int64_t cols, const float* w, const int32_t* pos, int64_t tokens, int64_t top_k, void* drows,
+                         float* dw, void* stream) {
+  g_err[0] = 0;
+  int rc = check_routes("moe_unsort_grad", dtype, cols, tokens, top_k);
+  if (rc) return rc;
+  if (tokens == 0 || (!drows && !dw)) return KTMI_OK;
+  const int es = dtype == KTMI_F32 ? 4 : 2;
+  KTMI_REQUIRE(dy && pos && (!dw || rows) && aligned(dy, es) && aligned(rows, es) && aligned(drows, es), KTMI_EINVAL,
+               "moe_unsort_grad: null pointer, or one not aligned to its type");
+  KTMI_REQUIRE(dy_stride >= cols || tokens <= 1, KTMI_EINVAL, "moe_unsort_grad: dy_stride %lld below cols %lld",
+               (long long)dy_stride, (long long)cols);
+  KTMI_REQUIRE(!dw || row_stride >= cols || tokens * top_k <= 1, KTMI_EINVAL,
+               "moe_unsort_grad: row_stride %lld below cols %lld", (long long)row_stride, (long long)cols);
+  return launch_moe_unsort_grad(dy, dy_stride, rows, row_stride, dtype, cols, w, pos, tokens, top_k, drows, dw,
+                                (hipStream_t)stream);
+}
+
+// ---- products with 4-bit weights
+
+// n: rows of x, routes: rows of y
+static int check_w4(const char* what, const W4Args& a, int64_t n) {
+  KTMI_REQUIRE(dtype_ok(a.x_dtype) && dtype_ok(a.scale_dtype), KTMI_EINVAL, "%s: x dtype %d scale dtype %d", what,
+               a.x_dtype, a.scale_dtype);
+  KTMI_REQUIRE(a.cols > 0 && a.cols <= (1 << 24) && a.rows > 0 && a.rows <= (1 << 24), KTMI_EINVAL,
+               "%s: cols %lld rows %lld (1 to 2^24)", what, (long long)a.cols, (long long)a.rows);
+  KTMI_REQUIRE(a.n_experts > 0 && a.n_experts <= SORT_MAX_EXPERTS, KTMI_EINVAL, "%s: %lld experts (1 to %lld)", what,
+               (long long)a.n_experts, (long long)SORT_MAX_EXPERTS);
+  KTMI_REQUIRE(a.group == 32 || a.group == 64 || (a.group > 0 && (a.group % 128 == 0 || a.group >= a.cols)), KTMI_EINVAL,
+               "%s: group %lld (32, 64, a multiple of 128, or at least cols)", what, (long long)a.group);
+  KTMI_REQUIRE(n >= 0 && a.top_k > 0 && a.n_routes >= 0, KTMI_EINVAL, "%s: %lld rows of x, top_k %lld", what, (long long)n,
+               (long long)a.top_k);
+  if (a.n_routes == 0) return KTMI_OK;
+  const int es = a.x_dtype == KTMI_F32 ? 4 : 2, ss = a.scale_dtype == KTMI_F32 ? 4 : 2;
+  KTMI_REQUIRE(a.x && a.codes && a.scales && a.y, KTMI_EINVAL, "%s: null pointer", what);
+  KTMI_REQUIRE(aligned(a.x, es) && aligned(a.y, es) && aligned(a.scales, ss), KTMI_EINVAL,
+               "%s: x, y and scales must be aligned to their types", what);
+  KTMI_REQUIRE(a.x_stride >= a.cols || n <= 1, KTMI_EINVAL, "%s: x_stride %lld below cols %lld", what, (long long)a.x_stride,
+               (long long)a.cols);
+  return KTMI_OK;
+}
+
+int ktmi_w4_vec(const void* x, int x_dtype, int64_t x_stride, int64_t cols, const void* codes, const void* scales,
+                int scale_dtype, const void* zeros, int64_t group, int64_t rows, int64_t tokens, void* y, void* stream) {
+  g_err[0] = 0;
+  const W4Args a = {x, x_stride, cols, (const uint8_t*)codes, scales, (const uint8_t*)zeros, group, rows, 1, nullptr, nullptr,
+                    1, tokens, y, nullptr, x_dtype, scale_dtype};
+  int rc = check_w4("w4_vec", a, tokens);
+  if (rc || tokens == 0) return rc;
+  KTMI_REQUIRE(tokens <= 0x7FFFFFFF, KTMI_EINVAL, "w4_vec: %lld rows (below 2^31)", (long long)tokens);
+  return launch_w4(a, (hipStream_t)stream);
+}
+
+int64_t ktmi_moe_w4_vec_workspace(int64_t tokens, int64_t top_k, int64_t n_experts) {
+  if (tokens <= 0 || top_k <= 0 || n_experts <= 0 || tokens > 0x7FFFFFFF / top_k) return 0;
+  return w4_workspace(tokens, top_k, n_experts);
+}
+
+int ktmi_moe_w4_vec(const void* x, int x_dtype, int64_t x_stride, int64_t cols, const void* codes, const void* scales,
+                    int scale_dtype, const void* zeros, int64_t group, int64_t rows, int64_t n_experts,
+                    const int32_t* ids, int64_t top_k, int64_t tokens, void* y, void* workspace, int64_t ws_bytes,
+                    void* stream) {
+  g_err[0] = 0;
+  KTMI_REQUIRE(tokens >= 0 && top_k > 0 && top_k <= 65535 && tokens <= 0x7FFFFFFF / top_k, KTMI_EINVAL,
+               "moe_w4_vec: %lld tokens x top-%lld (at most 65535 a token, 2^31 in all)", (long long)tokens, (long long)top_k);
+  const W4Args a = {x, x_stride, cols, (const uint8_t*)codes, scales, (const uint8_t*)zeros, group, rows, n_experts, ids,
+                    nullptr, top_k, tokens * top_k, y, (uint8_t*)workspace, x_dtype, scale_dtype};
+  int rc = check_w4("moe_w4_vec", a, tokens);
+  if (rc || tokens == 0) return rc;
+  KTMI_REQUIRE(ids, KTMI_EINVAL, "moe_w4_vec: null pointer");
+  const int64_t need = w4_workspace(tokens, top_k, n_experts);
+  KTMI_REQUIRE(need == 0 || (workspace && ws_bytes >= need && aligned(workspace, 16)), KTMI_ESPACE,
+               "moe_w4_vec: workspace %lld < %lld bytes", (long long)ws_bytes, (long long)need);
+  return launch_w4(a, (hipStream_t)stream);
+}
+
+int ktmi_moe_w4_sorted(const void* x, int x_dtype, int64_t x_stride, int64_t cols, const void* codes,
+                       const void* scales, int scale_dtype, const void* zeros, int64_t group, int64_t rows,
+                       int64_t n_experts, const int32_t* offsets, int64_t n_rows, void* y, void* stream) {
+  g_err[0] = 0;
+  const W4Args a = {x, x_stride, cols, (const uint8_t*)codes, scales, (const uint8_t*)zeros, group, rows, n_experts, nullptr,
+                    offsets, 1, n_rows, y, nullptr, x_dtype, scale_dtype};
+  int rc = check_w4("moe_w4_sorted", a, n_rows);
+  if (rc || n_rows == 0) return rc;
+  KTMI_REQUIRE(offsets, KTMI_EINVAL, "moe_w4_sorted: null pointer");
+  KTMI_REQUIRE(n_rows <= 0x7FFFFFFF, KTMI_EINVAL, "moe_w4_sorted: %lld rows (below 2^31)", (long long)n_rows);
+  return launch_w4(a, (hipStream_t)stream);
+}
+
 // ---- scratch for ktmi_moe_layer_noalloc
 // A file-scope device array that stands in for the caller's workspace. In host code its
 // name is a host-side stand-in, not a device address: the address on each device comes

@@ -13,6 +13,38 @@ int launch_silu_and_mul(const void* h, int dtype, int64_t R, int64_t N, void* ou
 int launch_combine(const void* out, int dtype, const float* w, int64_t T, int64_t top_k, int64_t K, void* res,
                    hipStream_t stream);
 
+// Tokens sorted by expert and back (moe_sort.hip). x_stride, row_stride, dy_stride in elements, es
+// the bytes of one; counts: moe_sort_chunks(routes) * (E + 1) ints; rows = NULL: the order alone.
+constexpr int64_t SORT_MAX_EXPERTS = 2048;
+int64_t moe_sort_chunks(int64_t routes);
+int launch_moe_sort(const uint8_t* x, int es, int64_t x_stride, int64_t cols, const int32_t* ids, int64_t tokens,
+                    int64_t top_k, int64_t E, uint8_t* rows, int32_t* offsets, int32_t* perm, int32_t* pos, int* counts,
+                    hipStream_t stream);
+int launch_moe_unsort(const void* rows, int dtype, int64_t row_stride, int64_t cols, const float* w, const int32_t* pos,
+                      int64_t tokens, int64_t top_k, void* y, hipStream_t stream);
+int launch_moe_unsort_grad(const void* dy, int64_t dy_stride, const void* rows, int64_t row_stride, int dtype,
+                           int64_t cols, const float* w, const int32_t* pos, int64_t tokens, int64_t top_k, void* drows,
+                           float* dw, hipStream_t stream);
+
+// Products with 4-bit weights (w4.hip). Route r's activation row is r / top_k and its expert ids[r]; with
+// offsets instead, row r and the expert whose segment holds it; with neither, row r and the one matrix.
+struct W4Args {
+  const void* x;
+  int64_t x_stride, cols;
+  const uint8_t* codes;
+  const void* scales;
+  const uint8_t* zeros;
+  int64_t group, rows, n_experts;
+  const int32_t* ids;
+  const int32_t* offsets;
+  int64_t top_k, n_routes;
+  void* y;
+  uint8_t* ws;
+  int x_dtype, scale_dtype;
+};
+int64_t w4_workspace(int64_t tokens, int64_t top_k, int64_t n_experts);
+int launch_w4(const W4Args& a, hipStream_t stream);
+
 // GEMV over raw GGUF rows against q8_1 activations (the decode-window kernel).
 // xq: q8_1 rows of the tokens, xq_stride bytes apart. W: slot tensor (w_is_table = 0,
 // experts w_expert_stride bytes apart) or int64 table of per-slot addresses. Expert ids

@@ -1,0 +1,372 @@
+// Tokens sorted by expert and back, with the weights applied, and the gradients of both.
+//
+// With key(r) = ids[r] for a valid id and E for any other, a route's place is
+//   p(r) = #{r' : key(r') < key(r)  or  key(r') = key(r) and r' < r},
+// a stable counting sort: a histogram of each chunk of routes, then per chunk the places from the
+// totals of the keys below, of the chunks before and of the routes before inside the chunk. The
+// row copies, the weighted sums and the gradients then go by token: a token's row is read once
+// and its routes' places are wave-uniform.
+#include <type_traits>
+
+#include "kernels.h"
+
+namespace ktmi {
+
+namespace {
+
+constexpr int SORT_THREADS = 256;
+constexpr int SORT_CHUNK = 2048;  // routes of one block of the order's two kernels
+constexpr int ROW_WAVES = 4;      // waves of a row kernel's block, at most
+
+__device__ __forceinline__ int key_of(int id, int E) { return id >= 0 && id < E ? id : E; }
+
+__device__ __forceinline__ void sort_wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// counts[chunk][E + 1]: the chunk's routes by key
+__global__ __launch_bounds__(SORT_THREADS) void sort_count_kernel(const int32_t* __restrict__ ids, int R, int E,
+                                                                  int* __restrict__ counts) {
+  extern __shared__ int hist[];
+  for (int e = threadIdx.x; e <= E; e += SORT_THREADS) hist[e] = 0;
+  __syncthreads();
+  const int64_t r0 = (int64_t)blockIdx.x * SORT_CHUNK;
+#pragma unroll
+  for (int i = 0; i < SORT_CHUNK / SORT_THREADS; ++i) {
+    const int64_t r = r0 + i * SORT_THREADS + threadIdx.x;
+    if (r < R) atomicAdd(&hist[key_of(ids[r], E)], 1);
+  }
+  __syncthreads();
+  int* out = counts + (int64_t)blockIdx.x * (E + 1);
+  for (int e = threadIdx.x; e <= E; e += SORT_THREADS) out[e] = hist[e];
+}
+
+// exclusive sum over the block of one value a thread (SORT_THREADS threads); tmp: 4 ints of LDS
+__device__ __forceinline__ int block_exclusive(int v, int* tmp) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int s = v;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int u = __shfl_up(s, d);
+    if (lane >= d) s += u;
+  }
+  if (lane == 63) tmp[wave] = s;
+  __syncthreads();
+  int before = 0;
+  for (int w = 0; w < wave; ++w) before += tmp[w];
+  __syncthreads();
+  return before + s - v;
+}
+
+// The places of a chunk's routes. LDS: the keys' first places [E + 1], then one running place for
+// every key and wave [4][E + 1]. Wave w owns routes [512 w, 512 w + 512) of the chunk, 64 at a
+// time in order; the lanes of one key find each other by ballots over the key's bits.
+__global__ __launch_bounds__(SORT_THREADS) void sort_place_kernel(const int32_t* __restrict__ ids, int R, int E,
+                                                                  int key_bits, const int* __restrict__ counts,
+                                                                  int chunks, int32_t* __restrict__ offsets,
+                                                                  int32_t* __restrict__ perm,
+                                                                  int32_t* __restrict__ pos) {
+  extern __shared__ int lds[];
+  __shared__ int tmp[4];
+  const int n = E + 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.x;
+  int* total = lds;
+  int* run = lds + n;
+  for (int e = threadIdx.x; e < n; e += SORT_THREADS) {
+    int before = 0, all = 0;
+    for (int i = 0; i < chunks; ++i) {
+      const int v = counts[(int64_t)i * n + e];
+      all += v;
+      if (i < c) before += v;
+    }
+    total[e] = all;
+    run[e] = before;
+    run[n + e] = run[2 * n + e] = run[3 * n + e] = 0;
+  }
+  __syncthreads();
+  // exclusive sums of the totals: each thread its own consecutive keys
+  const int per = (n + SORT_THREADS - 1) / SORT_THREADS;
+  const int e0 = threadIdx.x * per;
+  int sum = 0;
+  for (int e = e0; e < e0 + per && e < n; ++e) sum += total[e];
+  int at = block_exclusive(sum, tmp);
+  for (int e = e0; e < e0 + per && e < n; ++e) {
+    const int v = total[e];
+    run[e] += at;
+    if (c == 0) offsets[e] = at;
+    at += v;
+  }
+  // the wave's own routes and their counts for the waves after it
+  int key[SORT_CHUNK / SORT_THREADS];
+  const int64_t r0 = (int64_t)c * SORT_CHUNK + wave * (SORT_CHUNK / 4);
+#pragma unroll
+  for (int i = 0; i < SORT_CHUNK / SORT_THREADS; ++i) {
+    const int64_t r = r0 + 64 * i + lane;
+    key[i] = r < R ? key_of(ids[r], E) : -1;
+    if (key[i] >= 0 && wave < 3) atomicAdd(&run[(wave + 1) * n + key[i]], 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < n; e += SORT_THREADS) {
+    int v = run[e];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) run[w * n + e] = v += run[w * n + e];
+  }
+  __syncthreads();
+  int* mine = run + wave * n;
+  const uint64_t below = (1ull << lane) - 1ull;
+#pragma unroll
+  for (int i = 0; i < SORT_CHUNK / SORT_THREADS; ++i) {
+    const bool in = key[i] >= 0;
+    uint64_t same = __ballot(in);
+    for (int b = 0; b < key_bits; ++b) {
+      const bool bit = (key[i] >> b) & 1;
+      const uint64_t m = __ballot(bit);
+      same &= bit ? m : ~m;
+    }
+    if (in) {
+      const int rank = __popcll(same & below);
+      const int first = mine[key[i]];
+      sort_wave_fence();
+      if (rank == 0) mine[key[i]] = first + __popcll(same);
+      const int p = first + rank, r = (int)(r0 + 64 * i + lane);
+      const bool valid = key[i] < E;
+      perm[p] = valid ? r : ~r;
+      pos[r] = valid ? p : ~p;
+    }
+    sort_wave_fence();
+  }
+}
+
+// 16 bytes of a row at any alignment of its elements
+__device__ __forceinline__ u32x4_t load16(const void* p) { return gload<u32x4_a2_t>(p); }
+__device__ __forceinline__ void store16(void* p, const u32x4_t& v) { *(u32x4_a2_t*)p = v; }
+
+// A row of `bytes` bytes in 16-byte pieces, lane by lane; the last piece ends with the row and may
+// overlap the one before it. Rows below 16 bytes go element by element (ES bytes each).
+template <int ES>
+__global__ __launch_bounds__(64 * ROW_WAVES) void sort_rows_kernel(const uint8_t* __restrict__ x, int64_t x_stride,
+                                                                   int64_t bytes, const int32_t* __restrict__ pos,
+                                                                   int top_k, uint8_t* __restrict__ rows) {
+  const int64_t t = blockIdx.x;
+  const int64_t at = 16 * ((int64_t)blockIdx.y * blockDim.x + threadIdx.x);
+  if (at >= bytes) return;
+  const int32_t* tp = pos + t * top_k;
+  if (bytes >= 16) {
+    const int64_t b = at < bytes - 16 ? at : bytes - 16;
+    const u32x4_t v = load16(x + t * x_stride + b), zero = {0, 0, 0, 0};
+    for (int j = 0; j < top_k; ++j) {
+      const int p = tp[j];
+      store16(rows + (int64_t)(p >= 0 ? p : ~p) * bytes + b, p >= 0 ? v : zero);
+    }
+  } else {
+    using E = typename std::conditional<ES == 4, uint32_t, uint16_t>::type;
+    for (int64_t i = 0; i < bytes / ES; ++i) {
+      const E v = ((const E*)(x + t * x_stride))[i];
+      for (int j = 0; j < top_k; ++j) {
+        const int p = tp[j];
+        ((E*)(rows + (int64_t)(p >= 0 ? p : ~p) * bytes))[i] = p >= 0 ? v : (E)0;
+      }
+    }
+  }
+}
+
+// V values of a row: 16 bytes of them, or one (rows shorter than 16 bytes)
+template <typename T, int V>
+struct Piece {
+  float f[V];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (V == 1) {
+      f[0] = (float)p[0];
+    } else {
+      const u32x4_t w = load16(p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t u = w[i];  // a bit cast of w[i] itself takes element 0
+        if constexpr (sizeof(T) == 4) {
+          f[i] = __builtin_bit_cast(float, u);
+        } else {
+          f[2 * i] = (float)__builtin_bit_cast(T, (uint16_t)u);
+          f[2 * i + 1] = (float)__builtin_bit_cast(T, (uint16_t)(u >> 16));
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (V == 1) {
+      p[0] = (T)f[0];
+    } else {
+      u32x4_t w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4)
+          w[i] = __builtin_bit_cast(uint32_t, f[i]);
+        else
+          w[i] = (uint32_t)__builtin_bit_cast(uint16_t, (T)f[2 * i]) |
+                 (uint32_t)__builtin_bit_cast(uint16_t, (T)f[2 * i + 1]) << 16;
+      }
+      store16(p, w);
+    }
+  }
+};
+
+template <typename T, int V>
+__global__ __launch_bounds__(64 * ROW_WAVES) void unsort_kernel(const T* __restrict__ rows, int64_t row_stride,
+                                                                int64_t cols, const float* __restrict__ w,
+                                                                const int32_t* __restrict__ pos, int top_k, int n_rows,
+                                                                T* __restrict__ y) {
+  const int64_t t = blockIdx.x;
+  const int64_t at = V * ((int64_t)blockIdx.y * blockDim.x + threadIdx.x);
+  if (at >= cols) return;
+  const int64_t c = at < cols - V ? at : cols - V;
+  Piece<T, V> acc;
+#pragma unroll
+  for (int i = 0; i < V; ++i) acc.f[i] = 0.0f;
+  for (int j = 0; j < top_k; ++j) {
+    const int p = pos[t * top_k + j];
+    if (p < 0 || p >= n_rows) continue;
+    const float wj = w ? w[t * top_k + j] : 1.0f;
+    Piece<T, V> v;
+    v.load(rows + p * row_stride + c);
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc.f[i] = fmaf(wj, v.f[i], acc.f[i]);
+  }
+  acc.store(y + t * cols + c);
+}
+
+// One block a token: dy[t] against its routes' rows. The dots are summed a lane's own pieces first,
+// then over the wave's lanes and over the waves, always in the same order.
+template <typename T, int V>
+__global__ __launch_bounds__(64 * ROW_WAVES) void unsort_grad_kernel(const T* __restrict__ dy, int64_t dy_stride,
+                                                                     const T* __restrict__ rows, int64_t row_stride,
+                                                                     int64_t cols, const float* __restrict__ w,
+                                                                     const int32_t* __restrict__ pos, int top_k,
+                                                                     int n_rows, T* __restrict__ drows,
+                                                                     float* __restrict__ dw) {
+  __shared__ float part[ROW_WAVES];
+  const int64_t t = blockIdx.x;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int j = 0; j < top_k; ++j) {
+    const int p = pos[t * top_k + j], q = p >= 0 ? p : ~p;
+    const bool valid = p >= 0 && p < n_rows;
+    const float wj = valid ? (w ? w[t * top_k + j] : 1.0f) : 0.0f;
+    float dot = 0.0f;
+    for (int64_t at = (int64_t)V * threadIdx.x; at < cols; at += (int64_t)V * blockDim.x) {
+      const int64_t c = at < cols - V ? at : cols - V;
+      const int skip = (int)(at - c);  // values of this piece that the one before holds too
+      Piece<T, V> d, o;
+      d.load(dy + t * dy_stride + c);
+      if (dw && valid) {
+        o.load(rows + p * row_stride + c);
+#pragma unroll
+        for (int i = 0; i < V; ++i) dot = i < skip ? dot : fmaf(d.f[i], o.f[i], dot);
+      }
+      if (drows && q < n_rows) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) o.f[i] = valid ? wj * d.f[i] : 0.0f;
+        o.store(drows + q * cols + c);
+      }
+    }
+    if (dw) {
+#pragma unroll
+      for (int s = 32; s; s >>= 1) dot += __shfl_xor(dot, s);
+      if (lane == 0) part[wave] = dot;
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        float all = 0.0f;
+        for (int i = 0; i < (int)(blockDim.x >> 6); ++i) all += part[i];
+        dw[t * top_k + j] = valid ? all : 0.0f;
+      }
+      __syncthreads();
+    }
+  }
+}
+
+int row_threads(int64_t pieces) { return (int)(pieces >= 64 * ROW_WAVES ? 64 * ROW_WAVES : (pieces + 63) / 64 * 64); }
+
+}  // namespace
+
+int64_t moe_sort_chunks(int64_t routes) { return (routes + SORT_CHUNK - 1) / SORT_CHUNK; }
+
+int launch_moe_sort(const uint8_t* x, int es, int64_t x_stride, int64_t cols, const int32_t* ids, int64_t tokens,
+                    int64_t top_k, int64_t E, uint8_t* rows, int32_t* offsets, int32_t* perm, int32_t* pos, int* counts,
+                    hipStream_t stream) {
+  const int R = (int)(tokens * top_k), n = (int)E + 1;
+  const int chunks = (int)moe_sort_chunks(R);
+  int bits = 0;
+  while ((n - 1) >> bits) ++bits;
+  if (chunks) sort_count_kernel<<<chunks, SORT_THREADS, n * sizeof(int), stream>>>(ids, R, (int)E, counts);
+  sort_place_kernel<<<chunks ? chunks : 1, SORT_THREADS, 5 * n * sizeof(int), stream>>>(ids, R, (int)E, bits, counts, chunks,
+                                                                                        offsets, perm, pos);
+  if (rows && R) {
+    const int64_t bytes = cols * es, pieces = (bytes + 15) / 16;
+    const int th = row_threads(pieces);
+    dim3 grid((unsigned)tokens, (unsigned)((pieces + th - 1) / th));
+    if (es == 4)
+      sort_rows_kernel<4><<<grid, th, 0, stream>>>(x, x_stride * es, bytes, pos, (int)top_k, rows);
+    else
+      sort_rows_kernel<2><<<grid, th, 0, stream>>>(x, x_stride * es, bytes, pos, (int)top_k, rows);
+  }
+  KTMI_HIP_TRY(hipGetLastError());
+  return KTMI_OK;
+}
+
+namespace {
+
+template <typename T>
+void unsort_of(const void* rows, int64_t row_stride, int64_t cols, const float* w, const int32_t* pos, int64_t tokens,
+               int64_t top_k, void* y, hipStream_t stream) {
+  constexpr int V = 16 / sizeof(T);
+  const int v = cols >= V ? V : 1;
+  const int64_t pieces = (cols + v - 1) / v;
+  const int th = row_threads(pieces), R = (int)(tokens * top_k);
+  dim3 grid((unsigned)tokens, (unsigned)((pieces + th - 1) / th));
+  if (v == V)
+    unsort_kernel<T, V><<<grid, th, 0, stream>>>((const T*)rows, row_stride, cols, w, pos, (int)top_k, R, (T*)y);
+  else
+    unsort_kernel<T, 1><<<grid, th, 0, stream>>>((const T*)rows, row_stride, cols, w, pos, (int)top_k, R, (T*)y);
+}
+
+template <typename T>
+void unsort_grad_of(const void* dy, int64_t dy_stride, const void* rows, int64_t row_stride, int64_t cols, const float* w,
+                    const int32_t* pos, int64_t tokens, int64_t top_k, void* drows, float* dw, hipStream_t stream) {
+  constexpr int V = 16 / sizeof(T);
+  const int v = cols >= V ? V : 1;
+  const int th = row_threads((cols + v - 1) / v), R = (int)(tokens * top_k);
+  if (v == V)
+    unsort_grad_kernel<T, V><<<(unsigned)tokens, th, 0, stream>>>((const T*)dy, dy_stride, (const T*)rows, row_stride, cols,
+                                                                  w, pos, (int)top_k, R, (T*)drows, dw);
+  else
+    unsort_grad_kernel<T, 1><<<(unsigned)tokens, th, 0, stream>>>((const T*)dy, dy_stride, (const T*)rows, row_stride, cols,
+                                                                  w, pos, (int)top_k, R, (T*)drows, dw);
+}
+
+}  // namespace
+
+int launch_moe_unsort(const void* rows, int dtype, int64_t row_stride, int64_t cols, const float* w, const int32_t* pos,
+                      int64_t tokens, int64_t top_k, void* y, hipStream_t stream) {
+  switch (dtype) {
+    case KTMI_F32: unsort_of<float>(rows, row_stride, cols, w, pos, tokens, top_k, y, stream); break;
+    case KTMI_F16: unsort_of<_Float16>(rows, row_stride, cols, w, pos, tokens, top_k, y, stream); break;
+    default: unsort_of<__bf16>(rows, row_stride, cols, w, pos, tokens, top_k, y, stream); break;
+  }
+  KTMI_HIP_TRY(hipGetLastError());
+  return KTMI_OK;
+}
+
+int launch_moe_unsort_grad(const void* dy, int64_t dy_stride, const void* rows, int64_t row_stride, int dtype,
+                           int64_t cols, const float* w, const int32_t* pos, int64_t tokens, int64_t top_k, void* drows,
+                           float* dw, hipStream_t stream) {
+  switch (dtype) {
+    case KTMI_F32:
+      unsort_grad_of<float>(dy, dy_stride, rows, row_stride, cols, w, pos, tokens, top_k, drows, dw, stream);
+      break;
+    case KTMI_F16:
+      unsort_grad_of<_Float16>(dy, dy_stride, rows, row_stride, cols, w, pos, tokens, top_k, drows, dw, stream);
+      break;
+    default: unsort_grad_of<__bf16>(dy, dy_stride, rows, row_stride, cols, w, pos, tokens, top_k, drows, dw, stream); break;
+  }
+  KTMI_HIP_TRY(hipGetLastError());
+  return KTMI_OK;
+}
+
+}  // namespace ktmi

@@ -1,0 +1,369 @@
+"""Products with 4-bit weights and group scales (kt_w4_vec).
+
+Most cases use small integers for x and powers of two for the scales: every product and partial sum
+is then exact in fp32 whatever the order of the sums, so the only rounding is the last one and the
+outputs have to be equal bit for bit. Others use general values against 64 bits."""
+import math
+
+import pytest
+import torch
+
+import kt_prefill_lend_amd.kt_w4_vec as W
+from kt_prefill_lend_amd import _lib
+
+gpu = pytest.mark.gpu
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def groups_of(K, G):
+    return -(-K // G)
+
+
+def make_weights(lead, N, K, G, zeros, sdtype, seed, dev, exact=True):
+    g = torch.Generator().manual_seed(seed)
+    q = torch.randint(0, 256, (*lead, N, (K + 1) // 2), generator=g, dtype=torch.uint8)
+    shape = (*lead, N, groups_of(K, G))
+    s = 2.0 ** torch.randint(-3, 1, shape, generator=g).float() if exact else torch.randn(shape, generator=g) * 0.01
+    z = torch.randint(0, 16, shape, generator=g, dtype=torch.uint8) if zeros else None
+    return q.to(dev), s.to(sdtype).to(dev), None if z is None else z.to(dev)
+
+
+def make_x(T, K, dtype, seed, dev, exact=True):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randint(-2, 3, (T, K), generator=g).float() if exact else torch.randn((T, K), generator=g)
+    return x.to(dtype).to(dev)
+
+
+def matrix(q, s, z, G, K):
+    """(the weights, their size (code + zero point) * scale) in 64 bits."""
+    v = torch.stack([q & 15, q >> 4], -1).flatten(-2)[..., :K].double()
+    at = torch.arange(K, device=q.device) // G
+    zz = torch.full_like(v, 8.0) if z is None else z.double()[..., at]
+    sc = s.double()[..., at]
+    return (v - zz) * sc, (v + zz) * sc.abs()
+
+
+def routed(x, q, s, z, G, ids, top_k):
+    """y [R, N] and the sums of the terms' sizes, in 64 bits."""
+    K = x.shape[1]
+    y = torch.zeros((ids.numel(), q.shape[1]), dtype=torch.float64, device=x.device)
+    size = torch.zeros_like(y)
+    xd = x.double()
+    for e in range(q.shape[0]):
+        r = (ids == e).nonzero().reshape(-1)
+        if r.numel():
+            w, m = matrix(q[e], s[e], None if z is None else z[e], G, K)
+            y[r] = xd[r // top_k] @ w.t()
+            size[r] = xd[r // top_k].abs() @ m.t()
+    return y, size
+
+
+def same(got, want64):
+    """got is the exact result rounded once to its type (exact in fp32 before that)."""
+    assert torch.equal(got, want64.float().to(got.dtype)), (got.double() - want64).abs().max()
+
+
+# tokens, N, K, group
+SHAPES = [
+    (1, 1, 1, 32), (1, 3, 2, 32), (2, 17, 31, 64), (3, 16, 32, 32), (1, 64, 128, 128), (4, 33, 96, 32), (5, 65, 130, 64),
+    (1, 515, 1111, 128), (16, 48, 256, 32), (17, 80, 192, 64), (33, 16, 640, 128), (64, 100, 513, 32), (65, 31, 384, 128),
+    (1, 256, 2048, 128), (7, 40, 1024, 1024), (9, 24, 1000, 1000), (3, 20, 520, 4096), (2, 130, 4096, 256), (130, 70, 288, 32),
+]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("T,N,K,G", SHAPES)
+def test_dense_exact(dev, T, N, K, G, zeros, dtype):
+    q, s, z = make_weights((), N, K, G, zeros, dtype, N + K, dev)
+    x = make_x(T, K, dtype, T, dev)
+    same(W.w4_vec(x, q, s, z, G), x.double() @ matrix(q, s, z, G, K)[0].t())
+
+
+def routes(T, k, E, cold, seed, dev):
+    g = torch.Generator().manual_seed(seed)
+    ids = torch.randint(0, E, (T * k,), generator=g, dtype=torch.int32)
+    ids[torch.rand(T * k, generator=g) < cold] = -1
+    return ids.to(dev)
+
+
+# tokens, top_k, experts, N, K, group, share of routes without an expert
+ROUTED = [
+    (1, 1, 1, 5, 64, 32, 0.0), (1, 8, 40, 64, 256, 128, 0.3), (5, 3, 7, 72, 130, 64, 0.2), (13, 10, 9, 48, 384, 128, 0.4),
+    (64, 8, 3, 33, 160, 32, 0.1), (40, 8, 300, 16, 96, 32, 0.0), (6, 2, 4, 20, 77, 64, 1.0),
+    # more routes than a window's: past 1024, and one expert with most of them
+    (260, 4, 5, 24, 64, 32, 0.1), (1100, 1, 2, 17, 40, 64, 0.0),
+]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("T,k,E,N,K,G,cold", ROUTED)
+def test_routed_exact(dev, T, k, E, N, K, G, cold, zeros, dtype):
+    q, s, z = make_weights((E,), N, K, G, zeros, dtype, N + K, dev)
+    x, ids = make_x(T, K, dtype, T, dev), routes(T, k, E, cold, T, dev)
+    y = W.moe_w4_vec(x, q, s, ids, k, z, G)
+    same(y, routed(x, q, s, z, G, ids, k)[0])
+    assert (y[ids < 0] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("counts,tail,N,K,G", [
+    ([1], 0, 5, 64, 32), ([0, 3, 0, 0, 17, 1, 0], 4, 72, 384, 128), ([0, 0, 0], 7, 9, 96, 64), ([70, 0, 33], 0, 40, 130, 64),
+    ([5] * 60, 3, 16, 96, 32), ([300, 2], 1, 24, 256, 128), ([0] * 500 + [2, 1], 2, 33, 64, 32)])
+def test_sorted_exact(dev, counts, tail, N, K, G, zeros, dtype):
+    E, R = len(counts), sum(counts) + tail
+    q, s, z = make_weights((E,), N, K, G, zeros, dtype, N + K, dev)
+    ids = torch.cat([torch.full((n,), e) for e, n in enumerate(counts)] + [torch.full((tail,), -1)]).to(dev)
+    offsets = torch.tensor([0] + counts).cumsum(0).to(torch.int32).to(dev)
+    x = make_x(R, K, dtype, 5, dev)
+    y = W.moe_w4_sorted(x, q, s, offsets, z, G)
+    same(y, routed(x, q, s, z, G, ids, 1)[0])
+    assert (y[R - tail:] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sdtype", DTYPES)
+@pytest.mark.parametrize("T,N,K,G,zeros", [(1, 64, 2048, 128, False), (3, 48, 1000, 64, True), (24, 32, 512, 32, True)])
+def test_general_values(dev, T, N, K, G, zeros, dtype, sdtype):
+    """Against 64 bits. Every element: K products and the zero points' share of them, each addition off by
+    2^-24 of a partial sum at most, then the group's scale and sum, then the last rounding. And as a
+    whole: a chain of 2 K roundings of independent sign, of partial sums at most about three times the
+    final ones' size, is off by 3 sqrt(2 K) 2^-24 of it."""
+    q, s, z = make_weights((), N, K, G, zeros, sdtype, 3, dev, exact=False)
+    x = make_x(T, K, dtype, 4, dev, exact=False)
+    w, m = matrix(q, s, z, G, K)
+    want, size = x.double() @ w.t(), x.double().abs() @ m.t()
+    got = W.w4_vec(x, q, s, z, G).double()
+    u = torch.finfo(dtype).eps / 2
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0  # half a step below f16's normal numbers
+    assert ((got - want).abs() <= u * want.abs() + (1 + u) * (2 * K + 4) * 2.0 ** -24 * size + tiny).all()
+    assert (got - want).norm() <= (u + 3 * math.sqrt(2 * K) * 2.0 ** -24) * want.norm()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_every_code_and_zero_point(dev, dtype):
+    """Each of the 16 codes against each of the 256 zero points a byte can hold, at every place of a group."""
+    N, K, G = 256, 32, 32
+    q = torch.arange(N * 16, dtype=torch.int64).reshape(N, 16)
+    q = ((q * 7 + q // 16) % 256).to(torch.uint8).to(dev)
+    z = torch.arange(256, dtype=torch.uint8).reshape(N, 1).to(dev)
+    s = torch.ones((N, 1), dtype=dtype, device=dev)
+    x = torch.eye(K).to(dtype).to(dev)
+    y = W.w4_vec(x, q, s, z, G)
+    same(y, matrix(q, s, z, G, K)[0].t())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_infinities_and_nan(dev, dtype, bad):
+    """A value of x that is not finite gives what the products' plain sum gives (an infinity where the weight
+    is not zero, NaN where it is), in its own row alone."""
+    T, N, K, G = 5, 40, 384, 64
+    q, s, z = make_weights((), N, K, G, True, dtype, 3, dev)
+    x = make_x(T, K, dtype, 4, dev)
+    clean = W.w4_vec(x, q, s, z, G)
+    x[2, 77] = bad
+    got = W.w4_vec(x, q, s, z, G)
+    assert torch.equal(got[[0, 1, 3, 4]], clean[[0, 1, 3, 4]])
+    weight = matrix(q, s, z, G, K)[0][:, 77]
+    want = weight * bad
+    assert (weight == 0).any() and (weight > 0).any() and (weight < 0).any()
+    assert torch.equal(got[2].double().isnan(), want.isnan())
+    assert torch.equal(got[2].double()[~want.isnan()], want[~want.isnan()])
+    # the same row as one of an expert's routes
+    ids = torch.zeros(T, dtype=torch.int32, device=dev)
+    again = W.moe_w4_vec(x, q[None], s[None], ids, 1, z[None], G)
+    assert torch.equal(again.nan_to_num(7.0), got.nan_to_num(7.0))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_large_and_small_values(dev, dtype):
+    """Values near the ends of x's range keep their bits: each output is one product."""
+    f = torch.finfo(dtype)
+    K = 64
+    vals = torch.tensor([f.max / 8, -f.max / 16, f.tiny, -f.tiny * 1.5, f.tiny / 2, 1.0, f.eps, 1 + f.eps], dtype=dtype)
+    x = torch.zeros((8, K), dtype=dtype)
+    x[torch.arange(8), torch.arange(8) * 7] = vals
+    x = x.to(dev)
+    q = torch.full((4, K // 2), 0x99, dtype=torch.uint8, device=dev)  # code 9, weight 1
+    q[1] = 0x77  # weight -1
+    q[2] = 0x88  # weight 0
+    q[3] = 0xCC  # weight 4
+    s = torch.ones((4, 1), dtype=dtype, device=dev)
+    y = W.w4_vec(x, q, s, None, 64)
+    want = (vals.double()[:, None] * torch.tensor([1.0, -1.0, 0.0, 4.0], dtype=torch.float64)).to(dev)
+    assert torch.equal(y.double(), want)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_strides_and_alignment(dev, dtype):
+    T, k, E, N, K, G = 6, 2, 5, 37, 256, 64
+    q, s, z = make_weights((E,), N, K, G, True, dtype, 8, dev)
+    x, ids = make_x(T, K, dtype, 9, dev), routes(T, k, E, 0.2, 9, dev)
+    want = W.moe_w4_vec(x, q, s, ids, k, z, G)
+    same(want, routed(x, q, s, z, G, ids, k)[0])
+    wide = torch.full((T, K + 9), float("nan"), dtype=dtype, device=dev)
+    wide[:, 3:K + 3] = x
+    odd = torch.empty(q.numel() + 1, dtype=torch.uint8, device=dev)[1:]
+    odd.copy_(q.reshape(-1))
+    odd_s = torch.empty(s.numel() + 1, dtype=dtype, device=dev)[1:]
+    odd_s.copy_(s.reshape(-1))
+    odd_z = torch.empty(z.numel() + 1, dtype=torch.uint8, device=dev)[1:]
+    odd_z.copy_(z.reshape(-1))
+    assert torch.equal(W.moe_w4_vec(wide[:, 3:K + 3], odd.view(q.shape), odd_s.view(s.shape), ids, k, odd_z.view(z.shape), G), want)
+    assert torch.equal(W.moe_w4_vec(x, q.view(torch.int32), s, ids, k, z, G), want)
+    part = torch.cat([q, q], 1)[:, :N]  # experts apart
+    assert not part.is_contiguous()
+    assert torch.equal(W.moe_w4_vec(x.t().contiguous().t(), part, s, torch.stack([ids, ids], 1)[:, 0], k, z, G), want)
+    one = make_x(1, K, dtype, 3, dev).expand(T, K)
+    same(W.moe_w4_vec(one, q, s, ids, k, z, G), routed(one, q, s, z, G, ids, k)[0])
+
+
+@gpu
+def test_ids_and_offsets_outside_the_range(dev):
+    E, N, K, G = 3, 20, 64, 32
+    q, s, z = make_weights((E,), N, K, G, False, torch.bfloat16, 8, dev)
+    x = make_x(6, K, torch.bfloat16, 9, dev)
+    ids = torch.tensor([0, 3, 2, -1, 2 ** 31 - 1, -2 ** 31], dtype=torch.int32, device=dev)
+    y = W.moe_w4_vec(x, q, s, ids, 1, z, G)
+    same(y, routed(x, q, s, z, G, ids, 1)[0])
+    # segments past the rows are cut at them
+    offsets = torch.tensor([-5, 2, 4, 900], dtype=torch.int32, device=dev)
+    y = W.moe_w4_sorted(x, q, s, offsets, z, G)
+    same(y, routed(x, q, s, z, G, torch.tensor([0, 0, 1, 1, 2, 2], device=dev), 1)[0])
+
+
+@gpu
+def test_no_rows(dev):
+    q, s, z = make_weights((2,), 8, 64, 32, False, torch.bfloat16, 8, dev)
+    x = torch.empty((0, 64), dtype=torch.bfloat16, device=dev)
+    ids = torch.empty((0,), dtype=torch.int32, device=dev)
+    assert W.w4_vec(x, q[0], s[0], None, 32).shape == (0, 8)
+    assert W.moe_w4_vec(x, q, s, ids, 4, None, 32).shape == (0, 8)
+    assert W.moe_w4_sorted(x, q, s, torch.zeros(3, dtype=torch.int32, device=dev), None, 32).shape == (0, 8)
+
+
+@gpu
+def test_codes_past_32_bits(dev):
+    """A matrix behind more than 4 GiB of codes."""
+    E, N, K, G = 5, 32768, 65536, 65536
+    q = torch.zeros((E, N, K // 2), dtype=torch.uint8, device=dev)
+    q[4] = 0x99
+    q[4, N - 1, K // 2 - 1] = 0xA9
+    s = torch.ones((E, N, 1), dtype=torch.float32, device=dev)
+    x = torch.zeros((2, K), dtype=torch.float32, device=dev)
+    x[0, :64], x[0, K - 1], x[1, 5] = 1.0, 1.0, 3.0
+    ids = torch.tensor([4, 4], dtype=torch.int32, device=dev)
+    for y in (W.moe_w4_vec(x, q, s, ids, 1, None, G),
+              W.moe_w4_sorted(x, q, s, torch.tensor([0, 0, 0, 0, 0, 2], dtype=torch.int32, device=dev), None, G)):
+        assert (y[0, :N - 1] == 65).all() and y[0, N - 1] == 66 and (y[1] == 3).all()
+
+
+@gpu
+@pytest.mark.parametrize("T", [1, 20])
+def test_graphs_and_streams(dev, T):
+    """Two captured graphs replayed between eager calls, and calls on two streams at once."""
+    k, E, N, K, G = 4, 12, 80, 512, 128
+    q, s, z = make_weights((E,), N, K, G, True, torch.bfloat16, 8, dev, exact=False)
+    x = [make_x(T, K, torch.bfloat16, i, dev, exact=False) for i in range(2)]
+    ids = [routes(T, k, E, 0.2, i, dev) for i in range(2)]
+
+    def step(i):
+        return [W.moe_w4_vec(x[i], q, s, ids[i], k, z, G), W.w4_vec(x[i], q[i], s[i], z[i], G)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(0)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step(i))
+        graphs.append(g)
+    for turn in range(4):
+        for i in range(2):
+            x[i].copy_(make_x(T, K, torch.bfloat16, 10 + turn + i, dev, exact=False))
+            ids[i].copy_(routes(T, k, E, 0.2 * turn, 20 + turn + i, dev))
+        for i in ((0, 1) if turn % 2 else (1, 0)):
+            graphs[i].replay()
+        for i in range(2):
+            assert all(torch.equal(a, b) for a, b in zip(outs[i], step(i)))
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        a = step(0)
+    b = step(1)
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, r) for p, r in zip(a + b, step(0) + step(1)))
+
+
+# ---------------------------------------------------------------- refusals (no GPU)
+
+def test_refusals():
+    x, q, s = torch.zeros(2, 64), torch.zeros(3, 32, dtype=torch.uint8), torch.zeros(3, 2)
+    z = torch.zeros(3, 2, dtype=torch.uint8)
+    for args, error in [
+            ((x.double(), q, s, z, 32), TypeError), ((x, q.long(), s, z, 32), TypeError), ((x, q, s.double(), z, 32), TypeError),
+            ((x, q, s, z.int(), 32), TypeError), ((x[0], q, s, z, 32), ValueError), ((x[:, :63], q[:, :31], s, z, 32), ValueError),
+            ((x, q, s, z, 48), ValueError), ((x, q, s, z, 0), ValueError), ((x, q, s, z, 63), ValueError),
+            ((x, q, s[:, :1], z, 32), ValueError), ((x, q, s, z[:2], 32), ValueError), ((x, q[None], s, z, 32), ValueError),
+            ((x, q, s, z, 64), ValueError), ((x.requires_grad_(True), q, s, z, 32), RuntimeError),
+            ((x.detach()[:, :60], torch.zeros(3, 8, dtype=torch.int32), s, z, 32), ValueError),
+            ((torch.zeros(2, 64), q, s, z, 32), ValueError)]:  # the last: not on the GPU
+        with pytest.raises(error, match="w4_vec"):
+            W.w4_vec(*args)
+    x, qe, se = torch.zeros(2, 64), q[None], s[None]
+    ids = torch.zeros(4, dtype=torch.int32)
+    for args, error in [((x, qe, se, ids.long(), 2), TypeError), ((x, qe, se, ids, 3), ValueError), ((x, qe, se, ids, 0), ValueError),
+                        ((x, q, s, ids, 2), ValueError), ((x, qe[:0], se[:0], ids, 2), ValueError), ((x, qe, se, ids, 2), ValueError)]:
+        with pytest.raises(error, match="moe_w4_vec"):
+            W.moe_w4_vec(*args, group_size=32)
+    off = torch.zeros(2, dtype=torch.int32)
+    for args, error in [((x, qe, se, off.long()), TypeError), ((x, qe, se, off[:1]), ValueError), ((x, qe, se, off[None]), ValueError),
+                        ((x, qe, se, off), ValueError)]:
+        with pytest.raises(error, match="moe_w4_sorted"):
+            W.moe_w4_sorted(*args, group_size=32)
+
+
+def test_c_refusals():
+    """Argument errors of the entry points come before any device work (the pointers are never read)."""
+    L = _lib.lib()
+    p = 4096
+
+    def dense(x=p, dt=2, xs=64, K=64, q=p, s=p, st=2, z=0, G=32, N=8, T=2, y=p):
+        return L.ktmi_w4_vec(x, dt, xs, K, q, s, st, z, G, N, T, y, 0)
+
+    for kw in [dict(dt=3), dict(st=5), dict(K=0), dict(N=0), dict(T=-1), dict(G=48), dict(G=0), dict(G=63), dict(x=0), dict(q=0),
+               dict(s=0), dict(y=0), dict(x=p + 1), dict(s=p + 1), dict(y=p + 1), dict(xs=63), dict(K=1 << 25, xs=1 << 25)]:
+        assert dense(**kw) == -1 and b"w4_vec" in L.ktmi_last_error(), kw
+    assert dense(T=0) == 0
+
+    def routed_(E=4, ids=p, k=2, T=2, ws=p, n=1 << 30, **kw):
+        a = dict(x=p, dt=2, xs=64, K=64, q=p, s=p, st=2, z=0, G=32, N=8, y=p) | kw
+        return L.ktmi_moe_w4_vec(a["x"], a["dt"], a["xs"], a["K"], a["q"], a["s"], a["st"], a["z"], a["G"], a["N"], E, ids, k, T,
+                                 a["y"], ws, n, 0)
+
+    for kw in [dict(E=0), dict(E=W.MAX_EXPERTS + 1), dict(ids=0), dict(k=0), dict(k=65536), dict(T=-1), dict(T=1 << 31), dict(G=33)]:
+        assert routed_(**kw) == -1 and b"moe_w4_vec" in L.ktmi_last_error(), kw
+    need = L.ktmi_moe_w4_vec_workspace(100000, 8, 4)
+    if need:
+        assert routed_(T=100000, k=8, n=need - 1) == -4 and routed_(T=100000, k=8, ws=0) == -4
+    assert routed_(T=0) == 0
+
+    def sorted_(E=4, off=p, R=2, N=8, y=p):
+        return L.ktmi_moe_w4_sorted(p, 2, 64, 64, p, p, 2, 0, 32, N, E, off, R, y, 0)
+
+    for kw in [dict(E=0), dict(off=0), dict(R=-1), dict(N=0), dict(y=0)]:
+        assert sorted_(**kw) == -1 and b"moe_w4_sorted" in L.ktmi_last_error(), kw
+    assert sorted_(R=0) == 0
