@@ -161,7 +161,7 @@ int ktmi_moe_w4_vec(const void* x, int x_dtype, int64_t x_stride, int64_t cols, 
                     const int32_t* ids, int64_t top_k, int64_t tokens, void* y, void* workspace, int64_t ws_bytes,
                     void* stream);
 /* rows sorted by expert (ktmi_moe_sort): y[p] = W[e] x[p] for offsets[e] <= p < offsets[e+1],
- * y [n_rows, rows]; rows past offsets[n_experts] give zero rows. offsets must ascend within
+ * y [n_rows, rows]; rows in no segment give zero rows. offsets must ascend within
  * [0, n_rows]; values outside are clamped to it. */
 int ktmi_moe_w4_sorted(const void* x, int x_dtype, int64_t x_stride, int64_t cols, const void* codes,
                        const void* scales, int scale_dtype, const void* zeros, int64_t group, int64_t rows,

@@ -253,7 +253,7 @@ int ktmi_w4_vec(const void* x, int x_dtype, int64_t x_stride, int64_t cols, cons
                 int scale_dtype, const void* zeros, int64_t group, int64_t rows, int64_t tokens, void* y, void* stream) {
   g_err[0] = 0;
   const W4Args a = {x, x_stride, cols, (const uint8_t*)codes, scales, (const uint8_t*)zeros, group, rows, 1, nullptr, nullptr,
-                    1, tokens, y, nullptr, x_dtype, scale_dtype};
+                    1, tokens, y, nullptr, x_dtype, scale_dtype, nullptr};
   int rc = check_w4("w4_vec", a, tokens);
   if (rc || tokens == 0) return rc;
   KTMI_REQUIRE(tokens <= 0x7FFFFFFF, KTMI_EINVAL, "w4_vec: %lld rows (below 2^31)", (long long)tokens);
@@ -273,7 +273,7 @@ int ktmi_moe_w4_vec(const void* x, int x_dtype, int64_t x_stride, int64_t cols, 
   KTMI_REQUIRE(tokens >= 0 && top_k > 0 && top_k <= 65535 && tokens <= 0x7FFFFFFF / top_k, KTMI_EINVAL,
                "moe_w4_vec: %lld tokens x top-%lld (at most 65535 a token, 2^31 in all)", (long long)tokens, (long long)top_k);
   const W4Args a = {x, x_stride, cols, (const uint8_t*)codes, scales, (const uint8_t*)zeros, group, rows, n_experts, ids,
-                    nullptr, top_k, tokens * top_k, y, (uint8_t*)workspace, x_dtype, scale_dtype};
+                    nullptr, top_k, tokens * top_k, y, (uint8_t*)workspace, x_dtype, scale_dtype, nullptr};
   int rc = check_w4("moe_w4_vec", a, tokens);
   if (rc || tokens == 0) return rc;
   KTMI_REQUIRE(ids, KTMI_EINVAL, "moe_w4_vec: null pointer");
@@ -288,7 +288,7 @@ int ktmi_moe_w4_sorted(const void* x, int x_dtype, int64_t x_stride, int64_t col
                        int64_t n_experts, const int32_t* offsets, int64_t n_rows, void* y, void* stream) {
   g_err[0] = 0;
   const W4Args a = {x, x_stride, cols, (const uint8_t*)codes, scales, (const uint8_t*)zeros, group, rows, n_experts, nullptr,
-                    offsets, 1, n_rows, y, nullptr, x_dtype, scale_dtype};
+                    offsets, 1, n_rows, y, nullptr, x_dtype, scale_dtype, nullptr};
   int rc = check_w4("moe_w4_sorted", a, n_rows);
   if (rc || n_rows == 0) return rc;
   KTMI_REQUIRE(offsets, KTMI_EINVAL, "moe_w4_sorted: null pointer");
