@@ -30,7 +30,9 @@ constexpr int W4_STEP = 128;           // columns of a step: 16 bytes of codes a
 constexpr int W4_RING = 8;             // steps of codes in flight a wave, a turn of the ring
 constexpr int W4_IDS = 64;             // routes whose ids a wave holds one a lane
 constexpr int W4_VMCNT0 = 0xF70;       // s_waitcnt operand: vector memory loads only
-constexpr int W4_X_BYTES = 64 << 10;   // LDS for a stage's activations, about
+constexpr int W4_X_BYTES = 64 << 10;   // LDS for a stage's activations, about: two blocks a CU
+constexpr int W4_CU_LDS = 160 << 10;
+constexpr int W4_X_SPLIT = 112 << 10;  // where the blocks are few: one a CU
 
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
@@ -270,31 +272,24 @@ __global__ __launch_bounds__(64 * KS * WR) void w4_mfma_kernel(W4Args a, W4Plan 
   rest = rest < 0x7FFFFFFF / SS ? rest : 0x7FFFFFFF / SS;
   // the lane's row of tile t (past the last row: the last)
   auto row_of = [&](int t) { return t * RB + rb < rows_left ? t * RB + rb : rows_left - 1; };
-  // 16 bytes of codes of step s of the row at byte `at`, those past the row's end replaced by its last ones
-  auto load_codes = [&](int at, int s, bool in) {
-    const int b = 64 * s + 16 * g;
-    return __builtin_amdgcn_raw_buffer_load_b128(buffer(codes, in ? rows_left * (int64_t)half : 0),
-                                                 at + (b < half - 16 ? b : half - 16), 0, 0);
-  };
-  const float steps_inv = (float)W4_STEP / (float)a.group;  // SPS = 1: the group of step s is s / (group / 128)
-  auto group_of = [&](int s) { return SPS == 1 ? (int)(((float)s + 0.5f) * steps_inv) : SPS * s; };
-  auto scale_bits = [&](uint32_t u) {
-    if constexpr (S4) return __builtin_bit_cast(float, u);
-    return a.scale_dtype == KTMI_F16 ? half_bits_to_float((uint16_t)u) : bf2f((uint16_t)u);
-  };
+  const int total = (cols + W4_STEP - 1) / W4_STEP;  // steps of a row
+  // Codes past a row's end meet zeros of x: the next row's, or the zeros that a buffer's end gives for
+  // whole words. Rows that do not end with a word take the plain loop, which loads up to their end.
+  const bool ragged = half & 3;
+  auto group_of = [&](int s) { return SPS > 1 ? SPS * s : a.group == W4_STEP ? s : s / (int)(a.group / W4_STEP); };
   auto pack_zero = [&](uint32_t z) { return O::pack(-(float)z, -(float)z); };
-  // The scales and zero points of a turn's W4_RING steps from group i0 of the row with `at` scales before
-  // it, packed as in memory. Read 16 bytes at a time, past the row's end too, where the turn of the wave's
-  // last row ends inside the weights; one by one where not.
+  // The scales and zero points of the W4_RING steps from s on of the row with `at` scales before it,
+  // packed as in memory. Where the turn of the wave's last row ends inside the weights, 16 bytes at a
+  // time, past the row's end too; there, and for groups of several steps, one by one.
   constexpr int TURN = W4_RING * SPS, PER = 4 / SS;
   struct Turn {
     uint32_t s[TURN / PER], z[TURN / 4];
   };
-  auto load_turn = [&](int at, int last_at, int i0, bool in) {
+  auto load_turn = [&](int at, int last_at, int s, bool in) {
     Turn t;
     const auto sb = buffer(scales, in ? rest * SS : 0), zb = buffer(zeros, in ? rest : 0);
-    const int i = at + i0;
-    if (last_at + i0 + TURN <= rest) {  // uniform
+    if ((SPS > 1 || a.group == W4_STEP) && last_at + SPS * s + TURN <= rest) {  // uniform
+      const int i = at + SPS * s;
 #pragma unroll
       for (int j = 0; j < TURN / PER; j += 4) {
         const u32x4_t v = __builtin_amdgcn_raw_buffer_load_b128(sb, SS * i + 4 * j, 0, 0);
@@ -311,45 +306,35 @@ __global__ __launch_bounds__(64 * KS * WR) void w4_mfma_kernel(W4Args a, W4Plan 
     } else {
 #pragma unroll
       for (int j = 0; j < TURN; ++j) {
+        const int i = at + group_of(s + j / SPS) + j % SPS;
         if constexpr (S4) {
-          t.s[j] = __builtin_amdgcn_raw_buffer_load_b32(sb, 4 * (i + j), 0, 0);
+          t.s[j] = __builtin_amdgcn_raw_buffer_load_b32(sb, 4 * i, 0, 0);
         } else {
-          const uint32_t u = __builtin_amdgcn_raw_buffer_load_b16(sb, 2 * (i + j), 0, 0);
+          const uint32_t u = __builtin_amdgcn_raw_buffer_load_b16(sb, 2 * i, 0, 0);
           t.s[j / 2] = j % 2 ? t.s[j / 2] | u << 16 : u;
         }
         if constexpr (Z) {
-          const uint32_t u = __builtin_amdgcn_raw_buffer_load_b8(zb, i + j, 0, 0);
+          const uint32_t u = __builtin_amdgcn_raw_buffer_load_b8(zb, i, 0, 0);
           t.z[j / 4] = j % 4 ? t.z[j / 4] | u << (8 * (j % 4)) : u;
         }
       }
     }
     return t;
   };
-  // scales in fp32 (0 past the row's last) and packed -z of step u of a turn that begins at step s
-  auto scales_of = [&](const Turn& t, int s, int u, float (&sc)[SPS], uint32_t (&zz)[SPS]) {
-    if (SPS == 1 && a.group != W4_STEP) {  // uniform: a group of several steps
-      const int j = group_of(s + u) - group_of(s);
-      uint32_t v = t.s[0], z = Z ? t.z[0] : 0;
+  // element j of a turn in fp32; of a turn that reaches past the row's last group, 0 for those past it
+  auto scale_of = [&](const Turn& t, int j) {
+    const uint32_t u = t.s[j / PER];
+    if constexpr (S4) return __builtin_bit_cast(float, u);
+    const uint16_t h = (uint16_t)(u >> 16 * (j % PER));
+    return a.scale_dtype == KTMI_F16 ? half_bits_to_float(h) : bf2f(h);
+  };
+  auto drop_past = [&](Turn& t, int s) {
 #pragma unroll
-      for (int q = 0; q < TURN; ++q) {
-        if (j == q) {
-          v = PER == 2 ? t.s[q / PER] >> 16 * (q % PER) : t.s[q / PER];
-          if (Z) z = t.z[q / 4] >> 8 * (q % 4);
-        }
-      }
-      sc[0] = scale_bits(PER == 2 ? v & 0xFFFFu : v);
-      zz[0] = Z ? pack_zero(z & 255u) : neg8;
-    } else {
-#pragma unroll
-      for (int q = 0; q < SPS; ++q) {
-        const int j = SPS * u + q;
-        sc[q] = scale_bits(PER == 2 ? (t.s[j / PER] >> 16 * (j % PER)) & 0xFFFFu : t.s[j / PER]);
-        zz[q] = Z ? pack_zero((t.z[j / 4] >> 8 * (j % 4)) & 255u) : neg8;
-      }
+    for (int j = 0; j < TURN; ++j) {
+      const int step = s + j / SPS;
+      if (step >= total || group_of(step) + j % SPS >= groups)  // uniform
+        t.s[j / PER] &= PER == 1 ? 0u : j % 2 ? 0xFFFFu : 0xFFFF0000u;
     }
-    if (group_of(s + u) + SPS > groups)  // uniform
-#pragma unroll
-      for (int q = 0; q < SPS; ++q) sc[q] = group_of(s + u) + q < groups ? sc[q] : 0.0f;
   };
   // steps a wave of a stage: all, or as many as the activations' room takes
   int per_stage = ((p.x_bytes / (PLANES * m) - 16) / (2 * W4_STEP * KS));
@@ -453,13 +438,9 @@ __global__ __launch_bounds__(64 * KS * WR) void w4_mfma_kernel(W4Args a, W4Plan 
 
   f32x4_t acc[MT];
   // step s, the at-th of the stage
-  auto compute = [&](auto plain, u32x4_t raw, const float (&scale)[SPS], const uint32_t (&zz)[SPS], int s, int at) {
+  auto compute = [&](auto plain, const u32x4_t& raw, const float* scale, const uint32_t (&zz)[SPS], int at) {
     constexpr bool PLAIN = decltype(plain)::value;
     constexpr int J = 4 / SPS;
-    if ((half & 15) && 64 * s + 64 > half) {  // uniform: what a lane loaded may end with the row
-      const int over = 64 * s + 16 * g - (half - 16);
-      raw = shift_down(raw, over < 0 ? 0 : over < 15 ? over : 15);
-    }
     uint32_t w[4] = {raw[0], raw[1], raw[2], raw[3]};
     regroup<SPS>(w);
 #pragma unroll
@@ -475,7 +456,7 @@ __global__ __launch_bounds__(64 * KS * WR) void w4_mfma_kernel(W4Args a, W4Plan 
       }
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
-        if (t < mg) {  // uniform
+        if (t == 0 || t < mg) {  // uniform
           f32x4_t d = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
           for (int j = 0; j < J; ++j)
@@ -487,6 +468,9 @@ __global__ __launch_bounds__(64 * KS * WR) void w4_mfma_kernel(W4Args a, W4Plan 
             }
 #pragma unroll
           for (int i = 0; i < 4; ++i) acc[t][i] = fmaf(scale[sub], d[i], acc[t][i]);
+          // the sums are taken here, in the block of their MFMAs: moved past the branch behind it, the
+          // compiler left out the wait states between an MFMA and the reader of its result
+          asm volatile("" : "+v"(acc[t]));
         }
       }
     }
@@ -524,28 +508,26 @@ __global__ __launch_bounds__(64 * KS * WR) void w4_mfma_kernel(W4Args a, W4Plan 
       // the activations' loads, the first steps', then the activations' stores
       const Batch b = fetch(first * W4_STEP, threadIdx.x);
       __builtin_amdgcn_sched_barrier(0);  // in this order
-      // the ring runs on through the tiles, each padded to whole turns by steps that load nothing
+      const int valid = n < total - s0 ? n : total - s0;  // the wave's steps that the rows have
+      // the ring runs on from turn to turn and tile to tile; in a turn's loads past its valid steps are
+      // others' codes, which no sum takes
       u32x4_t ring[W4_RING];
-      int next = 0, next_tile = 0, next_at = row_of(0) * half;
-      auto advance = [&]() {
-        const u32x4_t v = load_codes(next_at, s0 + next, next < n && next_tile < tiles);
-        if (++next >= n && next % W4_RING == 0) {  // uniform
-          next = 0;
-          next_at = row_of(++next_tile) * half;
-        }
-        return v;
+      auto codes_at = [&](int t, int i) { return row_of(t) * half + 64 * (s0 + i) + 16 * g; };
+      auto load_step = [&](int at, int u, bool in) {
+        return __builtin_amdgcn_raw_buffer_load_b128(buffer(codes, in ? rows_left * (int64_t)half : 0), at + 64 * u, 0, 0);
       };
       auto turn_of = [&](int t, int i) {  // from step i of tile t; past the tile's end: the next tile's first
         const bool on = i >= n;
         t += on;
         const int last = t * RB + RB < rows_left ? t * RB + RB - 1 : rows_left - 1;
-        return load_turn(row_of(t) * groups, last * groups, group_of(s0 + (on ? 0 : i)), t < tiles);
+        return load_turn(row_of(t) * groups, last * groups, s0 + (on ? 0 : i), t < tiles);
       };
       Turn turn;
       if constexpr (!PLAIN) {
         turn = turn_of(0, 0);
+        const int at = codes_at(0, 0);
 #pragma unroll
-        for (int u = 0; u < W4_RING; ++u) ring[u] = advance();
+        for (int u = 0; u < W4_RING; ++u) ring[u] = load_step(at, u, true);
         __builtin_amdgcn_sched_barrier(0);
       }
       if (i0) __syncthreads();  // every wave is done with the stage before
@@ -553,7 +535,7 @@ __global__ __launch_bounds__(64 * KS * WR) void w4_mfma_kernel(W4Args a, W4Plan 
       __syncthreads();
       for (int t = 0; t < tiles; ++t) {
         if constexpr (PLAIN) {
-          for (int i = 0; i < n; ++i) {
+          for (int i = 0; i < valid; ++i) {
             float sc[SPS];
             uint32_t zz[SPS];
 #pragma unroll
@@ -563,26 +545,41 @@ __global__ __launch_bounds__(64 * KS * WR) void w4_mfma_kernel(W4Args a, W4Plan 
               sc[q] = gr < groups ? scale_as_float(a.scales, a.scale_dtype, at) : 0.0f;
               zz[q] = Z ? pack_zero(gload<uint8_t>(a.zeros + at)) : neg8;
             }
-            compute(plain, load_codes(row_of(t) * half, s0 + i, true), sc, zz, s0 + i, kw * n + i);
+            const int over = 64 * (s0 + i) + 16 * g - (half - 16);  // bytes of the lane's 16 past the row's end
+            u32x4_t raw = load_step(codes_at(t, i) - (over > 0 ? over : 0), 0, true);
+            raw = shift_down(raw, over < 0 ? 0 : over < 15 ? over : 15);
+            compute(plain, raw, sc, zz, kw * n + i);
           }
         } else {
           for (int i = 0; i < n; i += W4_RING) {
-            const Turn now = turn;
+            Turn now = turn;
             turn = turn_of(t, i + W4_RING);
+            const bool last = i + W4_RING >= n;
+            const int at_next = codes_at(t + last, last ? 0 : i + W4_RING);
+            const bool in = t + last < tiles;
+            if (s0 + i + W4_RING >= total) drop_past(now, s0 + i);  // uniform
 #pragma unroll
             for (int u = 0; u < W4_RING; u += 2) {
+              // two steps; the second may be past the wave's last, then with scales of 0
+              if (i + u < valid) {  // uniform
+                const bool both = i + u + 1 < valid;
 #pragma unroll
-              for (int v = u; v < u + 2; ++v)
-                if (i + v < n) {  // uniform
+                for (int v = u; v < u + 2; ++v) {
                   float sc[SPS];
                   uint32_t zz[SPS];
-                  scales_of(now, s0 + i, v, sc, zz);
-                  compute(plain, ring[v], sc, zz, s0 + i + v, kw * n + i + v);
+#pragma unroll
+                  for (int q = 0; q < SPS; ++q) {
+                    const int j = SPS * v + q;
+                    sc[q] = v == u || both ? scale_of(now, j) : 0.0f;
+                    zz[q] = Z ? pack_zero((now.z[j / 4] >> 8 * (j % 4)) & 255u) : neg8;
+                  }
+                  compute(plain, ring[v], sc, zz, kw * n + i + (v == u || both ? v : u));
                 }
+              }
               __builtin_amdgcn_sched_barrier(0);  // the steps' registers take the loads: no copies that wait
               // both halves of each row's 128 bytes at once
-              ring[u] = advance();
-              ring[u + 1] = advance();
+              ring[u] = load_step(at_next, u, in);
+              ring[u + 1] = load_step(at_next, u + 1, in);
             }
           }
         }
@@ -606,7 +603,7 @@ __global__ __launch_bounds__(64 * KS * WR) void w4_mfma_kernel(W4Args a, W4Plan 
     if constexpr (KS > 1) check();
     return __syncthreads_or(bad);
   };
-  if (run(std::false_type{})) run(std::true_type{});
+  if (ragged || run(std::false_type{})) run(std::true_type{});
 
   // the waves' sums over their columns meet in LDS, in the order of the columns' parts
   if constexpr (KS > 1) {
@@ -666,22 +663,25 @@ int launch_as(const W4Args& a, int64_t items, int64_t expected, hipStream_t stre
   constexpr int PLANES = std::is_same<T, float>::value ? 3 : 1, RB = 16 * WR, UNIT = W4_STEP * KS;
   const int64_t tiles = (a.rows + RB - 1) / RB;
   W4Plan p;
-  // row tiles a block: so many that about three blocks a CU are left, whose loads of activations and
-  // searches for their item are then fewer; their codes and scales stay within 2^31 bytes
-  int64_t deep = KS > 1 ? 1 : expected * tiles / 768;
+  p.steps = (int)((a.cols + UNIT - 1) / UNIT);
+  const int64_t rows = a.n_routes < 16 * MT ? a.n_routes : 16 * MT;  // at most, of an item
+  // room for one step of every row; up to the limit, or all columns of every row
+  const int64_t least = PLANES * rows * (2 * UNIT + 16), whole = PLANES * rows * (2 * (int64_t)UNIT * p.steps + 16);
+  const int64_t limit = KS > 1 ? W4_X_SPLIT : W4_X_BYTES;
+  int64_t x_bytes = whole < limit ? whole : limit;
+  if (x_bytes < least) x_bytes = least;
+  if (KS > 1 && x_bytes < (KS - 1) * WR * MT * 64 * 16) x_bytes = (KS - 1) * WR * MT * 64 * 16;
+  p.x_bytes = (int)((x_bytes + 15) / 16 * 16);
+  // row tiles a block: so many that the blocks left are about those that the chip holds at once (three a
+  // CU by their registers, fewer by their LDS), whose loads of activations and searches for their item
+  // are then fewer; their codes and scales stay within 2^31 bytes
+  const int64_t held = W4_CU_LDS / p.x_bytes < 3 ? W4_CU_LDS / p.x_bytes : 3;
+  int64_t deep = KS > 1 ? 1 : expected * tiles / (256 * (held < 1 ? 1 : held));
   const int64_t most = 0x7FFFFFFFll / (RB * ((a.cols + 1) / 2));
   deep = deep > 8 ? 8 : deep;
   deep = deep > most ? most : deep;
   p.deep = (int)(deep < 1 ? 1 : deep);
   p.blocks = (int)((tiles + p.deep - 1) / p.deep);
-  p.steps = (int)((a.cols + UNIT - 1) / UNIT);
-  const int64_t rows = a.n_routes < 16 * MT ? a.n_routes : 16 * MT;  // at most, of an item
-  // room for one step of every row; up to W4_X_BYTES, or all columns of every row
-  const int64_t least = PLANES * rows * (2 * UNIT + 16), whole = PLANES * rows * (2 * (int64_t)UNIT * p.steps + 16);
-  int64_t x_bytes = whole < W4_X_BYTES ? whole : W4_X_BYTES;
-  if (x_bytes < least) x_bytes = least;
-  if (KS > 1 && x_bytes < (KS - 1) * WR * MT * 64 * 16) x_bytes = (KS - 1) * WR * MT * 64 * 16;
-  p.x_bytes = (int)((x_bytes + 15) / 16 * 16);
   const int64_t bytes = p.x_bytes + (KS == 1 && whole > x_bytes ? p.deep * WR * MT * 64 * 16 : 0);
   KTMI_REQUIRE(items * p.blocks <= 0x7FFFFFFF, KTMI_EINVAL, "w4: %lld blocks (below 2^31)", (long long)(items * p.blocks));
   auto kernel = w4_mfma_kernel<T, SPS, S4, Z, MT, KS, WR>;
