@@ -46,6 +46,11 @@ struct W4Args {
 constexpr int W4_LDS_MOST = 128 << 10;
 int64_t w4_workspace(int64_t tokens, int64_t top_k, int64_t n_experts);
 int launch_w4(const W4Args& a, hipStream_t stream);
+int launch_w4_bf16(const W4Args& a, hipStream_t stream);  // by activation type: one pass without a sort
+int launch_w4_f16(const W4Args& a, hipStream_t stream);
+int launch_w4_f32(const W4Args& a, hipStream_t stream);
+constexpr int W4_STEP = 128;  // columns of a step: 16 bytes of codes a lane
+constexpr int W4_IDS = 64;    // routes whose ids a wave holds one a lane
 
 // GEMV over raw GGUF rows against q8_1 activations (the decode-window kernel).
 // xq: q8_1 rows of the tokens, xq_stride bytes apart. W: slot tensor (w_is_table = 0,

@@ -16,6 +16,7 @@ namespace {
 
 constexpr int SORT_THREADS = 256;
 constexpr int SORT_CHUNK = 2048;  // routes of one block of the order's two kernels
+constexpr int SORT_SMALL = 4096;  // routes of a call that takes one launch
 constexpr int ROW_WAVES = 4;      // waves of a row kernel's block, at most
 
 __device__ __forceinline__ int key_of(int id, int E) { return id >= 0 && id < E ? id : E; }
@@ -74,10 +75,15 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_place_kernel(const int32_t*
   int* run = lds + n;
   for (int e = threadIdx.x; e < n; e += SORT_THREADS) {
     int before = 0, all = 0;
-    for (int i = 0; i < chunks; ++i) {
-      const int v = counts[(int64_t)i * n + e];
-      all += v;
-      if (i < c) before += v;
+    for (int i0 = 0; i0 < chunks; i0 += 16) {  // sixteen loads on their way at once
+      int v[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = counts[(int64_t)(i0 + i < chunks ? i0 + i : chunks - 1) * n + e];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        all += i0 + i < chunks ? v[i] : 0;
+        before += i0 + i < c ? v[i] : 0;
+      }
     }
     total[e] = all;
     run[e] = before;
@@ -140,6 +146,83 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_place_kernel(const int32_t*
 // 16 bytes of a row at any alignment of its elements
 __device__ __forceinline__ u32x4_t load16(const void* p) { return gload<u32x4_a2_t>(p); }
 __device__ __forceinline__ void store16(void* p, const u32x4_t& v) { *(u32x4_a2_t*)p = v; }
+
+// A call of up to SORT_SMALL routes in one launch: block (token, piece of its row) counts the places of
+// the token's routes itself, against all ids, while its part of the row is on its way; the block past
+// the last token makes the offsets. key << 14 | route orders the routes by one comparison.
+template <int ES>
+__global__ __launch_bounds__(SORT_THREADS) void sort_small_kernel(const uint8_t* __restrict__ x, int64_t x_stride,
+                                                                  int64_t bytes, const int32_t* __restrict__ ids,
+                                                                  int tokens, int top_k, int E,
+                                                                  int32_t* __restrict__ offsets, int32_t* __restrict__ perm,
+                                                                  int32_t* __restrict__ pos, uint8_t* __restrict__ rows) {
+  static_assert(SORT_SMALL <= 1 << 14 && SORT_MAX_EXPERTS < 1 << 17, "an order fits 31 bits");
+  extern __shared__ int lds[];  // the last block's E + 1 counts
+  __shared__ int part[4][8];
+  const int R = tokens * top_k, t = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (t == tokens) {
+    if (blockIdx.y) return;
+    for (int e = threadIdx.x; e <= E; e += SORT_THREADS) lds[e] = 0;
+    __syncthreads();
+    for (int r = threadIdx.x; r < R; r += SORT_THREADS) atomicAdd(&lds[key_of(ids[r], E)], 1);
+    __syncthreads();
+    const int per = (E + SORT_THREADS) / SORT_THREADS, e0 = threadIdx.x * per;
+    int sum = 0;
+    for (int e = e0; e < e0 + per && e <= E; ++e) sum += lds[e];
+    int at = block_exclusive(sum, part[0]);
+    for (int e = e0; e < e0 + per && e <= E; ++e) {
+      offsets[e] = at;
+      at += lds[e];
+    }
+    return;
+  }
+  const int64_t at = 16 * ((int64_t)blockIdx.y * SORT_THREADS + threadIdx.x);
+  const int64_t b = at < bytes - 16 ? at : bytes - 16;
+  u32x4_t v = {0, 0, 0, 0};
+  const u32x4_t zero = v;
+  if (rows && bytes >= 16 && at < bytes) v = load16(x + t * x_stride + b);
+  for (int j0 = 0; j0 < top_k; j0 += 8) {
+    int mine[8], count[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int r = t * top_k + (j0 + j < top_k ? j0 + j : top_k - 1);
+      mine[j] = key_of(ids[r], E) << 14 | r;
+      count[j] = 0;
+    }
+    for (int r0 = 64 * wave; r0 < R; r0 += SORT_THREADS) {
+      const int r = r0 + lane;
+      const int order = r < R ? key_of(ids[r], E) << 14 | r : 0x7FFFFFFF;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) count[j] += __popcll(__ballot(order < mine[j]));
+    }
+    if (j0) __syncthreads();
+    if (lane == 0)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) part[wave][j] = count[j];
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (j0 + j < top_k) {
+        const int p = part[0][j] + part[1][j] + part[2][j] + part[3][j];
+        const bool valid = mine[j] >> 14 < E;
+        const int r = t * top_k + j0 + j;
+        if (blockIdx.y == 0 && threadIdx.x == 0) {
+          perm[p] = valid ? r : ~r;
+          pos[r] = valid ? p : ~p;
+        }
+        if (rows && at < bytes) {
+          if (bytes >= 16) {
+            store16(rows + p * bytes + b, valid ? v : zero);
+          } else {
+            using U = typename std::conditional<ES == 4, uint32_t, uint16_t>::type;
+            for (int64_t i = 0; i < bytes / ES; ++i)
+              ((U*)(rows + p * bytes))[i] = valid ? ((const U*)(x + t * x_stride))[i] : (U)0;
+          }
+        }
+      }
+    }
+  }
+}
 
 // A row of `bytes` bytes in 16-byte pieces, lane by lane; the last piece ends with the row and may
 // overlap the one before it. Rows below 16 bytes go element by element (ES bytes each).
@@ -221,14 +304,23 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void unsort_kernel(const T* __restr
   Piece<T, V> acc;
 #pragma unroll
   for (int i = 0; i < V; ++i) acc.f[i] = 0.0f;
-  for (int j = 0; j < top_k; ++j) {
-    const int p = pos[t * top_k + j];
-    if (p < 0 || p >= n_rows) continue;
-    const float wj = w ? w[t * top_k + j] : 1.0f;
-    Piece<T, V> v;
-    v.load(rows + p * row_stride + c);
+  for (int j0 = 0; j0 < top_k; j0 += 8) {  // eight rows on their way at once
+    int p[8];
+    Piece<T, V> v[8];
 #pragma unroll
-    for (int i = 0; i < V; ++i) acc.f[i] = fmaf(wj, v.f[i], acc.f[i]);
+    for (int j = 0; j < 8; ++j) {
+      p[j] = j0 + j < top_k ? pos[t * top_k + j0 + j] : -1;
+      if (p[j] >= n_rows) p[j] = -1;
+      if (p[j] >= 0) v[j].load(rows + p[j] * row_stride + c);  // uniform
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (p[j] >= 0) {
+        const float wj = w ? w[t * top_k + j0 + j] : 1.0f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc.f[i] = fmaf(wj, v[j].f[i], acc.f[i]);
+      }
+    }
   }
   acc.store(y + t * cols + c);
 }
@@ -242,41 +334,61 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void unsort_grad_kernel(const T* __
                                                                      const int32_t* __restrict__ pos, int top_k,
                                                                      int n_rows, T* __restrict__ drows,
                                                                      float* __restrict__ dw) {
-  __shared__ float part[ROW_WAVES];
+  __shared__ float part[ROW_WAVES][8];
   const int64_t t = blockIdx.x;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int j = 0; j < top_k; ++j) {
-    const int p = pos[t * top_k + j], q = p >= 0 ? p : ~p;
-    const bool valid = p >= 0 && p < n_rows;
-    const float wj = valid ? (w ? w[t * top_k + j] : 1.0f) : 0.0f;
-    float dot = 0.0f;
+  for (int j0 = 0; j0 < top_k; j0 += 8) {
+    int p[8];
+    float wj[8], dot[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      p[j] = j0 + j < top_k ? pos[t * top_k + j0 + j] : n_rows;  // n_rows: no row at all
+      wj[j] = p[j] >= 0 && p[j] < n_rows ? (w ? w[t * top_k + j0 + j] : 1.0f) : 0.0f;
+      dot[j] = 0.0f;
+    }
     for (int64_t at = (int64_t)V * threadIdx.x; at < cols; at += (int64_t)V * blockDim.x) {
       const int64_t c = at < cols - V ? at : cols - V;
       const int skip = (int)(at - c);  // values of this piece that the one before holds too
-      Piece<T, V> d, o;
+      Piece<T, V> d, o[8];
       d.load(dy + t * dy_stride + c);
-      if (dw && valid) {
-        o.load(rows + p * row_stride + c);
+      if (dw)
 #pragma unroll
-        for (int i = 0; i < V; ++i) dot = i < skip ? dot : fmaf(d.f[i], o.f[i], dot);
-      }
-      if (drows && q < n_rows) {
+        for (int j = 0; j < 8; ++j)
+          if (p[j] >= 0 && p[j] < n_rows) o[j].load(rows + p[j] * row_stride + c);  // uniform
+      if (drows)
 #pragma unroll
-        for (int i = 0; i < V; ++i) o.f[i] = valid ? wj * d.f[i] : 0.0f;
-        o.store(drows + q * cols + c);
-      }
+        for (int j = 0; j < 8; ++j) {
+          const int q = p[j] >= 0 ? p[j] : ~p[j];
+          if (q < n_rows) {
+            Piece<T, V> r;
+#pragma unroll
+            for (int i = 0; i < V; ++i) r.f[i] = p[j] >= 0 ? wj[j] * d.f[i] : 0.0f;
+            r.store(drows + q * cols + c);
+          }
+        }
+      if (dw)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (p[j] >= 0 && p[j] < n_rows)
+#pragma unroll
+            for (int i = 0; i < V; ++i) dot[j] = i < skip ? dot[j] : fmaf(d.f[i], o[j].f[i], dot[j]);
     }
     if (dw) {
 #pragma unroll
-      for (int s = 32; s; s >>= 1) dot += __shfl_xor(dot, s);
-      if (lane == 0) part[wave] = dot;
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int s = 32; s; s >>= 1) dot[j] += __shfl_xor(dot[j], s);
+      if (j0) __syncthreads();
+      if (lane == 0)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) part[wave][j] = dot[j];
       __syncthreads();
-      if (threadIdx.x == 0) {
+      const int j = threadIdx.x;
+      if (j < 8 && j0 + j < top_k) {
         float all = 0.0f;
-        for (int i = 0; i < (int)(blockDim.x >> 6); ++i) all += part[i];
-        dw[t * top_k + j] = valid ? all : 0.0f;
+        for (int i = 0; i < (int)(blockDim.x >> 6); ++i) all += part[i][j];
+        dw[t * top_k + j0 + j] = all;  // without a row: its sums are 0
       }
-      __syncthreads();
     }
   }
 }
@@ -285,7 +397,7 @@ int row_threads(int64_t pieces) { return (int)(pieces >= 64 * ROW_WAVES ? 64 * R
 
 }  // namespace
 
-int64_t moe_sort_chunks(int64_t routes) { return (routes + SORT_CHUNK - 1) / SORT_CHUNK; }
+int64_t moe_sort_chunks(int64_t routes) { return routes <= SORT_SMALL ? 0 : (routes + SORT_CHUNK - 1) / SORT_CHUNK; }
 
 int launch_moe_sort(const uint8_t* x, int es, int64_t x_stride, int64_t cols, const int32_t* ids, int64_t tokens,
                     int64_t top_k, int64_t E, uint8_t* rows, int32_t* offsets, int32_t* perm, int32_t* pos, int* counts,
@@ -294,6 +406,15 @@ int launch_moe_sort(const uint8_t* x, int es, int64_t x_stride, int64_t cols, co
   const int chunks = (int)moe_sort_chunks(R);
   int bits = 0;
   while ((n - 1) >> bits) ++bits;
+  if (R <= SORT_SMALL) {
+    const int64_t bytes = rows ? cols * es : 1, per = 16 * SORT_THREADS;
+    dim3 grid((unsigned)tokens + 1, (unsigned)((bytes + per - 1) / per));
+    auto kernel = es == 4 ? sort_small_kernel<4> : sort_small_kernel<2>;
+    kernel<<<grid, SORT_THREADS, n * sizeof(int), stream>>>(x, x_stride * es, bytes, ids, (int)tokens, (int)top_k, (int)E,
+                                                            offsets, perm, pos, rows);
+    KTMI_HIP_TRY(hipGetLastError());
+    return KTMI_OK;
+  }
   if (chunks) sort_count_kernel<<<chunks, SORT_THREADS, n * sizeof(int), stream>>>(ids, R, (int)E, counts);
   sort_place_kernel<<<chunks ? chunks : 1, SORT_THREADS, 5 * n * sizeof(int), stream>>>(ids, R, (int)E, bits, counts, chunks,
                                                                                         offsets, perm, pos);

@@ -1,0 +1,8 @@
+// The 4-bit products' kernels (w4_kernel.h) for one activation type.
+#include "w4_kernel.h"
+
+namespace ktmi {
+
+int launch_w4_bf16(const W4Args& a, hipStream_t stream) { return launch_t<__bf16>(a, stream); }
+
+}  // namespace ktmi

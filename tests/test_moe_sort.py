@@ -60,6 +60,7 @@ SHAPES = [
     # one route more and less than the blocks of the order take
     (255, 4, 16, 64, 0.1), (1025, 1, 2048, 8, 0.0), (2047, 1, 3, 24, 0.1), (2049, 1, 300, 16, 0.1),
     (683, 6, 64, 33, 0.9), (4097, 8, 129, 40, 0.3),
+    (512, 8, 2048, 12, 0.2), (4097, 1, 2047, 10, 0.1), (6144, 1, 3, 8, 0.0), (2049, 3, 300, 16, 0.1),
 ]
 
 
@@ -404,12 +405,12 @@ def test_c_refusals():
     def sort(x=p, dt=2, stride=8, cols=8, ids=p, T=4, k=2, E=3, rows=p, off=p, perm=p, pos=p, ws=p, n=1 << 20):
         return L.ktmi_moe_sort(x, dt, stride, cols, ids, T, k, E, rows, off, perm, pos, ws, n, 0)
 
-    assert L.ktmi_moe_sort_workspace(4, 2, 3) > 0 and L.ktmi_moe_sort_workspace(0, 2, 3) == 0
+    assert L.ktmi_moe_sort_workspace(70000, 2, 3) > 0 and L.ktmi_moe_sort_workspace(0, 2, 3) == 0
     for kw, code in [(dict(dt=3), -1), (dict(cols=0), -1), (dict(cols=1 << 25, stride=1 << 25), -1), (dict(T=-1), -1),
                      (dict(k=0), -1), (dict(T=1 << 31), -1), (dict(T=1 << 62, k=4), -1), (dict(E=0), -1),
                      (dict(E=S.MAX_EXPERTS + 1), -1), (dict(x=0), -1), (dict(ids=0), -1), (dict(off=0), -1),
                      (dict(perm=0), -1), (dict(pos=0), -1), (dict(x=p + 1), -1), (dict(rows=p + 1), -1),
-                     (dict(stride=7), -1), (dict(ws=0), -4), (dict(n=1), -4)]:
+                     (dict(stride=7), -1), (dict(T=70000, ws=0), -4), (dict(T=70000, n=1), -4)]:
         assert sort(**kw) == code and b"moe_sort" in L.ktmi_last_error(), kw
 
     def unsort(rows=p, dt=2, stride=8, cols=8, w=p, pos=p, T=4, k=2, y=p):
