@@ -15,7 +15,7 @@ namespace ktmi {
 namespace {
 
 constexpr int SORT_THREADS = 256;
-constexpr int SORT_CHUNK = 2048;  // routes of one block of the order's two kernels
+constexpr int SORT_MAX_PER = 8;   // routes of a thread of the order's two kernels, at most
 constexpr int SORT_SMALL = 4096;  // routes of a call that takes one launch
 constexpr int ROW_WAVES = 4;      // waves of a row kernel's block, at most
 
@@ -27,14 +27,15 @@ __device__ __forceinline__ void sort_wave_fence() {
 }
 
 // counts[chunk][E + 1]: the chunk's routes by key
+template <int PER>
 __global__ __launch_bounds__(SORT_THREADS) void sort_count_kernel(const int32_t* __restrict__ ids, int R, int E,
                                                                   int* __restrict__ counts) {
   extern __shared__ int hist[];
   for (int e = threadIdx.x; e <= E; e += SORT_THREADS) hist[e] = 0;
   __syncthreads();
-  const int64_t r0 = (int64_t)blockIdx.x * SORT_CHUNK;
+  const int64_t r0 = (int64_t)blockIdx.x * (PER * SORT_THREADS);
 #pragma unroll
-  for (int i = 0; i < SORT_CHUNK / SORT_THREADS; ++i) {
+  for (int i = 0; i < PER; ++i) {
     const int64_t r = r0 + i * SORT_THREADS + threadIdx.x;
     if (r < R) atomicAdd(&hist[key_of(ids[r], E)], 1);
   }
@@ -61,8 +62,9 @@ __device__ __forceinline__ int block_exclusive(int v, int* tmp) {
 }
 
 // The places of a chunk's routes. LDS: the keys' first places [E + 1], then one running place for
-// every key and wave [4][E + 1]. Wave w owns routes [512 w, 512 w + 512) of the chunk, 64 at a
-// time in order; the lanes of one key find each other by ballots over the key's bits.
+// every key and wave [4][E + 1]. Wave w owns the w-th quarter of the chunk, 64 routes at a time in
+// order; the lanes of one key find each other by ballots over the key's bits.
+template <int PER>
 __global__ __launch_bounds__(SORT_THREADS) void sort_place_kernel(const int32_t* __restrict__ ids, int R, int E,
                                                                   int key_bits, const int* __restrict__ counts,
                                                                   int chunks, int32_t* __restrict__ offsets,
@@ -91,22 +93,22 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_place_kernel(const int32_t*
   }
   __syncthreads();
   // exclusive sums of the totals: each thread its own consecutive keys
-  const int per = (n + SORT_THREADS - 1) / SORT_THREADS;
-  const int e0 = threadIdx.x * per;
+  const int span = (n + SORT_THREADS - 1) / SORT_THREADS;
+  const int e0 = threadIdx.x * span;
   int sum = 0;
-  for (int e = e0; e < e0 + per && e < n; ++e) sum += total[e];
+  for (int e = e0; e < e0 + span && e < n; ++e) sum += total[e];
   int at = block_exclusive(sum, tmp);
-  for (int e = e0; e < e0 + per && e < n; ++e) {
+  for (int e = e0; e < e0 + span && e < n; ++e) {
     const int v = total[e];
     run[e] += at;
     if (c == 0) offsets[e] = at;
     at += v;
   }
   // the wave's own routes and their counts for the waves after it
-  int key[SORT_CHUNK / SORT_THREADS];
-  const int64_t r0 = (int64_t)c * SORT_CHUNK + wave * (SORT_CHUNK / 4);
+  int key[PER];
+  const int64_t r0 = ((int64_t)c * 4 + wave) * (64 * PER);
 #pragma unroll
-  for (int i = 0; i < SORT_CHUNK / SORT_THREADS; ++i) {
+  for (int i = 0; i < PER; ++i) {
     const int64_t r = r0 + 64 * i + lane;
     key[i] = r < R ? key_of(ids[r], E) : -1;
     if (key[i] >= 0 && wave < 3) atomicAdd(&run[(wave + 1) * n + key[i]], 1);
@@ -121,7 +123,7 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_place_kernel(const int32_t*
   int* mine = run + wave * n;
   const uint64_t below = (1ull << lane) - 1ull;
 #pragma unroll
-  for (int i = 0; i < SORT_CHUNK / SORT_THREADS; ++i) {
+  for (int i = 0; i < PER; ++i) {
     const bool in = key[i] >= 0;
     uint64_t same = __ballot(in);
     for (int b = 0; b < key_bits; ++b) {
@@ -253,18 +255,28 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void sort_rows_kernel(const uint8_t
   }
 }
 
-// V values of a row: 16 bytes of them, or one (rows shorter than 16 bytes)
+// V values of a row as loaded, and in fp32: 16 bytes of them, or one (rows shorter than 16 bytes)
+template <typename T, int V>
+struct Loaded {
+  using W = typename std::conditional<V == 1, T, u32x4_t>::type;
+  W w;
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (V == 1)
+      w = p[0];
+    else
+      w = load16(p);
+  }
+};
 template <typename T, int V>
 struct Piece {
   float f[V];
-  __device__ __forceinline__ void load(const T* p) {
+  __device__ __forceinline__ void take(const Loaded<T, V>& from) {
     if constexpr (V == 1) {
-      f[0] = (float)p[0];
+      f[0] = (float)from.w;
     } else {
-      const u32x4_t w = load16(p);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t u = w[i];  // a bit cast of w[i] itself takes element 0
+        const uint32_t u = from.w[i];  // a bit cast of w[i] itself takes element 0
         if constexpr (sizeof(T) == 4) {
           f[i] = __builtin_bit_cast(float, u);
         } else {
@@ -306,7 +318,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void unsort_kernel(const T* __restr
   for (int i = 0; i < V; ++i) acc.f[i] = 0.0f;
   for (int j0 = 0; j0 < top_k; j0 += 8) {  // eight rows on their way at once
     int p[8];
-    Piece<T, V> v[8];
+    Loaded<T, V> v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       p[j] = j0 + j < top_k ? pos[t * top_k + j0 + j] : -1;
@@ -317,8 +329,10 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void unsort_kernel(const T* __restr
     for (int j = 0; j < 8; ++j) {
       if (p[j] >= 0) {
         const float wj = w ? w[t * top_k + j0 + j] : 1.0f;
+        Piece<T, V> o;
+        o.take(v[j]);
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc.f[i] = fmaf(wj, v[j].f[i], acc.f[i]);
+        for (int i = 0; i < V; ++i) acc.f[i] = fmaf(wj, o.f[i], acc.f[i]);
       }
     }
   }
@@ -349,12 +363,14 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void unsort_grad_kernel(const T* __
     for (int64_t at = (int64_t)V * threadIdx.x; at < cols; at += (int64_t)V * blockDim.x) {
       const int64_t c = at < cols - V ? at : cols - V;
       const int skip = (int)(at - c);  // values of this piece that the one before holds too
-      Piece<T, V> d, o[8];
-      d.load(dy + t * dy_stride + c);
+      Loaded<T, V> dl, l[8];
+      dl.load(dy + t * dy_stride + c);
       if (dw)
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (p[j] >= 0 && p[j] < n_rows) o[j].load(rows + p[j] * row_stride + c);  // uniform
+          if (p[j] >= 0 && p[j] < n_rows) l[j].load(rows + p[j] * row_stride + c);  // uniform
+      Piece<T, V> d;
+      d.take(dl);
       if (drows)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -369,9 +385,12 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void unsort_grad_kernel(const T* __
       if (dw)
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (p[j] >= 0 && p[j] < n_rows)
+          if (p[j] >= 0 && p[j] < n_rows) {
+            Piece<T, V> o;
+            o.take(l[j]);
 #pragma unroll
-            for (int i = 0; i < V; ++i) dot[j] = i < skip ? dot[j] : fmaf(d.f[i], o[j].f[i], dot[j]);
+            for (int i = 0; i < V; ++i) dot[j] = i < skip ? dot[j] : fmaf(d.f[i], o.f[i], dot[j]);
+          }
     }
     if (dw) {
 #pragma unroll
@@ -397,7 +416,12 @@ int row_threads(int64_t pieces) { return (int)(pieces >= 64 * ROW_WAVES ? 64 * R
 
 }  // namespace
 
-int64_t moe_sort_chunks(int64_t routes) { return routes <= SORT_SMALL ? 0 : (routes + SORT_CHUNK - 1) / SORT_CHUNK; }
+// Routes a thread: few, for more blocks, as long as the blocks' counts stay few to add up
+static int sort_per(int64_t routes) { return routes <= 65536 ? 2 : SORT_MAX_PER; }
+int64_t moe_sort_chunks(int64_t routes) {
+  const int64_t chunk = sort_per(routes) * SORT_THREADS;
+  return routes <= SORT_SMALL ? 0 : (routes + chunk - 1) / chunk;
+}
 
 int launch_moe_sort(const uint8_t* x, int es, int64_t x_stride, int64_t cols, const int32_t* ids, int64_t tokens,
                     int64_t top_k, int64_t E, uint8_t* rows, int32_t* offsets, int32_t* perm, int32_t* pos, int* counts,
@@ -415,10 +439,12 @@ int launch_moe_sort(const uint8_t* x, int es, int64_t x_stride, int64_t cols, co
     KTMI_HIP_TRY(hipGetLastError());
     return KTMI_OK;
   }
-  if (chunks) sort_count_kernel<<<chunks, SORT_THREADS, n * sizeof(int), stream>>>(ids, R, (int)E, counts);
-  sort_place_kernel<<<chunks ? chunks : 1, SORT_THREADS, 5 * n * sizeof(int), stream>>>(ids, R, (int)E, bits, counts, chunks,
-                                                                                        offsets, perm, pos);
-  if (rows && R) {
+  const bool few = sort_per(R) == 2;
+  auto count = few ? sort_count_kernel<2> : sort_count_kernel<SORT_MAX_PER>;
+  auto place = few ? sort_place_kernel<2> : sort_place_kernel<SORT_MAX_PER>;
+  count<<<chunks, SORT_THREADS, n * sizeof(int), stream>>>(ids, R, (int)E, counts);
+  place<<<chunks, SORT_THREADS, 5 * n * sizeof(int), stream>>>(ids, R, (int)E, bits, counts, chunks, offsets, perm, pos);
+  if (rows) {
     const int64_t bytes = cols * es, pieces = (bytes + 15) / 16;
     const int th = row_threads(pieces);
     dim3 grid((unsigned)tokens, (unsigned)((pieces + th - 1) / th));

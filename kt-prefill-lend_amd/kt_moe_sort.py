@@ -137,12 +137,16 @@ class _Sort(torch.autograd.Function):
         return rows, offsets, perm, pos
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, drows, *_):
+    def backward(ctx, drows, *ignored):
+        if torch.is_grad_enabled():
+            return _Sort.once(ctx, drows, *ignored)
         if drows is None:
             return None, None, None
         pos, = ctx.saved_tensors
         return _lib.on_device_of(drows, _launch_unsort, drows, None, pos), None, None
+
+    # of a graph for second derivatives: the same without a graph of its own, refused when one is asked for
+    once = staticmethod(torch.autograd.function.once_differentiable(lambda ctx, *grads: _Sort.backward(ctx, *grads)))
 
 
 class _Unsort(torch.autograd.Function):
@@ -153,11 +157,14 @@ class _Unsort(torch.autograd.Function):
         return _lib.on_device_of(rows, _launch_unsort, rows, topk_w, pos)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        if torch.is_grad_enabled():
+            return _Unsort.once(ctx, dy)
         rows, topk_w, pos = ctx.saved_tensors
         return (*_lib.on_device_of(dy, _launch_unsort_grad, dy, rows, topk_w, pos, ctx.needs_input_grad[0],
                                    rows is not None), None)
+
+    once = staticmethod(torch.autograd.function.once_differentiable(lambda ctx, dy: _Unsort.backward(ctx, dy)))
 
 
 def moe_sort(x: torch.Tensor, ids: torch.Tensor, n_experts: int) -> MoeSorted:
