@@ -43,7 +43,7 @@ struct W4Args {
   int x_dtype, scale_dtype;
   const int32_t* perm;  // with offsets: the route at each place (set by launch_w4 alone)
 };
-constexpr int W4_LDS_MOST = 128 << 10;
+constexpr int W4_LDS_MOST = 152 << 10;
 int64_t w4_workspace(int64_t tokens, int64_t top_k, int64_t n_experts);
 int launch_w4(const W4Args& a, hipStream_t stream);
 int launch_w4_bf16(const W4Args& a, hipStream_t stream);  // by activation type: one pass without a sort

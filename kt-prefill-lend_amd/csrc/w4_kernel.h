@@ -31,7 +31,7 @@ constexpr int W4_RING = 8;             // steps of codes in flight a wave, a tur
 constexpr int W4_VMCNT0 = 0xF70;       // s_waitcnt operand: vector memory loads only
 constexpr int W4_X_BYTES = 64 << 10;   // LDS for a stage's activations, about: two blocks a CU
 constexpr int W4_CU_LDS = 160 << 10;
-constexpr int W4_X_SPLIT = 112 << 10;  // where the blocks are few: one a CU
+constexpr int W4_X_SPLIT = 136 << 10;  // where the blocks are few: one a CU
 
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
@@ -368,7 +368,7 @@ __global__ __launch_bounds__(64 * KS * WR) void w4_mfma_kernel(W4Args a, W4Plan 
 #pragma unroll
     for (int q = 0; q < 3; ++q) put(r, c, u32x4_t{part[q][0], part[q][1], part[q][2], part[q][3]}, q);
   };
-  constexpr int XB = PLANES == 1 ? 8 : 4;  // a thread's loads of a batch
+  constexpr int XB = PLANES == 1 ? 8 : 4;  // a thread's loads of a batch, the second half only where there are so many
   const int x_all = m * chunks;
   struct Batch {
     u32x4_t v[XB][PLANES == 1 ? 1 : 2];
@@ -377,8 +377,7 @@ __global__ __launch_bounds__(64 * KS * WR) void w4_mfma_kernel(W4Args a, W4Plan 
   // the thread's chunks from i0 on; past the last the last again
   auto fetch = [&](int k0, int i0) {
     Batch b;
-#pragma unroll
-    for (int j = 0; j < XB; ++j) {
+    auto part = [&](int j) {
       const int i = i0 + j * TH < x_all ? i0 + j * TH : x_all - 1;
       const int r = (int)(((float)i + 0.5f) * chunks_inv), c = i - r * chunks, k = k0 + 8 * c;
       b.at[j] = r << 16 | c;
@@ -389,12 +388,16 @@ __global__ __launch_bounds__(64 * KS * WR) void w4_mfma_kernel(W4Args a, W4Plan 
         b.v[j][0] = gload<u32x4_a4_t>(x);
         b.v[j][1] = gload<u32x4_a4_t>(x + 4);
       }
-    }
+    };
+#pragma unroll
+    for (int j = 0; j < XB / 2; ++j) part(j);
+    if (x_all > XB / 2 * TH)  // uniform
+#pragma unroll
+      for (int j = XB / 2; j < XB; ++j) part(j);
     return b;
   };
   auto store = [&](int k0, int i0, const Batch& b) {
-#pragma unroll
-    for (int j = 0; j < XB; ++j) {
+    auto part = [&](int j) {
       const int r = b.at[j] >> 16, c = b.at[j] & 0xFFFF, k = k0 + 8 * c;
       if (i0 + j * TH < x_all && (k + 8 <= cols || k >= cols)) {
         const bool in = k < cols;
@@ -407,7 +410,12 @@ __global__ __launch_bounds__(64 * KS * WR) void w4_mfma_kernel(W4Args a, W4Plan 
           put3(r, c, u);
         }
       }
-    }
+    };
+#pragma unroll
+    for (int j = 0; j < XB / 2; ++j) part(j);
+    if (x_all > XB / 2 * TH)
+#pragma unroll
+      for (int j = XB / 2; j < XB; ++j) part(j);
   };
   auto fill = [&](int k0, const Batch& b) {
     store(k0, threadIdx.x, b);
@@ -704,17 +712,22 @@ int launch_one(const W4Args& a, int64_t items, int64_t expected, hipStream_t str
 template <typename T, int SPS>
 int launch_sps(const W4Args& a, hipStream_t stream) {
   constexpr bool F32 = std::is_same<T, float>::value;
-  const int64_t mean = a.offsets ? a.n_routes / a.n_experts : a.ids ? 1 : a.n_routes;  // rows of an expert, about
+  // rows of an expert, about: 16 a pass, or 32 where there are more (dense 4096 x 7168, bf16: 32 rows 33 us
+  // in one pass of 32, 64 rows 34 in two; in one of 64 with its shorter stages 71)
+  const int64_t mean = a.offsets ? a.n_routes / a.n_experts : a.ids ? 1 : a.n_routes;
   const bool many = !F32 && mean > 16;
-  const int64_t rows = many ? 64 : 16;
+  const int64_t rows = many ? 32 : 16;
   const int64_t items = a.ids ? a.n_routes
                         : a.offsets ? (a.n_experts < a.n_routes ? a.n_experts : a.n_routes) + a.n_routes / rows
                                     : (a.n_routes + rows - 1) / rows;
   // items that have rows, at most but for passes after an expert's first
-  const int64_t expected = a.ids || !a.offsets ? items : a.n_experts < a.n_routes ? a.n_experts : a.n_routes;
-  const bool split = expected * ((a.rows + 63) / 64) < 1024;
+  const int64_t expected = !a.ids && !a.offsets ? items : a.n_experts < a.n_routes ? a.n_experts : a.n_routes;
+  // Four waves share 16 weight rows (32 of the larger passes) where whole rows a wave would leave CUs idle:
+  // 7168 x 2048 bf16 dense, one row, 7.4 us; 23 experts of 1024 x 2048, 10.8 us without and 20.4 with
+  const bool split = expected * ((a.rows + 63) / 64) < 256;
   if constexpr (!F32)
-    if (many) return split ? launch_one<T, SPS, 4, 4, 2>(a, items, expected, stream) : launch_one<T, SPS, 4, 1, 4>(a, items, expected, stream);
+    if (many)
+      return split ? launch_one<T, SPS, 2, 4, 2>(a, items, expected, stream) : launch_one<T, SPS, 2, 1, 4>(a, items, expected, stream);
   return split ? launch_one<T, SPS, 1, 4, 1>(a, items, expected, stream) : launch_one<T, SPS, 1, 1, 4>(a, items, expected, stream);
 }
 
