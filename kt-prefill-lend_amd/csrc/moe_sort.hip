@@ -163,8 +163,8 @@ __device__ __forceinline__ void store16(void* p, const u32x4_t& v) {
 
 // A call of up to SORT_SMALL routes in one launch: block (token, piece of its row) counts the places of
 // the token's routes itself, against all ids, while its part of the row is on its way; the block past
-// the last token makes the offsets. key << 14 | route orders the routes by one comparison.
-template <int ES>
+// the last token makes the offsets. G routes of the token at a time. key << 14 | route orders the routes by one comparison.
+template <int ES, int G>
 __global__ __launch_bounds__(SORT_THREADS) void sort_small_kernel(const uint8_t* __restrict__ x, int64_t x_stride,
                                                                   int64_t bytes, const int32_t* __restrict__ ids,
                                                                   int tokens, int top_k, int E,
@@ -172,7 +172,7 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_small_kernel(const uint8_t*
                                                                   int32_t* __restrict__ pos, uint8_t* __restrict__ rows) {
   static_assert(SORT_SMALL <= 1 << 14 && SORT_MAX_EXPERTS < 1 << 17, "an order fits 31 bits");
   extern __shared__ int lds[];  // the last block's E + 1 counts
-  __shared__ int part[4][8];
+  __shared__ int part[4][G];
   const int R = tokens * top_k, t = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (t == tokens) {
     if (blockIdx.y) return;
@@ -195,27 +195,33 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_small_kernel(const uint8_t*
   u32x4_t v = {0, 0, 0, 0};
   const u32x4_t zero = v;
   if (rows && bytes >= 16 && at < bytes) v = load16(x + t * x_stride + b);
-  for (int j0 = 0; j0 < top_k; j0 += 8) {
-    int mine[8], count[8];
+  for (int j0 = 0; j0 < top_k; j0 += G) {
+    int mine[G], count[G];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < G; ++j) {
       const int r = t * top_k + (j0 + j < top_k ? j0 + j : top_k - 1);
       mine[j] = key_of(ids[r], E) << 14 | r;
       count[j] = 0;
     }
-    for (int r0 = 64 * wave; r0 < R; r0 += SORT_THREADS) {
-      const int r = r0 + lane;
-      const int order = r < R ? key_of(ids[r], E) << 14 | r : 0x7FFFFFFF;
+    for (int r0 = 64 * wave; r0 < R; r0 += 4 * SORT_THREADS) {  // four loads on their way at once
+      int id[4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) count[j] += __popcll(__ballot(order < mine[j]));
+      for (int i = 0; i < 4; ++i) id[i] = ids[r0 + i * SORT_THREADS + lane < R ? r0 + i * SORT_THREADS + lane : R - 1];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = r0 + i * SORT_THREADS + lane;
+        const int order = r < R ? key_of(id[i], E) << 14 | r : 0x7FFFFFFF;
+#pragma unroll
+        for (int j = 0; j < G; ++j) count[j] += __popcll(__ballot(order < mine[j]));
+      }
     }
     if (j0) __syncthreads();
     if (lane == 0)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) part[wave][j] = count[j];
+      for (int j = 0; j < G; ++j) part[wave][j] = count[j];
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < G; ++j) {
       if (j0 + j < top_k) {
         const int p = part[0][j] + part[1][j] + part[2][j] + part[3][j];
         const bool valid = mine[j] >> 14 < E;
@@ -445,7 +451,8 @@ int launch_moe_sort(const uint8_t* x, int es, int64_t x_stride, int64_t cols, co
   if (R <= SORT_SMALL) {
     const int64_t bytes = rows ? cols * es : 1, per = 16 * SORT_THREADS;
     dim3 grid((unsigned)tokens + 1, (unsigned)((bytes + per - 1) / per));
-    auto kernel = es == 4 ? sort_small_kernel<4> : sort_small_kernel<2>;
+    auto kernel = es == 4 ? (top_k > 8 ? sort_small_kernel<4, 16> : sort_small_kernel<4, 8>)
+                          : (top_k > 8 ? sort_small_kernel<2, 16> : sort_small_kernel<2, 8>);
     kernel<<<grid, SORT_THREADS, n * sizeof(int), stream>>>(x, x_stride * es, bytes, ids, (int)tokens, (int)top_k, (int)E,
                                                             offsets, perm, pos, rows);
     KTMI_HIP_TRY(hipGetLastError());

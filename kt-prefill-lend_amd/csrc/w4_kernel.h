@@ -692,9 +692,6 @@ int launch_as(const W4Args& a, int64_t items, int64_t expected, hipStream_t stre
   const int64_t bytes = p.x_bytes + (KS == 1 && whole > x_bytes ? p.deep * WR * MT * 64 * 16 : 0);
   KTMI_REQUIRE(items * p.blocks <= 0x7FFFFFFF, KTMI_EINVAL, "w4: %lld blocks (below 2^31)", (long long)(items * p.blocks));
   auto kernel = w4_mfma_kernel<T, SPS, S4, Z, MT, KS, WR>;
-  static const hipError_t attr =
-      hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, W4_LDS_MOST);
-  KTMI_HIP_TRY(attr);
   KTMI_REQUIRE(bytes <= W4_LDS_MOST, KTMI_EINVAL, "w4: %lld bytes of LDS", (long long)bytes);
   kernel<<<(unsigned)(items * p.blocks), 64 * KS * WR, bytes, stream>>>(a, p);
   return KTMI_OK;

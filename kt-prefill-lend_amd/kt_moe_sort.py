@@ -35,7 +35,7 @@ _CODES = {torch.float32: _lib.KTMI_F32, torch.float16: _lib.KTMI_F16, torch.bflo
 
 def _rows_of(t):
     """t with its values of a row next to each other and rows that do not overlap."""
-    return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
+    return t if t.is_contiguous() or (t.stride(1) == 1 and t.stride(0) >= t.shape[1]) else t.contiguous()
 
 
 def _check_gpu(what, *tensors):

@@ -40,12 +40,13 @@ def _check(what, x, codes, scales, zeros, group, lead):
         raise ValueError(f"{what}: group_size {group} (32, 64, a multiple of 128, or at least K = {K})")
     per = 2 if codes.dtype == torch.uint8 else 8
     width, groups = -(-K // per), -(-K // group)
-    if codes.dim() != 2 + lead or codes.shape[-1] != width or (per == 8 and K % 8) or codes.shape[-2] == 0:
+    *front, last = codes.shape
+    if len(front) != 1 + lead or last != width or (per == 8 and K % 8) or front[-1] == 0:
         raise ValueError(f"{what}: codes must be {'[E, N, ' if lead else '[N, '}{width}] for K = {K}, got {codes.dtype} "
                          f"{list(codes.shape)}")
-    if lead and not 0 < codes.shape[0] <= MAX_EXPERTS:
-        raise ValueError(f"{what}: {codes.shape[0]} experts (1 to {MAX_EXPERTS})")
-    want = codes.shape[:-1] + (groups,)
+    if lead and not 0 < front[0] <= MAX_EXPERTS:
+        raise ValueError(f"{what}: {front[0]} experts (1 to {MAX_EXPERTS})")
+    want = (*front, groups)
     if scales.shape != want:
         raise ValueError(f"{what}: scales must be {list(want)}, got {list(scales.shape)}")
     if zeros is not None:
