@@ -152,10 +152,10 @@ __device__ __forceinline__ void w4_wave_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// The block's item: expert e, its rows of y at list[0 .. m) and of x at from[0 .. m); returns m, 0 for
+// The block's item: expert e, its rows of x at src[0 .. m) and of y at dst[0 .. m); returns m, 0 for
 // none. Every wave writes the same lists and reads what it wrote: no barrier.
-template <int MT>
-__device__ __forceinline__ int find_item(const W4Args& a, int item, int& e, int* list, int* from) {
+template <typename T, int MT>
+__device__ __forceinline__ int find_item(const W4Args& a, int item, int& e, const T** src, T** dst) {
   const int lane = threadIdx.x & 63;
   constexpr int ROWS = 16 * MT;
   if (a.ids) {
@@ -168,8 +168,8 @@ __device__ __forceinline__ int find_item(const W4Args& a, int item, int& e, int*
     if (rank % ROWS) return 0;
     const int mine = __popcll(same & ((1ull << lane) - 1ull)) - rank;
     if (id == e && mine >= 0 && mine < ROWS) {
-      list[mine] = lane;
-      from[mine] = lane / (int)a.top_k;
+      src[mine] = (const T*)a.x + lane / (int)a.top_k * a.x_stride;
+      dst[mine] = (T*)a.y + lane * a.rows;
     }
     w4_wave_fence();
     const int m = __popcll(same) - rank;
@@ -212,8 +212,8 @@ __device__ __forceinline__ int find_item(const W4Args& a, int item, int& e, int*
   if (m > ROWS) m = ROWS;
   if (lane < m) {
     const int r = a.perm ? a.perm[first + lane] : first + lane;
-    list[lane] = r;
-    from[lane] = a.perm ? r / (int)a.top_k : r;
+    src[lane] = (const T*)a.x + (a.perm ? r / (int)a.top_k : r) * a.x_stride;
+    dst[lane] = (T*)a.y + r * a.rows;
   }
   w4_wave_fence();
   return m > 0 ? m : 0;
@@ -225,13 +225,14 @@ __global__ __launch_bounds__(64 * KS * WR) void w4_mfma_kernel(W4Args a, W4Plan 
   constexpr int PLANES = std::is_same<T, float>::value ? 3 : 1;
   constexpr int RB = 16 * WR, TH = 64 * KS * WR;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  __shared__ int list[16 * MT], from[16 * MT];
+  __shared__ const T* src[16 * MT];
+  __shared__ T* dst[16 * MT];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int item = blockIdx.x / p.blocks, n0 = (blockIdx.x - item * p.blocks) * p.deep * RB;
   const int rows_left = (int)(a.rows - n0 < RB * p.deep ? a.rows - n0 : RB * p.deep);
   T* y = (T*)a.y;
   int e;
-  const int m = find_item<MT>(a, item, e, list, from);
+  const int m = find_item<T, MT>(a, item, e, src, dst);
 
   // rows of no expert are zero: route `item` by its id, or every items-th row outside the segments
   // (of unsorted ids: the routes that the order puts there)
@@ -381,7 +382,7 @@ __global__ __launch_bounds__(64 * KS * WR) void w4_mfma_kernel(W4Args a, W4Plan 
       const int i = i0 + j * TH < x_all ? i0 + j * TH : x_all - 1;
       const int r = (int)(((float)i + 0.5f) * chunks_inv), c = i - r * chunks, k = k0 + 8 * c;
       b.at[j] = r << 16 | c;
-      const T* x = (const T*)a.x + from[r] * a.x_stride + (k < cols - 8 ? k : cols - 8);
+      const T* x = src[r] + (k < cols - 8 ? k : cols - 8);
       if constexpr (PLANES == 1) {
         b.v[j][0] = gload<u32x4_a2_t>(x);
       } else {
@@ -427,7 +428,7 @@ __global__ __launch_bounds__(64 * KS * WR) void w4_mfma_kernel(W4Args a, W4Plan 
     const int k = cols & ~7;
     if ((cols & 7) && k >= k0 && k < k0 + stage && threadIdx.x < m) {
       const int r = threadIdx.x, c = (k - k0) / 8;
-      const T* x = (const T*)a.x + from[r] * a.x_stride + k;
+      const T* x = src[r] + k;
       if constexpr (PLANES == 1) {
         uint32_t u[4] = {0, 0, 0, 0};
 #pragma unroll
@@ -491,7 +492,7 @@ __global__ __launch_bounds__(64 * KS * WR) void w4_mfma_kernel(W4Args a, W4Plan 
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int r = 16 * q + 4 * g + i;
-          if (r < m) y[list[r] * a.rows + n0 + t * RB + rb] = (T)acc[q][i];
+          if (r < m) *(__attribute__((address_space(1))) T*)(dst[r] + n0 + t * RB + rb) = (T)acc[q][i];  // global: a flat store drains the ring
         }
   };
   auto run = [&](auto plain) {
