@@ -6,6 +6,12 @@
 // totals of the keys below, of the chunks before and of the routes before inside the chunk. The
 // row copies, the weighted sums and the gradients then go by token: a token's row is read once
 // and its routes' places are wave-uniform.
+//
+// HBM bounds the long calls and launches the short ones. 16384 tokens of 2048 bf16 columns, 8 routes
+// each: the order 17 us (two launches), the copies 104 us for 604 MB (5.8 TB/s; a large copy on this
+// card moves 5.0 read and written, a fill 6.9); 4096 tokens: the sums back 24 us, their gradients 43 us for
+// 257 MB (6.0 TB/s). One token: one launch of 4 us. The order could be one launch less with blocks that
+// wait for each other's counts; that is left out, as a wait between blocks ends only if all of them run.
 #include <type_traits>
 
 #include "kernels.h"
@@ -29,7 +35,8 @@ __device__ __forceinline__ void sort_wave_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// counts[chunk][E + 1]: the chunk's routes by key
+// counts[chunk][E + 1]: the chunk's routes by key. Bound by LDS atomics on popular keys: 2 routes a
+// thread 2.8 us at 16376 routes, 8 a thread 5.4.
 template <int PER>
 __global__ __launch_bounds__(SORT_THREADS) void sort_count_kernel(const int32_t* __restrict__ ids, int R, int E,
                                                                   int* __restrict__ counts) {
@@ -66,7 +73,8 @@ __device__ __forceinline__ int block_exclusive(int v, int* tmp) {
 
 // The places of a chunk's routes. LDS: the keys' first places [E + 1], then one running place for
 // every key and wave [4][E + 1]. Wave w owns the w-th quarter of the chunk, 64 routes at a time in
-// order; the lanes of one key find each other by ballots over the key's bits.
+// order; the lanes of one key find each other by ballots over the key's bits. 5.2 us at 16376 routes of
+// 128 keys, 11.5 at 131072 of 256 (the counts of all chunks, sixteen loads at a time; one by one 29).
 template <int PER>
 __global__ __launch_bounds__(SORT_THREADS) void sort_place_kernel(const int32_t* __restrict__ ids, int R, int E,
                                                                   int key_bits, const int* __restrict__ counts,

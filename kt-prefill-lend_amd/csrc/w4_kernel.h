@@ -2,14 +2,15 @@
 //   y[r, n] = sum_g s[e, n, g] * sum_{c in g} (q[e, n, c] - z[e, n, g]) * x[r, c]
 //
 // w4_mfma_kernel, for rows of a step (128 columns) or more, runs the matrix cores for any number of
-// activation rows from one: v_mfma_f32_16x16x32 with 16 weight rows as its columns and up to 16
+// activation rows from one: v_mfma_f32_16x16x32 with 16 weight rows as its columns and 16
 // activation rows as its rows. A wave takes 16 weight rows in steps of 128 columns, 16 bytes of
-// codes a lane (lane l: row l % 16, column piece g = l / 16), loaded ahead into a ring of registers.
+// codes a lane (lane l: row l % 16, column piece g = l / 16), eight steps ahead in a ring of registers.
 //
 // Codes become operands exactly: an e4m3 byte of value n < 16 is n * 2^-9 (the subnormals run on
 // into the first normal binade), so one v_cvt_scalef32_pk turns two masked nibbles into two bf16 or
-// f16 integers. The zero point is a second product of the same activations with the constant -z, so
-// the group's sum D = sum (q - z) x is exact but for fp32 sums, and acc += s D. Infinite or NaN
+// f16 integers, seven instructions for eight codes. The zero point is a second product of the same
+// activations with the constant -z, so the group's sum D = sum (q - z) x is exact but for fp32 sums, and
+// acc += s D: no rounding of a weight. Infinite or NaN
 // activations (and products past fp32) make that inf - inf: a block whose sums are not all finite
 // runs again with q - z as the operand, which gives the plain sum's infinities and NaN.
 //
@@ -18,6 +19,16 @@
 //
 // The activations of the block's rows pass through LDS in column stages, values of each eight in the
 // order 0 2 4 6 1 3 5 7 in which the nibbles come out; columns past the row's end are zeros there.
+//
+// What bounds it: large calls the weights' bytes, of which about 4 TB/s come (20 experts of 4096 x 7168
+// bf16, 13 tokens: 74 us for 290 MB; 67 with the products left out), with the vector pipe at half
+// its rate behind them; small ones the chain from the ids to the loads to the sums (one row of 4096 x 7168
+// 8.3 us, 6.3 with nothing but its loads). What it took to get there, the former case: loads and
+// products of a step at a time 115 us; both 64-byte halves of a row's line and the scales of eight steps
+// asked for together 95 (single steps missed the vector cache with the second half, and with every scale);
+// row tiles after each other on the same activations, no condition inside a turn of the ring, as many
+// blocks as the chip holds 74. Many rows of x cost their passage through LDS: 4096 x 7168 at 16 rows 18 us,
+// at 64 rows 29.
 #pragma once
 #include <type_traits>
 
@@ -34,13 +45,11 @@ constexpr int W4_CU_LDS = 160 << 10;
 constexpr int W4_X_SPLIT = 136 << 10;  // where the blocks are few: one a CU
 
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 
 // what the MFMA takes: bf16 for bf16 and fp32 activations, f16 for f16
 template <typename T>
 struct Operand {
-  using V8 = bf16x8_t;
   static __device__ __forceinline__ f32x4_t mfma(const u32x4_t& a, const u32x4_t& b, const f32x4_t& c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
   }
