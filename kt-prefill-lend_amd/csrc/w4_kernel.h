@@ -739,14 +739,14 @@ int launch_sps(const W4Args& a, hipStream_t stream) {
 
 template <typename T>
 int launch_t(const W4Args& a, hipStream_t stream) {
+  W4Args b = a;
+  if (a.group >= a.cols) b.group = (a.cols + W4_STEP - 1) / W4_STEP * W4_STEP;  // one group of whole steps
   if (a.cols < W4_STEP) {
     const int64_t quads = (a.rows + 3) / 4;
     const dim3 grid((unsigned)a.n_routes, (unsigned)(quads < 65535 ? quads : 65535));
-    w4_short_kernel<T><<<grid, 256, 0, stream>>>(a);
+    w4_short_kernel<T><<<grid, 256, 0, stream>>>(b);
     return KTMI_OK;
   }
-  W4Args b = a;
-  if (a.group >= a.cols) b.group = (a.cols + W4_STEP - 1) / W4_STEP * W4_STEP;  // one group of whole steps
   return b.group == 32 ? launch_sps<T, 4>(b, stream) : b.group == 64 ? launch_sps<T, 2>(b, stream) : launch_sps<T, 1>(b, stream);
 }
 

@@ -61,6 +61,7 @@ def _check(what, x, codes, scales, zeros, group, lead):
 def _args(x, codes, scales, zeros, group):
     """The contiguous tensors of a call (kept alive by the caller) and the C arguments from x to group."""
     x, codes, scales = _rows_of(x), codes.contiguous(), scales.contiguous()
+    group = min(group, x.shape[1])  # one group a row, however large the size that says so
     zeros = None if zeros is None else zeros.contiguous()
     return (x, codes, scales, zeros), (x.data_ptr(), _CODES[x.dtype], x.stride(0), x.shape[1], codes.data_ptr(),
                                        scales.data_ptr(), _CODES[scales.dtype],

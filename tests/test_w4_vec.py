@@ -308,7 +308,35 @@ def test_graphs_and_streams(dev, T):
     assert all(torch.equal(p, r) for p, r in zip(a + b, step(0) + step(1)))
 
 
+LARGE_GROUPS = [2 ** 31, 2 ** 32, 2 ** 40, 2 ** 64 + 32]
+
+
+@pytest.mark.parametrize("G", LARGE_GROUPS)
+def test_group_sizes_past_32_bits_reach_c_as_one_group(G):
+    x, q, s = torch.ones(1, 64), torch.zeros((3, 32), dtype=torch.uint8), torch.ones(3, 1)
+    assert W._args(x, q, s, None, G)[1][-1] == 64
+
+
+@gpu
+@pytest.mark.parametrize("K", [1, 64, 127, 128, 200])
+@pytest.mark.parametrize("G", LARGE_GROUPS)
+def test_group_sizes_past_32_bits(dev, G, K):
+    q, s, z = make_weights((2,), 21, K, K, True, torch.bfloat16, 8, dev)
+    x = make_x(3, K, torch.bfloat16, 9, dev)
+    same(W.w4_vec(x, q[1], s[1], z[1], G), x.double() @ matrix(q[1], s[1], z[1], K, K)[0].t())
+    ids = torch.tensor([1, 0, -1], dtype=torch.int32, device=dev)
+    same(W.moe_w4_vec(x, q, s, ids, 1, z, G), routed(x, q, s, z, K, ids, 1)[0])
+    # the C entry by itself
+    if G < 2 ** 63:
+        y = torch.empty((3, 21), dtype=torch.bfloat16, device=dev)
+        L = _lib.lib()
+        assert L.ktmi_w4_vec(x.data_ptr(), _lib.KTMI_BF16, K, K, q.data_ptr(), s.data_ptr(), _lib.KTMI_BF16, z.data_ptr(), G,
+                             21, 3, y.data_ptr(), _lib.stream_ptr()) == 0
+        same(y, x.double() @ matrix(q[0], s[0], z[0], K, K)[0].t())
+
+
 # ---------------------------------------------------------------- refusals (no GPU)
+
 
 def test_refusals():
     x, q, s = torch.zeros(2, 64), torch.zeros(3, 32, dtype=torch.uint8), torch.zeros(3, 2)
