@@ -26,6 +26,11 @@ constexpr int SORT_MAX_PER = 8;   // routes of a thread of the order's two kerne
 // launch and 13.4 in three, 8192 20.0 and 15.2, 16376 43.4 and 21.6 (every block reads all ids).
 constexpr int SORT_SMALL = 4096;
 constexpr int64_t SORT_CACHED = 256 << 20;  // the last-level cache
+// Chunks up to which every chunk adds up the counts of all by itself; of more they are added up once, in a
+// launch of its own (else the work would grow with the routes' square). The order of 256 keys: 64 chunks
+// 14.5 us by themselves and 14.9 with the launch, 128 18.8 and 15.4, 256 27.2 and 16.6.
+constexpr int SORT_SCAN = 64;
+constexpr int SCAN_WAVES = 16;
 constexpr int ROW_WAVES = 4;      // waves of a row kernel's block, at most
 
 __device__ __forceinline__ int key_of(int id, int E) { return id >= 0 && id < E ? id : E; }
@@ -71,11 +76,44 @@ __device__ __forceinline__ int block_exclusive(int v, int* tmp) {
   return before + s - v;
 }
 
-// The places of a chunk's routes. LDS: the keys' first places [E + 1], then one running place for
+// counts[c][e] becomes the routes of key e before chunk c, counts[chunks][e] all of them. A block takes 64
+// keys, each of its waves a run of chunks: their sum first, then their running sums.
+__global__ __launch_bounds__(64 * SCAN_WAVES) void sort_scan_kernel(int* __restrict__ counts, int chunks, int n) {
+  __shared__ int part[SCAN_WAVES][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, e = blockIdx.x * 64 + lane;
+  const int span = (chunks + SCAN_WAVES - 1) / SCAN_WAVES, c0 = wave * span;
+  const int c1 = c0 + span < chunks ? c0 + span : chunks;
+  int v[16], sum = 0;
+  for (int c = c0; c < c1; c += 16) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = e < n && c + i < c1 ? counts[(int64_t)(c + i) * n + e] : 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum += v[i];
+  }
+  part[wave][lane] = sum;
+  __syncthreads();
+  int before = 0, all = 0;
+  for (int w = 0; w < SCAN_WAVES; ++w) {
+    before += w < wave ? part[w][lane] : 0;
+    all += part[w][lane];
+  }
+  for (int c = c0; c < c1; c += 16) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = e < n && c + i < c1 ? counts[(int64_t)(c + i) * n + e] : 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if (e < n && c + i < c1) counts[(int64_t)(c + i) * n + e] = before;
+      before += v[i];
+    }
+  }
+  if (wave == 0 && e < n) counts[(int64_t)chunks * n + e] = all;
+}
+
+// The places of a chunk's routes. SCANNED: the counts are as sort_scan_kernel leaves them. LDS: the keys' first places [E + 1], then one running place for
 // every key and wave [4][E + 1]. Wave w owns the w-th quarter of the chunk, 64 routes at a time in
 // order; the lanes of one key find each other by ballots over the key's bits. 5.2 us at 16376 routes of
-// 128 keys, 11.5 at 131072 of 256 (the counts of all chunks, sixteen loads at a time; one by one 29).
-template <int PER>
+// 128 keys, 11.5 at 131072 of 256 (64 chunks, the counts of all chunks, sixteen loads at a time; one by one 29).
+template <int PER, bool SCANNED>
 __global__ __launch_bounds__(SORT_THREADS) void sort_place_kernel(const int32_t* __restrict__ ids, int R, int E,
                                                                   int key_bits, const int* __restrict__ counts,
                                                                   int chunks, int32_t* __restrict__ offsets,
@@ -88,14 +126,19 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_place_kernel(const int32_t*
   int* run = lds + n;
   for (int e = threadIdx.x; e < n; e += SORT_THREADS) {
     int before = 0, all = 0;
-    for (int i0 = 0; i0 < chunks; i0 += 16) {  // sixteen loads on their way at once
-      int v[16];
+    if constexpr (SCANNED) {
+      before = counts[(int64_t)c * n + e];
+      all = counts[(int64_t)chunks * n + e];
+    } else {
+      for (int i0 = 0; i0 < chunks; i0 += 16) {  // sixteen loads on their way at once
+        int v[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = counts[(int64_t)(i0 + i < chunks ? i0 + i : chunks - 1) * n + e];
+        for (int i = 0; i < 16; ++i) v[i] = counts[(int64_t)(i0 + i < chunks ? i0 + i : chunks - 1) * n + e];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        all += i0 + i < chunks ? v[i] : 0;
-        before += i0 + i < c ? v[i] : 0;
+        for (int i = 0; i < 16; ++i) {
+          all += i0 + i < chunks ? v[i] : 0;
+          before += i0 + i < c ? v[i] : 0;
+        }
       }
     }
     total[e] = all;
@@ -444,16 +487,20 @@ int row_threads(int64_t pieces) { return (int)(pieces >= 64 * ROW_WAVES ? 64 * R
 
 // Routes a thread: few, for more blocks, as long as the blocks' counts stay few to add up
 static int sort_per(int64_t routes) { return routes <= 65536 ? 2 : SORT_MAX_PER; }
-int64_t moe_sort_chunks(int64_t routes) {
+static int64_t sort_chunks(int64_t routes) {
   const int64_t chunk = sort_per(routes) * SORT_THREADS;
-  return routes <= SORT_SMALL ? 0 : (routes + chunk - 1) / chunk;
+  return (routes + chunk - 1) / chunk;
+}
+int64_t moe_sort_counts(int64_t routes) {
+  if (routes <= SORT_SMALL) return 0;
+  const int64_t chunks = sort_chunks(routes);
+  return chunks + 1;  // and their totals, of many chunks
 }
 
 int launch_moe_sort(const uint8_t* x, int es, int64_t x_stride, int64_t cols, const int32_t* ids, int64_t tokens,
                     int64_t top_k, int64_t E, uint8_t* rows, int32_t* offsets, int32_t* perm, int32_t* pos, int* counts,
                     hipStream_t stream) {
   const int R = (int)(tokens * top_k), n = (int)E + 1;
-  const int chunks = (int)moe_sort_chunks(R);
   int bits = 0;
   while ((n - 1) >> bits) ++bits;
   if (R <= SORT_SMALL) {
@@ -466,10 +513,12 @@ int launch_moe_sort(const uint8_t* x, int es, int64_t x_stride, int64_t cols, co
     KTMI_HIP_TRY(hipGetLastError());
     return KTMI_OK;
   }
-  const bool few = sort_per(R) == 2;
+  const int chunks = (int)sort_chunks(R);
+  const bool few = sort_per(R) == 2, scan = !few && chunks > SORT_SCAN;
   auto count = few ? sort_count_kernel<2> : sort_count_kernel<SORT_MAX_PER>;
-  auto place = few ? sort_place_kernel<2> : sort_place_kernel<SORT_MAX_PER>;
+  auto place = few ? sort_place_kernel<2, false> : scan ? sort_place_kernel<SORT_MAX_PER, true> : sort_place_kernel<SORT_MAX_PER, false>;
   count<<<chunks, SORT_THREADS, n * sizeof(int), stream>>>(ids, R, (int)E, counts);
+  if (scan) sort_scan_kernel<<<(n + 63) / 64, 64 * SCAN_WAVES, 0, stream>>>(counts, chunks, n);
   place<<<chunks, SORT_THREADS, 5 * n * sizeof(int), stream>>>(ids, R, (int)E, bits, counts, chunks, offsets, perm, pos);
   if (rows) {
     const int64_t bytes = cols * es, pieces = (bytes + 15) / 16;

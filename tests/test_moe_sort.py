@@ -257,6 +257,16 @@ def test_offsets_past_32_bits(dev):
 
 
 @gpu
+@pytest.mark.parametrize("routes", [65536, 65537, 64 * 2048, 64 * 2048 + 1, 65 * 2048, 300001, 1 << 22])
+@pytest.mark.parametrize("E,cold", [(1, 0.5), (63, 0.0), (64, 0.1), (2048, 0.3)])
+def test_order_of_many_routes(dev, routes, E, cold):
+    """Chunks few and many, whose counts are added up in one way or the other."""
+    ids = make_ids(routes, 1, E, cold, 21, dev)
+    x = torch.arange(routes, dtype=torch.float32, device=dev)[:, None]
+    check_sorted(S.moe_sort(x, ids, E), x, ids, E)
+
+
+@gpu
 def test_repeats_bit_for_bit(dev):
     T, k, E, K = 300, 8, 32, 1000
     ids, x = make_ids(T, k, E, 0.1, 1, dev), make_x((T, K), torch.float32, 2, dev)
