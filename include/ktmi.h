@@ -120,7 +120,7 @@ int ktmi_combine(const void* out, int dtype, const float* w, int64_t T, int64_t 
  *   pos int32 [tokens, top_k]      pos[r] = the place of route r, ~place for a route of no expert
  *   rows [tokens*top_k, cols]      x[t] at each of its routes' places, zeros past offsets[n_experts]
  * x [tokens, cols] in x_dtype with x_stride elements between rows. rows = NULL (x unused): the
- * order alone. tokens*top_k < 2^31, n_experts <= 2048. Every output is written whole. */
+ * order alone. tokens*top_k < 2^31, top_k <= 65535, n_experts <= 2048. Every output is written whole. */
 int64_t ktmi_moe_sort_workspace(int64_t tokens, int64_t top_k, int64_t n_experts);
 int ktmi_moe_sort(const void* x, int x_dtype, int64_t x_stride, int64_t cols, const int32_t* ids, int64_t tokens,
                   int64_t top_k, int64_t n_experts, void* rows, int32_t* offsets, int32_t* perm, int32_t* pos,
@@ -148,7 +148,8 @@ int ktmi_moe_unsort_grad(const void* dy, int64_t dy_stride, const void* rows, in
  *         2j+1 in its high four bits (codes packed eight to an int32 along cols are the same bytes)
  *   scales [n_experts, rows, ceil(cols/group)] in scale_dtype; zeros uint8 of that shape, or NULL: 8
  *   group: 32, 64, a multiple of 128, or at least cols (one group a row)
- * x rows have x_stride elements between them. Any cols, rows and alignment of codes; scales,
+ * x rows have x_stride elements between them. Any cols, rows (to 2^24) and alignment of codes, at
+ * most 2^23 rows of y (and a grid below 2^32 threads, else KTMI_EINVAL); scales,
  * zeros, x and y as their types require. */
 /* dense: y[t] = W x[t], y [tokens, rows] */
 int ktmi_w4_vec(const void* x, int x_dtype, int64_t x_stride, int64_t cols, const void* codes, const void* scales,

@@ -163,8 +163,9 @@ static int check_routes(const char* what, int dtype, int64_t cols, int64_t token
   KTMI_REQUIRE(cols > 0 && cols <= (1 << 24) && tokens >= 0 && top_k > 0, KTMI_EINVAL,
                "%s: cols %lld (at most 2^24) tokens %lld top_k %lld", what, (long long)cols, (long long)tokens,
                (long long)top_k);
-  KTMI_REQUIRE(top_k <= 0x7FFFFFFF && tokens <= 0x7FFFFFFF / top_k, KTMI_EINVAL, "%s: %lld tokens x top-%lld routes (below 2^31)",
-               what, (long long)tokens, (long long)top_k);
+  KTMI_REQUIRE(top_k <= 65535 && tokens <= 0x7FFFFFFF / top_k, KTMI_EINVAL,
+               "%s: %lld tokens x top-%lld (at most 65535 a token, below 2^31 routes in all)", what, (long long)tokens,
+               (long long)top_k);
   return KTMI_OK;
 }
 
@@ -239,6 +240,7 @@ static int check_w4(const char* what, const W4Args& a, int64_t n) {
                "%s: group %lld (32, 64, a multiple of 128, or at least cols)", what, (long long)a.group);
   KTMI_REQUIRE(n >= 0 && a.top_k > 0 && a.n_routes >= 0, KTMI_EINVAL, "%s: %lld rows of x, top_k %lld", what, (long long)n,
                (long long)a.top_k);
+  KTMI_REQUIRE(a.n_routes <= W4_ROUTES, KTMI_EINVAL, "%s: %lld rows of y (at most 2^23)", what, (long long)a.n_routes);
   if (a.n_routes == 0) return KTMI_OK;
   const int es = a.x_dtype == KTMI_F32 ? 4 : 2, ss = a.scale_dtype == KTMI_F32 ? 4 : 2;
   KTMI_REQUIRE(a.x && a.codes && a.scales && a.y, KTMI_EINVAL, "%s: null pointer", what);
@@ -256,7 +258,6 @@ int ktmi_w4_vec(const void* x, int x_dtype, int64_t x_stride, int64_t cols, cons
                     1, tokens, y, nullptr, x_dtype, scale_dtype, nullptr};
   int rc = check_w4("w4_vec", a, tokens);
   if (rc || tokens == 0) return rc;
-  KTMI_REQUIRE(tokens <= 0x7FFFFFFF, KTMI_EINVAL, "w4_vec: %lld rows (below 2^31)", (long long)tokens);
   return launch_w4(a, (hipStream_t)stream);
 }
 
@@ -292,7 +293,6 @@ int ktmi_moe_w4_sorted(const void* x, int x_dtype, int64_t x_stride, int64_t col
   int rc = check_w4("moe_w4_sorted", a, n_rows);
   if (rc || n_rows == 0) return rc;
   KTMI_REQUIRE(offsets, KTMI_EINVAL, "moe_w4_sorted: null pointer");
-  KTMI_REQUIRE(n_rows <= 0x7FFFFFFF, KTMI_EINVAL, "moe_w4_sorted: %lld rows (below 2^31)", (long long)n_rows);
   return launch_w4(a, (hipStream_t)stream);
 }
 

@@ -50,6 +50,7 @@ int launch_w4_bf16(const W4Args& a, hipStream_t stream);  // by activation type:
 int launch_w4_f16(const W4Args& a, hipStream_t stream);
 int launch_w4_f32(const W4Args& a, hipStream_t stream);
 constexpr int W4_STEP = 128;  // columns of a step: 16 bytes of codes a lane
+constexpr int64_t W4_ROUTES = 1 << 23;  // rows of y of a call, at most: a grid has below 2^32 threads
 constexpr int W4_IDS = 64;    // routes whose ids a wave holds one a lane
 
 // GEMV over raw GGUF rows against q8_1 activations (the decode-window kernel).

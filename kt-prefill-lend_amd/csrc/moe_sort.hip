@@ -32,6 +32,7 @@ constexpr int64_t SORT_CACHED = 256 << 20;  // the last-level cache
 constexpr int SORT_SCAN = 64;
 constexpr int SCAN_WAVES = 16;
 constexpr int ROW_WAVES = 4;      // waves of a row kernel's block, at most
+constexpr int64_t ROW_TOKENS = 1 << 23;  // tokens (blocks) of a row kernel's launch, at most: a grid has below 2^32 threads
 
 __device__ __forceinline__ int key_of(int id, int E) { return id >= 0 && id < E ? id : E; }
 
@@ -523,11 +524,13 @@ int launch_moe_sort(const uint8_t* x, int es, int64_t x_stride, int64_t cols, co
   if (rows) {
     const int64_t bytes = cols * es, pieces = (bytes + 15) / 16;
     const int th = row_threads(pieces);
-    dim3 grid((unsigned)tokens, (unsigned)((pieces + th - 1) / th));
     const bool nt = (int64_t)R * bytes > SORT_CACHED;
     auto kernel = es == 4 ? (nt ? sort_rows_kernel<4, true> : sort_rows_kernel<4, false>)
                           : (nt ? sort_rows_kernel<2, true> : sort_rows_kernel<2, false>);
-    kernel<<<grid, th, 0, stream>>>(x, x_stride * es, bytes, pos, (int)top_k, rows);
+    for (int64_t t = 0; t < tokens; t += ROW_TOKENS) {
+      dim3 grid((unsigned)(tokens - t < ROW_TOKENS ? tokens - t : ROW_TOKENS), (unsigned)((pieces + th - 1) / th));
+      kernel<<<grid, th, 0, stream>>>(x + t * x_stride * es, x_stride * es, bytes, pos + t * top_k, (int)top_k, rows);
+    }
   }
   KTMI_HIP_TRY(hipGetLastError());
   return KTMI_OK;
@@ -542,11 +545,12 @@ void unsort_of(const void* rows, int64_t row_stride, int64_t cols, const float* 
   const int v = cols >= V ? V : 1;
   const int64_t pieces = (cols + v - 1) / v;
   const int th = row_threads(pieces), R = (int)(tokens * top_k);
-  dim3 grid((unsigned)tokens, (unsigned)((pieces + th - 1) / th));
-  if (v == V)
-    unsort_kernel<T, V><<<grid, th, 0, stream>>>((const T*)rows, row_stride, cols, w, pos, (int)top_k, R, (T*)y);
-  else
-    unsort_kernel<T, 1><<<grid, th, 0, stream>>>((const T*)rows, row_stride, cols, w, pos, (int)top_k, R, (T*)y);
+  auto kernel = v == V ? unsort_kernel<T, V> : unsort_kernel<T, 1>;
+  for (int64_t t = 0; t < tokens; t += ROW_TOKENS) {
+    dim3 grid((unsigned)(tokens - t < ROW_TOKENS ? tokens - t : ROW_TOKENS), (unsigned)((pieces + th - 1) / th));
+    kernel<<<grid, th, 0, stream>>>((const T*)rows, row_stride, cols, w ? w + t * top_k : w, pos + t * top_k, (int)top_k, R,
+                                    (T*)y + t * cols);
+  }
 }
 
 template <typename T>
@@ -555,12 +559,11 @@ void unsort_grad_of(const void* dy, int64_t dy_stride, const void* rows, int64_t
   constexpr int V = 16 / sizeof(T);
   const int v = cols >= V ? V : 1;
   const int th = row_threads((cols + v - 1) / v), R = (int)(tokens * top_k);
-  if (v == V)
-    unsort_grad_kernel<T, V><<<(unsigned)tokens, th, 0, stream>>>((const T*)dy, dy_stride, (const T*)rows, row_stride, cols,
-                                                                  w, pos, (int)top_k, R, (T*)drows, dw);
-  else
-    unsort_grad_kernel<T, 1><<<(unsigned)tokens, th, 0, stream>>>((const T*)dy, dy_stride, (const T*)rows, row_stride, cols,
-                                                                  w, pos, (int)top_k, R, (T*)drows, dw);
+  auto kernel = v == V ? unsort_grad_kernel<T, V> : unsort_grad_kernel<T, 1>;
+  for (int64_t t = 0; t < tokens; t += ROW_TOKENS)
+    kernel<<<(unsigned)(tokens - t < ROW_TOKENS ? tokens - t : ROW_TOKENS), th, 0, stream>>>(
+        (const T*)dy + t * dy_stride, dy_stride, (const T*)rows, row_stride, cols, w ? w + t * top_k : w, pos + t * top_k,
+        (int)top_k, R, (T*)drows, dw ? dw + t * top_k : dw);
 }
 
 }  // namespace

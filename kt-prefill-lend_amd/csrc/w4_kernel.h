@@ -699,7 +699,8 @@ int launch_as(const W4Args& a, int64_t items, int64_t expected, hipStream_t stre
   p.deep = (int)(deep < 1 ? 1 : deep);
   p.blocks = (int)((tiles + p.deep - 1) / p.deep);
   const int64_t bytes = p.x_bytes + (KS == 1 && whole > x_bytes ? p.deep * WR * MT * 64 * 16 : 0);
-  KTMI_REQUIRE(items * p.blocks <= 0x7FFFFFFF, KTMI_EINVAL, "w4: %lld blocks (below 2^31)", (long long)(items * p.blocks));
+  KTMI_REQUIRE(items * p.blocks * 64 * KS * WR < 1ll << 32, KTMI_EINVAL, "w4: a grid of %lld x %d threads (below 2^32)",
+               (long long)(items * p.blocks), 64 * KS * WR);
   auto kernel = w4_mfma_kernel<T, SPS, S4, Z, MT, KS, WR>;
   KTMI_REQUIRE(bytes <= W4_LDS_MOST, KTMI_EINVAL, "w4: %lld bytes of LDS", (long long)bytes);
   kernel<<<(unsigned)(items * p.blocks), 64 * KS * WR, bytes, stream>>>(a, p);

@@ -169,7 +169,7 @@ class _Unsort(torch.autograd.Function):
 
 def moe_sort(x: torch.Tensor, ids: torch.Tensor, n_experts: int) -> MoeSorted:
     """The rows of x [T, K] (bf16, f16 or f32) copied to each of their routes' places: ids int32 [T, k],
-    at most 2048 experts. Returns MoeSorted; differentiable in x."""
+    at most 2048 experts, k at most 65535, fewer than 2^31 routes. Returns MoeSorted; differentiable in x."""
     _check_sort(x, ids, n_experts)
     if x.requires_grad and torch.is_grad_enabled():
         return MoeSorted(*_Sort.apply(x, ids, n_experts))
@@ -178,8 +178,8 @@ def moe_sort(x: torch.Tensor, ids: torch.Tensor, n_experts: int) -> MoeSorted:
 
 def moe_unsort(rows: torch.Tensor, topk_w, pos: torch.Tensor) -> torch.Tensor:
     """y[t] = sum over k of topk_w[t, k] * rows[pos[t, k]], [T, K] in the rows' type: rows [T*k, K] in the
-    order of moe_sort, topk_w fp32 [T, k] or None (weights 1), pos its pos. Differentiable in rows and
-    topk_w."""
+    order of moe_sort, topk_w fp32 [T, k] or None (weights 1), pos its pos, which names every row once (so
+    that the rows' gradient is written whole). Differentiable in rows and topk_w."""
     _check_unsort(rows, topk_w, pos)
     if torch.is_grad_enabled() and (rows.requires_grad or (topk_w is not None and topk_w.requires_grad)):
         return _Unsort.apply(rows, topk_w, pos)

@@ -267,6 +267,33 @@ def test_order_of_many_routes(dev, routes, E, cold):
 
 
 @gpu
+@pytest.mark.parametrize("K,dtype", [(4, torch.float32), (2, torch.bfloat16)])
+def test_more_tokens_than_a_launch_takes(dev, K, dtype):
+    T, k, E = (1 << 23) + 3, 2, 9
+    ids = torch.randint(-1, E, (T, k), dtype=torch.int32, device=dev)
+    x = torch.randn((T, K), device=dev).to(dtype).requires_grad_(True)
+    s = S.moe_sort(x, ids, E)
+    _, order = torch.sort(torch.where(ids >= 0, ids, E).reshape(-1), stable=True)
+    hot = ids.reshape(-1)[order] >= 0
+    assert torch.equal(s.perm.long(), torch.where(hot, order, ~order))
+    want = torch.where(hot[:, None], x.detach()[order // k], 0)
+    assert torch.equal(s.rows.detach(), want)
+    # integer weights and values: sums of two terms that are exact in every type
+    rows = torch.randint(-3, 4, s.rows.shape, device=dev).to(dtype).requires_grad_(True)
+    w = torch.randint(-2, 3, (T, k), device=dev).float().requires_grad_(True)
+    dy = torch.randint(-3, 4, (T, K), device=dev).to(dtype)
+    y = S.moe_unsort(rows, w, s.pos)
+    drows, dw = torch.autograd.grad(y, (rows, w), dy)
+    at, there = torch.where(s.pos >= 0, s.pos, ~s.pos).long(), (s.pos >= 0)[..., None]
+    picked = torch.where(there, rows.detach()[at], 0).float()
+    assert torch.equal(y.detach().float(), (picked * w.detach()[..., None]).sum(1))
+    assert torch.equal(dw, (picked * dy[:, None].float()).sum(2))
+    assert torch.equal(drows[at].float(), torch.where(there, w.detach()[..., None] * dy[:, None].float(), 0))
+    dx, = torch.autograd.grad(s.rows, x, rows.detach())
+    assert torch.equal(dx.float(), picked.sum(1))
+
+
+@gpu
 def test_repeats_bit_for_bit(dev):
     T, k, E, K = 300, 8, 32, 1000
     ids, x = make_ids(T, k, E, 0.1, 1, dev), make_x((T, K), torch.float32, 2, dev)
@@ -438,3 +465,11 @@ def test_c_refusals():
                dict(drows=p + 1), dict(k=0)]:
         assert grad(**kw) == -1 and b"moe_unsort_grad" in L.ktmi_last_error(), kw
     assert grad(T=0) == 0 and grad(drows=0, dw=0) == 0
+
+
+def test_c_refuses_more_routes_a_token_than_a_block_takes():
+    L = _lib.lib()
+    p, k = 4096, 65536
+    assert L.ktmi_moe_sort(p, 2, 8, 8, p, 1, k, 3, p, p, p, p, p, 1 << 30, 0) == -1 and b"65535" in L.ktmi_last_error()
+    assert L.ktmi_moe_unsort(p, 2, 8, 8, p, p, 1, k, p, 0) == -1 and b"65535" in L.ktmi_last_error()
+    assert L.ktmi_moe_unsort_grad(p, 8, p, 8, 2, 8, p, p, 1, k, p, p, 0) == -1 and b"65535" in L.ktmi_last_error()

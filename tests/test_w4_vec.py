@@ -395,3 +395,15 @@ def test_c_refusals():
     for kw in [dict(E=0), dict(off=0), dict(R=-1), dict(N=0), dict(y=0)]:
         assert sorted_(**kw) == -1 and b"moe_w4_sorted" in L.ktmi_last_error(), kw
     assert sorted_(R=0) == 0
+
+
+def test_c_refuses_grids_past_32_bits():
+    L = _lib.lib()
+    p, most = 4096, 1 << 23
+    for K in (64, 128):
+        assert L.ktmi_w4_vec(p, 2, K, K, p, p, 2, 0, 32, 8, most + 1, p, 0) == -1 and b"2^23" in L.ktmi_last_error()
+        assert L.ktmi_moe_w4_sorted(p, 2, K, K, p, p, 2, 0, 32, 8, 4, p, most + 1, p, 0) == -1
+        assert b"2^23" in L.ktmi_last_error()
+        assert L.ktmi_moe_w4_vec(p, 2, K, K, p, p, 2, 0, 32, 8, 4, p, 2, most // 2 + 1, p, p, 1 << 40, 0) == -1
+        assert b"2^23" in L.ktmi_last_error()
+    assert L.ktmi_w4_vec(p, 2, 128, 128, p, p, 2, 0, 32, 1 << 24, most, p, 0) == -1 and b"2^32" in L.ktmi_last_error()
