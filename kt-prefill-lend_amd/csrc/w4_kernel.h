@@ -729,12 +729,17 @@ int launch_sps(const W4Args& a, hipStream_t stream) {
                                     : (a.n_routes + rows - 1) / rows;
   // items that have rows, at most but for passes after an expert's first
   const int64_t expected = !a.ids && !a.offsets ? items : a.n_experts < a.n_routes ? a.n_experts : a.n_routes;
-  // Four waves share 16 weight rows (32 of the larger passes) where whole rows a wave would leave CUs idle:
+  // Four waves share 16 weight rows (the larger passes' blocks have 32) where whole rows a wave would leave CUs idle:
   // 7168 x 2048 bf16 dense, one row, 7.4 us; 23 experts of 1024 x 2048, 10.8 us without and 20.4 with
   const bool split = expected * ((a.rows + 63) / 64) < 256;
+  // Larger passes share it by two, 64 weight rows a block, where blocks of 32, one a CU by their LDS, would
+  // be more than the CUs: 7168 x 2048, 64 rows 12.2 us (19.8 of 32); 32 rows, 224 blocks of 32, 11.7 (11.4)
+  const bool wide = expected * ((a.rows + 31) / 32) > 256;
   if constexpr (!F32)
     if (many)
-      return split ? launch_one<T, SPS, 2, 4, 2>(a, items, expected, stream) : launch_one<T, SPS, 2, 1, 4>(a, items, expected, stream);
+      return !split ? launch_one<T, SPS, 2, 1, 4>(a, items, expected, stream)
+             : wide ? launch_one<T, SPS, 2, 2, 4>(a, items, expected, stream)
+                    : launch_one<T, SPS, 2, 4, 2>(a, items, expected, stream);
   return split ? launch_one<T, SPS, 1, 4, 1>(a, items, expected, stream) : launch_one<T, SPS, 1, 1, 4>(a, items, expected, stream);
 }
 

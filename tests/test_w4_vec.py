@@ -308,6 +308,18 @@ def test_graphs_and_streams(dev, T):
     assert all(torch.equal(p, r) for p, r in zip(a + b, step(0) + step(1)))
 
 
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("T,N,K,G", [(64, 4113, 256, 128), (33, 8192, 130, 64), (40, 4200, 512, 32), (200, 1100, 392, 392),
+                                     (70, 3000, 4480, 128)])
+def test_dense_exact_of_many_weight_rows(dev, T, N, K, G, zeros, dtype):
+    """More blocks of 32 weight rows than CUs, fewer of 64 for 17 rows of x and more."""
+    q, s, z = make_weights((), N, K, G, zeros, dtype, 3, dev)
+    x = make_x(T, K, dtype, 5, dev)
+    same(W.w4_vec(x, q, s, z, G), x.double() @ matrix(q, s, z, G, K)[0].t())
+
+
 LARGE_GROUPS = [2 ** 31, 2 ** 32, 2 ** 40, 2 ** 64 + 32]
 
 
