@@ -78,13 +78,12 @@ def _launch_sort(stream, x, ids, n_experts):
     T, K = x.shape
     k = ids.shape[1]
     x, ids = _rows_of(x), ids.contiguous()
-    dev = x.device
-    rows = torch.empty((T * k, K), dtype=x.dtype, device=dev)
-    offsets = torch.empty((n_experts + 1,), dtype=torch.int32, device=dev)
-    perm = torch.empty((T * k,), dtype=torch.int32, device=dev)
-    pos = torch.empty((T, k), dtype=torch.int32, device=dev)
+    rows = x.new_empty((T * k, K))
+    offsets = ids.new_empty((n_experts + 1,))
+    perm = ids.new_empty((T * k,))
+    pos = ids.new_empty((T, k))
     need = L.ktmi_moe_sort_workspace(T, k, n_experts)
-    ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
+    ws = ids.new_empty((need,), dtype=torch.uint8) if need else None
     rc = L.ktmi_moe_sort(x.data_ptr(), _CODES[x.dtype], x.stride(0), K, ids.data_ptr(), T, k, n_experts,
                          rows.data_ptr(), offsets.data_ptr(), perm.data_ptr(), pos.data_ptr(),
                          ws.data_ptr() if need else None, need, stream)
@@ -99,7 +98,7 @@ def _launch_unsort(stream, rows, topk_w, pos):
     rows, pos = _rows_of(rows), pos.contiguous()
     if topk_w is not None:
         topk_w = topk_w.contiguous()
-    y = torch.empty((T, K), dtype=rows.dtype, device=rows.device)
+    y = rows.new_empty((T, K))
     rc = _lib.lib().ktmi_moe_unsort(rows.data_ptr(), _CODES[rows.dtype], rows.stride(0), K,
                                     None if topk_w is None else topk_w.data_ptr(), pos.data_ptr(), T, k, y.data_ptr(),
                                     stream)
@@ -115,8 +114,8 @@ def _launch_unsort_grad(stream, dy, rows, topk_w, pos, want_rows, want_w):
     rows = _rows_of(rows) if want_w else None
     if topk_w is not None:
         topk_w = topk_w.contiguous()
-    drows = torch.empty((T * k, K), dtype=dy.dtype, device=dy.device) if want_rows else None
-    dw = torch.empty((T, k), dtype=torch.float32, device=dy.device) if want_w else None
+    drows = dy.new_empty((T * k, K)) if want_rows else None
+    dw = dy.new_empty((T, k), dtype=torch.float32) if want_w else None
     rc = _lib.lib().ktmi_moe_unsort_grad(dy.data_ptr(), dy.stride(0), rows.data_ptr() if want_w else None,
                                          rows.stride(0) if want_w else K, _CODES[dy.dtype], K,
                                          None if topk_w is None else topk_w.data_ptr(), pos.data_ptr(), T, k,

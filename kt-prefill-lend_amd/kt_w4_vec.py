@@ -71,7 +71,7 @@ def _args(x, codes, scales, zeros, group):
 def _launch_dense(stream, x, codes, scales, zeros, group):
     keep, args = _args(x, codes, scales, zeros, group)
     T, N = x.shape[0], codes.shape[0]
-    y = torch.empty((T, N), dtype=x.dtype, device=x.device)
+    y = x.new_empty((T, N))
     rc = _lib.lib().ktmi_w4_vec(*args, N, T, y.data_ptr(), stream)
     if rc:
         _lib.check(rc, "w4_vec")
@@ -83,9 +83,9 @@ def _launch_routed(stream, x, codes, scales, ids, top_k, zeros, group):
     ids = ids.contiguous()
     T, (E, N) = x.shape[0], codes.shape[:2]
     L = _lib.lib()
-    y = torch.empty((T * top_k, N), dtype=x.dtype, device=x.device)
+    y = x.new_empty((T * top_k, N))
     need = L.ktmi_moe_w4_vec_workspace(T, top_k, E)
-    ws = torch.empty((need,), dtype=torch.uint8, device=x.device) if need else None
+    ws = x.new_empty((need,), dtype=torch.uint8) if need else None
     rc = L.ktmi_moe_w4_vec(*args, N, E, ids.data_ptr(), top_k, T, y.data_ptr(), ws.data_ptr() if need else None, need,
                            stream)
     if rc:
@@ -97,7 +97,7 @@ def _launch_sorted(stream, rows, codes, scales, offsets, zeros, group):
     keep, args = _args(rows, codes, scales, zeros, group)
     offsets = offsets.contiguous()
     R, (E, N) = rows.shape[0], codes.shape[:2]
-    y = torch.empty((R, N), dtype=rows.dtype, device=rows.device)
+    y = rows.new_empty((R, N))
     rc = _lib.lib().ktmi_moe_w4_sorted(*args, N, E, offsets.data_ptr(), R, y.data_ptr(), stream)
     if rc:
         _lib.check(rc, "moe_w4_sorted")
