@@ -20,14 +20,14 @@
 // The activations of the block's rows pass through LDS in column stages, values of each eight in the
 // order 0 2 4 6 1 3 5 7 in which the nibbles come out; columns past the row's end are zeros there.
 //
-// What bounds it: large calls the weights' bytes, of which 3.7 TB/s come (18 experts of 4096 x 7168 bf16,
-// 13 tokens: 74 us for 276 MB; a build of 95 us took 66 with nothing but its loads); small ones the chain
+// What bounds it: large calls the weights' bytes, of which 3.8 TB/s come (18 experts of 4096 x 7168 bf16,
+// 13 tokens: 72 us for 276 MB; a build of 95 us took 66 with nothing but its loads); small ones the chain
 // from the ids to the loads to the sums (one row of 4096 x 7168 8.3 us; a build of 10.0 took 6.3 with
 // nothing but its loads). What it took to get there, the former case: loads and products of a step at a
 // time 115 us; both 64-byte halves of a row's line and the scales of eight steps asked for together 95;
 // row tiles after each other on the same activations, no condition inside a turn of the ring, as many
-// blocks as the chip holds 74. Many rows of x cost their passage through LDS: 4096 x 7168 at 16 rows 18
-// us, at 64 rows 29.
+// blocks as the chip holds 72. Many rows of x cost their passage through LDS: 4096 x 7168 at 16 rows 18
+// us, at 64 rows 27.
 #pragma once
 #include <type_traits>
 
@@ -722,8 +722,8 @@ int launch_one(const W4Args& a, int64_t items, int64_t expected, hipStream_t str
 template <typename T, int SPS>
 int launch_sps(const W4Args& a, hipStream_t stream) {
   constexpr bool F32 = std::is_same<T, float>::value;
-  // rows of an expert, about: 16 a pass, or 32 where there are more (dense 4096 x 7168, bf16: 32 rows 33 us
-  // in one pass of 32, 64 rows 34 in two; in one of 64 with its shorter stages 71)
+  // rows of an expert, about: 16 a pass, or 32 where there are more (dense 4096 x 7168, bf16: 32 rows 26 us
+  // in one pass of 32, 64 rows 27 in two; in one of 64 with its shorter stages 71)
   const int64_t mean = a.offsets ? a.n_routes / a.n_experts : a.ids ? 1 : a.n_routes;
   const bool many = !F32 && mean > 16;
   const int64_t rows = many ? 32 : 16;
