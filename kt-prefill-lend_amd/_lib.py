@@ -134,11 +134,31 @@ def stream_ptr(device=None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def on_device_of(t, fn, *args):
-    """fn(stream handle, *args) with t's device current: the current stream of that device, on which the
-    call's launches and its tensors' allocations are ordered."""
+def _refuse_records(what, tensors):
+    """Refuses calls that torch would record without what the library computes in them: tensors with a
+    forward-mode tangent (the result would have none, a derivative of 0), and traces of torch's own operations
+    (they would hold the outputs' allocations alone)."""
     import torch
 
+    if torch.autograd.forward_ad._current_level >= 0:
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{what} has no forward-mode derivative: call it on the primal tensors")
+    if torch._C._is_tracing():
+        raise RuntimeError(f"{what} cannot be traced: its kernels are no torch operations")
+    if torch._C._len_torch_dispatch_stack() or torch._ops._len_torch_dispatch_stack_pre_dispatch():
+        from torch.fx.experimental.proxy_tensor import get_proxy_mode
+
+        if get_proxy_mode() is not None:
+            raise RuntimeError(f"{what} cannot be traced: its kernels are no torch operations")
+
+
+def on_device_of(what, t, fn, *args):
+    """fn(stream handle, *args) with t's device current: the current stream of that device, on which the
+    call's launches and its tensors' allocations are ordered. what: the call's name in errors."""
+    import torch
+
+    _refuse_records(what, args)
     index = t.get_device()
     if torch._C._cuda_getDevice() == index:
         return fn(torch._C._cuda_getCurrentRawStream(index), *args)

@@ -14,7 +14,8 @@ caching allocator, never synchronise and can be captured into a HIP graph. A cap
 needs, as any in torch, that no graph of the same leaves built outside the capture is alive.
 
 The gradients: of moe_sort with respect to x (the sum of its routes' rows), of moe_unsort with
-respect to the rows and the weights. They are not differentiable a second time.
+respect to the rows and the weights. They are not differentiable a second time. Forward-mode tangents
+(NotImplementedError) and traces by torch.jit.trace or make_fx (RuntimeError) are refused.
 """
 from __future__ import annotations
 
@@ -129,7 +130,7 @@ def _launch_unsort_grad(stream, dy, rows, topk_w, pos, want_rows, want_w):
 class _Sort(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, ids, n_experts):
-        rows, offsets, perm, pos = _lib.on_device_of(x, _launch_sort, x, ids, n_experts)
+        rows, offsets, perm, pos = _lib.on_device_of("moe_sort", x, _launch_sort, x, ids, n_experts)
         ctx.save_for_backward(pos)
         ctx.mark_non_differentiable(offsets, perm, pos)
         ctx.set_materialize_grads(False)
@@ -142,7 +143,7 @@ class _Sort(torch.autograd.Function):
         if drows is None:
             return None, None, None
         pos, = ctx.saved_tensors
-        return _lib.on_device_of(drows, _launch_unsort, drows, None, pos), None, None
+        return _lib.on_device_of("moe_sort's gradient", drows, _launch_unsort, drows, None, pos), None, None
 
     # of a graph for second derivatives: the same without a graph of its own, refused when one is asked for
     once = staticmethod(torch.autograd.function.once_differentiable(lambda ctx, *grads: _Sort.backward(ctx, *grads)))
@@ -153,15 +154,15 @@ class _Unsort(torch.autograd.Function):
     def forward(ctx, rows, topk_w, pos):
         want_w = topk_w is not None and ctx.needs_input_grad[1]
         ctx.save_for_backward(rows if want_w else None, topk_w, pos)
-        return _lib.on_device_of(rows, _launch_unsort, rows, topk_w, pos)
+        return _lib.on_device_of("moe_unsort", rows, _launch_unsort, rows, topk_w, pos)
 
     @staticmethod
     def backward(ctx, dy):
         if torch.is_grad_enabled():
             return _Unsort.once(ctx, dy)
         rows, topk_w, pos = ctx.saved_tensors
-        return (*_lib.on_device_of(dy, _launch_unsort_grad, dy, rows, topk_w, pos, ctx.needs_input_grad[0],
-                                   rows is not None), None)
+        return (*_lib.on_device_of("moe_unsort's gradient", dy, _launch_unsort_grad, dy, rows, topk_w, pos,
+                                   ctx.needs_input_grad[0], rows is not None), None)
 
     once = staticmethod(torch.autograd.function.once_differentiable(lambda ctx, dy: _Unsort.backward(ctx, dy)))
 
@@ -172,7 +173,7 @@ def moe_sort(x: torch.Tensor, ids: torch.Tensor, n_experts: int) -> MoeSorted:
     _check_sort(x, ids, n_experts)
     if x.requires_grad and torch.is_grad_enabled():
         return MoeSorted(*_Sort.apply(x, ids, n_experts))
-    return MoeSorted(*_lib.on_device_of(x, _launch_sort, x, ids, n_experts))
+    return MoeSorted(*_lib.on_device_of("moe_sort", x, _launch_sort, x, ids, n_experts))
 
 
 def moe_unsort(rows: torch.Tensor, topk_w, pos: torch.Tensor) -> torch.Tensor:
@@ -182,4 +183,4 @@ def moe_unsort(rows: torch.Tensor, topk_w, pos: torch.Tensor) -> torch.Tensor:
     _check_unsort(rows, topk_w, pos)
     if torch.is_grad_enabled() and (rows.requires_grad or (topk_w is not None and topk_w.requires_grad)):
         return _Unsort.apply(rows, topk_w, pos)
-    return _lib.on_device_of(rows, _launch_unsort, rows, topk_w, pos)
+    return _lib.on_device_of("moe_unsort", rows, _launch_unsort, rows, topk_w, pos)

@@ -15,7 +15,8 @@ shape, or None for 8 everywhere; group_size: 32, 64, a multiple of 128, or at le
 row). x: bf16, f16 or f32; the weights' values are exact, sums are in fp32 and rounded once to x's
 type. Any K and N (to 2^24), at most 2^23 rows of y. They run on the current stream of x's device, allocate from torch's caching
 allocator, never synchronise and can be captured into a HIP graph. No gradient: inputs that require
-one are refused while gradients are recorded.
+one are refused while gradients are recorded (RuntimeError), inputs with a forward-mode tangent always
+(NotImplementedError), and so are traces by torch.jit.trace or make_fx (RuntimeError).
 """
 from __future__ import annotations
 
@@ -108,7 +109,7 @@ def w4_vec(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros=Non
     """y [T, N] = x W^T for x [T, K] and one matrix, codes [N, ceil(K/2)]; made for up to 64 rows of x."""
     _check("w4_vec", x, codes, scales, zeros, group_size, 0)
     _check_gpu("w4_vec", x, codes, scales, zeros)
-    return _lib.on_device_of(x, _launch_dense, x, codes, scales, zeros, group_size)
+    return _lib.on_device_of("w4_vec", x, _launch_dense, x, codes, scales, zeros, group_size)
 
 
 def moe_w4_vec(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, ids: torch.Tensor, top_k: int, zeros=None,
@@ -122,7 +123,7 @@ def moe_w4_vec(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, ids: 
     if not 0 < top_k <= 65535 or ids.numel() != x.shape[0] * top_k:
         raise ValueError(f"moe_w4_vec: {ids.numel()} ids for {x.shape[0]} rows of x and top_k {top_k}")
     _check_gpu("moe_w4_vec", x, codes, scales, zeros, ids)
-    return _lib.on_device_of(x, _launch_routed, x, codes, scales, ids, top_k, zeros, group_size)
+    return _lib.on_device_of("moe_w4_vec", x, _launch_routed, x, codes, scales, ids, top_k, zeros, group_size)
 
 
 def moe_w4_sorted(rows: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, offsets: torch.Tensor, zeros=None,
@@ -135,4 +136,4 @@ def moe_w4_sorted(rows: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
     if offsets.dim() != 1 or offsets.shape[0] != codes.shape[0] + 1:
         raise ValueError(f"moe_w4_sorted: offsets must be [{codes.shape[0] + 1}], got {list(offsets.shape)}")
     _check_gpu("moe_w4_sorted", rows, codes, scales, zeros, offsets)
-    return _lib.on_device_of(rows, _launch_sorted, rows, codes, scales, offsets, zeros, group_size)
+    return _lib.on_device_of("moe_w4_sorted", rows, _launch_sorted, rows, codes, scales, offsets, zeros, group_size)

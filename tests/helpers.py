@@ -80,3 +80,24 @@ def scale_f16_fields(rows: np.ndarray, t: int, factor: float) -> np.ndarray:
         assert np.all(np.isfinite(s)) and np.array_equal(s.astype(np.float32), h.astype(np.float32) * factor)
         b[:, :, off:off + 2] = s.view(np.uint8)
     return out
+
+
+def check_refused_records(name, call, tensors):
+    """A call that torch cannot record is refused: a forward-mode tangent on any of the tensors, traces of
+    torch's operations."""
+    import pytest
+    import torch
+    from torch.autograd import forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    for i in range(len(tensors)):
+        for grad in (False, True):
+            with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+                dual = [forward_ad.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate(tensors)]
+                with pytest.raises(NotImplementedError, match=name):
+                    call(*dual)
+    with pytest.raises(RuntimeError, match=f"{name} cannot be traced"):
+        torch.jit.trace(call, tensors, check_trace=False)
+    for pre in (False, True):
+        with pytest.raises(RuntimeError, match=f"{name} cannot be traced"):
+            make_fx(call, pre_dispatch=pre)(*tensors)

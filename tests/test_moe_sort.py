@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import kt_prefill_lend_amd.kt_moe_sort as S
+from helpers import check_refused_records
 from kt_prefill_lend_amd import _lib
 
 gpu = pytest.mark.gpu
@@ -473,3 +474,40 @@ def test_c_refuses_more_routes_a_token_than_a_block_takes():
     assert L.ktmi_moe_sort(p, 2, 8, 8, p, 1, k, 3, p, p, p, p, p, 1 << 30, 0) == -1 and b"65535" in L.ktmi_last_error()
     assert L.ktmi_moe_unsort(p, 2, 8, 8, p, p, 1, k, p, 0) == -1 and b"65535" in L.ktmi_last_error()
     assert L.ktmi_moe_unsort_grad(p, 8, p, 8, 2, 8, p, p, 1, k, p, p, 0) == -1 and b"65535" in L.ktmi_last_error()
+
+
+# ---------------------------------------------------------------- what torch would record without the kernels
+
+def calls_of_tensors(dev):
+    """name -> (call, its tensors that could carry a derivative); sizes are the smallest."""
+    x, rows = torch.ones(2, 4, device=dev), torch.ones(4, 4, device=dev)
+    ids, w = torch.zeros(2, 2, dtype=torch.int32, device=dev), torch.ones(2, 2, device=dev)
+    pos = torch.arange(4, dtype=torch.int32, device=dev).reshape(2, 2)
+    return {"moe_sort": (lambda x: S.moe_sort(x, ids, 3).rows, (x,)),
+            "moe_unsort": (lambda rows, w: S.moe_unsort(rows, w, pos), (rows, w))}
+
+
+@pytest.mark.filterwarnings("ignore:Converting a tensor")
+@pytest.mark.parametrize("name", ["moe_sort", "moe_unsort"])
+def test_records_without_the_kernels_are_refused(monkeypatch, name):
+    monkeypatch.setattr(S, "_check_gpu", lambda *a: None)
+    check_refused_records(name, *calls_of_tensors("cpu")[name])
+
+
+@gpu
+@pytest.mark.filterwarnings("ignore:Converting a tensor")
+@pytest.mark.parametrize("name", ["moe_sort", "moe_unsort"])
+def test_records_without_the_kernels_are_refused_on_the_gpu(dev, name):
+    from torch.autograd import forward_ad
+
+    call, tensors = calls_of_tensors(dev)[name]
+    want = call(*tensors)
+    check_refused_records(name, call, tensors)
+    with forward_ad.dual_level():  # a level by itself changes nothing
+        assert torch.equal(call(*tensors), want)
+        # a tangent of what comes back through the gradient
+        leaves = [t.clone().requires_grad_(True) for t in tensors]
+        y = call(*leaves)
+        with pytest.raises(NotImplementedError, match=f"{name}'s gradient"):
+            torch.autograd.grad(y, leaves, forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)))
+    assert torch.equal(call(*tensors), want)

@@ -9,6 +9,7 @@ import pytest
 import torch
 
 import kt_prefill_lend_amd.kt_w4_vec as W
+from helpers import check_refused_records
 from kt_prefill_lend_amd import _lib
 
 gpu = pytest.mark.gpu
@@ -419,3 +420,32 @@ def test_c_refuses_grids_past_32_bits():
         assert L.ktmi_moe_w4_vec(p, 2, K, K, p, p, 2, 0, 32, 8, 4, p, 2, most // 2 + 1, p, p, 1 << 40, 0) == -1
         assert b"2^23" in L.ktmi_last_error()
     assert L.ktmi_w4_vec(p, 2, 128, 128, p, p, 2, 0, 32, 1 << 24, most, p, 0) == -1 and b"2^32" in L.ktmi_last_error()
+
+
+# ---------------------------------------------------------------- what torch would record without the kernels
+
+
+def record_calls(dev):
+    """name -> (call, its tensors that could carry a derivative)."""
+    x, q, s = torch.ones(2, 64, device=dev), torch.zeros((3, 32), dtype=torch.uint8, device=dev), torch.ones(3, 2, device=dev)
+    ids, offsets = torch.zeros(2, dtype=torch.int32, device=dev), torch.tensor([0, 2], dtype=torch.int32, device=dev)
+    return {"w4_vec": (lambda x, s: W.w4_vec(x, q, s, None, 32), (x, s)),
+            "moe_w4_vec": (lambda x, s: W.moe_w4_vec(x, q[None], s, ids, 1, None, 32), (x, s[None])),
+            "moe_w4_sorted": (lambda x, s: W.moe_w4_sorted(x, q[None], s, offsets, None, 32), (x, s[None]))}
+
+
+@pytest.mark.filterwarnings("ignore:Converting a tensor")
+@pytest.mark.parametrize("name", ["w4_vec", "moe_w4_vec", "moe_w4_sorted"])
+def test_records_without_the_kernels_are_refused(monkeypatch, name):
+    monkeypatch.setattr(W, "_check_gpu", lambda *a: None)
+    check_refused_records(name, *record_calls("cpu")[name])
+
+
+@gpu
+@pytest.mark.filterwarnings("ignore:Converting a tensor")
+@pytest.mark.parametrize("name", ["w4_vec", "moe_w4_vec", "moe_w4_sorted"])
+def test_records_without_the_kernels_are_refused_on_the_gpu(dev, name):
+    call, tensors = record_calls(dev)[name]
+    want = call(*tensors)
+    check_refused_records(name, call, tensors)
+    assert torch.equal(call(*tensors), want)
