@@ -171,7 +171,7 @@ static int check_routes(const char* what, int dtype, int64_t cols, int64_t token
 
 int64_t ktmi_moe_sort_workspace(int64_t tokens, int64_t top_k, int64_t n_experts) {
   if (tokens <= 0 || top_k <= 0 || n_experts <= 0 || tokens > 0x7FFFFFFF / top_k) return 0;
-  return moe_sort_counts(tokens * top_k) * (n_experts + 1) * (int64_t)sizeof(int);
+  return moe_sort_counts(tokens, top_k) * (n_experts + 1) * (int64_t)sizeof(int);
 }
 
 int ktmi_moe_sort(const void* x, int x_dtype, int64_t x_stride, int64_t cols, const int32_t* ids, int64_t tokens,

@@ -14,9 +14,9 @@ int launch_combine(const void* out, int dtype, const float* w, int64_t T, int64_
                    hipStream_t stream);
 
 // Tokens sorted by expert and back (moe_sort.hip). x_stride, row_stride, dy_stride in elements, es
-// the bytes of one; counts: moe_sort_counts(routes) * (E + 1) ints; rows = NULL: the order alone.
+// the bytes of one; counts: moe_sort_counts(tokens, top_k) * (E + 1) ints; rows = NULL: the order alone.
 constexpr int64_t SORT_MAX_EXPERTS = 2048;
-int64_t moe_sort_counts(int64_t routes);
+int64_t moe_sort_counts(int64_t tokens, int64_t top_k);
 int launch_moe_sort(const uint8_t* x, int es, int64_t x_stride, int64_t cols, const int32_t* ids, int64_t tokens,
                     int64_t top_k, int64_t E, uint8_t* rows, int32_t* offsets, int32_t* perm, int32_t* pos, int* counts,
                     hipStream_t stream);

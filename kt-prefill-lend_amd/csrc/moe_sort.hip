@@ -22,9 +22,22 @@ namespace {
 
 constexpr int SORT_THREADS = 256;
 constexpr int SORT_MAX_PER = 8;   // routes of a thread of the order's two kernels, at most
-// Routes of a call that takes one launch. 2048 bf16 columns, 8 routes a token: 5120 routes 13.0 us in one
-// launch and 13.4 in three, 8192 20.0 and 15.2, 16376 43.4 and 21.6 (every block reads all ids).
+// Routes of a call that takes one launch, at most. 2048 bf16 columns, 8 routes a token: 5120 routes 13.0 us in
+// one launch and 13.4 in three, 8192 20.0 and 15.2, 16376 43.4 and 21.6 (every block reads all ids).
 constexpr int SORT_SMALL = 4096;
+// Routes a token of one launch, at most: a block takes its token's all at once. Of more, 16 at a time, the launches of
+// the order and the copies won at every size: 17 a token, 60 tokens of 2048 bf16 columns 10.9 and 10.7 us, 240 tokens
+// 23.0 and 12.4; 32 a token, one token 13.3 and 9.6.
+constexpr int SORT_SMALL_K = 16;
+// Comparisons of one launch, at most: every block (a token and 4 KB of its row) holds its token's routes against all
+// ids, 8 of them or 16 (which counts double), so few routes a token and wide rows cost it most. Against the launches of
+// the order and the copies, us: the order of 4096 routes 7.4 and 7.2 at 8 a token (2^24 comparisons), 12.5 and 7.4 at 2
+// (2^26), 20.7 and 7.3 at 1, of 4000 at 10 11.5 and 7.3 (2^25.6), of 2000 7.5 and 7.1 (2^23.6). With 7168 f32 columns 4096
+// routes 28.9 and 27.9 at 8 (2^26.8), 119 and 42.3 at 1 (2^29.8); 2048 14.0 and 18.2 at 8 (2^24.8); 1024 at 1 16.8 and 16.8
+// (2^25.8). Up to SORT_NO_WS comparisons of the order it is one launch whatever the rows' width, which needs no
+// workspace: 512 routes at 1, 7168 f32 columns, 10.3 and 10.8.
+constexpr int64_t SORT_ORDER_WORK = 1 << 24, SORT_ROWS_WORK = 1 << 26, SORT_NO_WS = 1 << 22;
+constexpr int SORT_PIECE = 4096;  // bytes of a row that a block of the one launch copies
 constexpr int64_t SORT_CACHED = 256 << 20;  // the last-level cache
 // Chunks up to which every chunk adds up the counts of all by itself; of more they are added up once, in a
 // launch of its own (else the work would grow with the routes' square). The order of 256 keys: 64 chunks
@@ -213,15 +226,16 @@ __device__ __forceinline__ void store16(void* p, const u32x4_t& v) {
     *(u32x4_a2_t*)p = v;
 }
 
-// A call of up to SORT_SMALL routes in one launch: block (token, piece of its row) counts the places of
+// A call of few routes (sort_in_one) in one launch: block (token, piece of its row) counts the places of
 // the token's routes itself, against all ids, while its part of the row is on its way; the block past
-// the last token makes the offsets. G routes of the token at a time. key << 14 | route orders the routes by one comparison.
+// the last token makes the offsets. G: room for the token's routes. key << 14 | route orders the routes by one comparison.
 template <int ES, int G>
 __global__ __launch_bounds__(SORT_THREADS) void sort_small_kernel(const uint8_t* __restrict__ x, int64_t x_stride,
                                                                   int64_t bytes, const int32_t* __restrict__ ids,
                                                                   int tokens, int top_k, int E,
                                                                   int32_t* __restrict__ offsets, int32_t* __restrict__ perm,
                                                                   int32_t* __restrict__ pos, uint8_t* __restrict__ rows) {
+  static_assert(SORT_PIECE == 16 * SORT_THREADS, "a thread copies 16 bytes");
   static_assert(SORT_SMALL <= 1 << 14 && SORT_MAX_EXPERTS < 1 << 17, "an order fits 31 bits");
   extern __shared__ int lds[];  // the last block's E + 1 counts
   __shared__ int part[4][G];
@@ -247,49 +261,46 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_small_kernel(const uint8_t*
   u32x4_t v = {0, 0, 0, 0};
   const u32x4_t zero = v;
   if (rows && bytes >= 16 && at < bytes) v = load16(x + t * x_stride + b);
-  for (int j0 = 0; j0 < top_k; j0 += G) {
-    int mine[G], count[G];
+  int mine[G], count[G];
 #pragma unroll
-    for (int j = 0; j < G; ++j) {
-      const int r = t * top_k + (j0 + j < top_k ? j0 + j : top_k - 1);
-      mine[j] = key_of(ids[r], E) << 14 | r;
-      count[j] = 0;
+  for (int j = 0; j < G; ++j) {
+    const int r = t * top_k + (j < top_k ? j : top_k - 1);
+    mine[j] = key_of(ids[r], E) << 14 | r;
+    count[j] = 0;
+  }
+  for (int r0 = 64 * wave; r0 < R; r0 += 4 * SORT_THREADS) {  // four loads on their way at once
+    int id[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) id[i] = ids[r0 + i * SORT_THREADS + lane < R ? r0 + i * SORT_THREADS + lane : R - 1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = r0 + i * SORT_THREADS + lane;
+      const int order = r < R ? key_of(id[i], E) << 14 | r : 0x7FFFFFFF;
+#pragma unroll
+      for (int j = 0; j < G; ++j) count[j] += __popcll(__ballot(order < mine[j]));
     }
-    for (int r0 = 64 * wave; r0 < R; r0 += 4 * SORT_THREADS) {  // four loads on their way at once
-      int id[4];
+  }
+  if (lane == 0)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) id[i] = ids[r0 + i * SORT_THREADS + lane < R ? r0 + i * SORT_THREADS + lane : R - 1];
+    for (int j = 0; j < G; ++j) part[wave][j] = count[j];
+  __syncthreads();
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = r0 + i * SORT_THREADS + lane;
-        const int order = r < R ? key_of(id[i], E) << 14 | r : 0x7FFFFFFF;
-#pragma unroll
-        for (int j = 0; j < G; ++j) count[j] += __popcll(__ballot(order < mine[j]));
+  for (int j = 0; j < G; ++j) {
+    if (j < top_k) {
+      const int p = part[0][j] + part[1][j] + part[2][j] + part[3][j];
+      const bool valid = mine[j] >> 14 < E;
+      const int r = t * top_k + j;
+      if (blockIdx.y == 0 && threadIdx.x == 0) {
+        perm[p] = valid ? r : ~r;
+        pos[r] = valid ? p : ~p;
       }
-    }
-    if (j0) __syncthreads();
-    if (lane == 0)
-#pragma unroll
-      for (int j = 0; j < G; ++j) part[wave][j] = count[j];
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < G; ++j) {
-      if (j0 + j < top_k) {
-        const int p = part[0][j] + part[1][j] + part[2][j] + part[3][j];
-        const bool valid = mine[j] >> 14 < E;
-        const int r = t * top_k + j0 + j;
-        if (blockIdx.y == 0 && threadIdx.x == 0) {
-          perm[p] = valid ? r : ~r;
-          pos[r] = valid ? p : ~p;
-        }
-        if (rows && at < bytes) {
-          if (bytes >= 16) {
-            store16(rows + p * bytes + b, valid ? v : zero);
-          } else {
-            using U = typename std::conditional<ES == 4, uint32_t, uint16_t>::type;
-            for (int64_t i = 0; i < bytes / ES; ++i)
-              ((U*)(rows + p * bytes))[i] = valid ? ((const U*)(x + t * x_stride))[i] : (U)0;
-          }
+      if (rows && at < bytes) {
+        if (bytes >= 16) {
+          store16(rows + p * bytes + b, valid ? v : zero);
+        } else {
+          using U = typename std::conditional<ES == 4, uint32_t, uint16_t>::type;
+          for (int64_t i = 0; i < bytes / ES; ++i)
+            ((U*)(rows + p * bytes))[i] = valid ? ((const U*)(x + t * x_stride))[i] : (U)0;
         }
       }
     }
@@ -492,9 +503,19 @@ static int64_t sort_chunks(int64_t routes) {
   const int64_t chunk = sort_per(routes) * SORT_THREADS;
   return (routes + chunk - 1) / chunk;
 }
-int64_t moe_sort_counts(int64_t routes) {
-  if (routes <= SORT_SMALL) return 0;
-  const int64_t chunks = sort_chunks(routes);
+// Comparisons of the order in one launch; where it does not take the routes, more than any limit
+static int64_t sort_work(int64_t tokens, int64_t top_k) {
+  if (tokens * top_k > SORT_SMALL || top_k > SORT_SMALL_K) return INT64_MAX;
+  return tokens * (tokens * top_k) * (top_k > 8 ? 32 : 8);
+}
+static bool sort_in_one(int64_t tokens, int64_t top_k, int64_t pieces) {  // pieces of a row, 0: the order alone
+  const int64_t work = sort_work(tokens, top_k);
+  if (work <= SORT_NO_WS) return true;
+  return pieces ? work <= SORT_ROWS_WORK / pieces : work <= SORT_ORDER_WORK;
+}
+int64_t moe_sort_counts(int64_t tokens, int64_t top_k) {
+  if (sort_work(tokens, top_k) <= SORT_NO_WS) return 0;
+  const int64_t chunks = sort_chunks(tokens * top_k);
   return chunks + 1;  // and their totals, of many chunks
 }
 
@@ -504,9 +525,10 @@ int launch_moe_sort(const uint8_t* x, int es, int64_t x_stride, int64_t cols, co
   const int R = (int)(tokens * top_k), n = (int)E + 1;
   int bits = 0;
   while ((n - 1) >> bits) ++bits;
-  if (R <= SORT_SMALL) {
-    const int64_t bytes = rows ? cols * es : 1, per = 16 * SORT_THREADS;
-    dim3 grid((unsigned)tokens + 1, (unsigned)((bytes + per - 1) / per));
+  const int64_t row_pieces = rows ? (cols * es + SORT_PIECE - 1) / SORT_PIECE : 0;
+  if (sort_in_one(tokens, top_k, row_pieces)) {
+    const int64_t bytes = rows ? cols * es : 1;
+    dim3 grid((unsigned)tokens + 1, rows ? (unsigned)row_pieces : 1);
     auto kernel = es == 4 ? (top_k > 8 ? sort_small_kernel<4, 16> : sort_small_kernel<4, 8>)
                           : (top_k > 8 ? sort_small_kernel<2, 16> : sort_small_kernel<2, 8>);
     kernel<<<grid, SORT_THREADS, n * sizeof(int), stream>>>(x, x_stride * es, bytes, ids, (int)tokens, (int)top_k, (int)E,

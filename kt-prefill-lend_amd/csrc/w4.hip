@@ -20,7 +20,7 @@ int64_t ints(int64_t n) { return (n + 3) / 4 * 4; }
 int64_t w4_workspace(int64_t tokens, int64_t top_k, int64_t E) {
   const int64_t R = tokens * top_k;
   if (R <= W4_IDS) return 0;
-  return 4 * (ints(E + 1) + 2 * ints(R) + ints(moe_sort_counts(R) * (E + 1)));
+  return 4 * (ints(E + 1) + 2 * ints(R) + ints(moe_sort_counts(tokens, top_k) * (E + 1)));
 }
 
 int launch_w4(const W4Args& a, hipStream_t stream) {

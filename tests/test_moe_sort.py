@@ -511,3 +511,44 @@ def test_records_without_the_kernels_are_refused_on_the_gpu(dev, name):
         with pytest.raises(NotImplementedError, match=f"{name}'s gradient"):
             torch.autograd.grad(y, leaves, forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)))
     assert torch.equal(call(*tensors), want)
+
+
+# ---------------------------------------------------------------- few routes a token, wide rows
+
+def test_workspace_follows_the_order_work():
+    """Few routes a token make every block of the one launch dearer: such calls may take the chunked order, so
+    they have its workspace; decode-sized calls have none."""
+    L = _lib.lib()
+    for T, k in [(1, 8), (64, 8), (77, 10), (512, 1), (0, 4)]:
+        assert L.ktmi_moe_sort_workspace(T, k, 256) == 0, (T, k)
+    for T, k in [(4096, 1), (2048, 2), (1025, 1), (1024, 4), (4097, 1), (1, 4096), (3, 17)]:
+        assert L.ktmi_moe_sort_workspace(T, k, 256) >= 4 * 257 * 2, (T, k)
+    assert L.ktmi_moe_sort(4096, 2, 8, 8, 4096, 4096, 1, 256, 4096, 4096, 4096, 4096, None, 0, 0) == -4
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,k,E,K,cold", [
+    (4096, 1, 256, 40, 0.2), (4095, 1, 2048, 2050, 0.0), (2048, 2, 300, 1030, 0.1), (1025, 1, 5, 9000, 0.3),
+    (1024, 4, 129, 7001, 0.0), (513, 1, 16, 4100, 0.1), (512, 8, 64, 5000, 0.2), (256, 16, 33, 3000, 0.0),
+    (200, 20, 40, 2100, 0.1), (400, 10, 40, 2100, 0.1), (1, 4096, 2000, 100, 0.1), (3, 17, 5, 50, 0.3)])
+def test_sort_few_routes_a_token(dev, T, k, E, K, cold, dtype):
+    ids, x = make_ids(T, k, E, cold, T + K, dev), make_x((T, K), dtype, 3, dev)
+    check_sorted(S.moe_sort(x, ids, E), x, ids, E)
+
+
+@gpu
+@pytest.mark.parametrize("T,k", [(1, 8), (512, 1), (513, 1), (1448, 1), (1449, 1), (2048, 2), (4096, 1), (512, 8), (1365, 3),
+                                 (1, 17), (240, 17), (1, 4096), (256, 16)])
+def test_order_alone(dev, T, k):
+    """Without rows, with exactly the workspace that the query names."""
+    E, L = 130, _lib.lib()
+    ids = make_ids(T, k, E, 0.1, T, dev)
+    need = L.ktmi_moe_sort_workspace(T, k, E)
+    off, perm, pos = (torch.full((n,), 77, dtype=torch.int32, device=dev) for n in (E + 1, T * k, T * k))
+    ws = torch.full((need + 64,), 93, dtype=torch.uint8, device=dev)
+    _lib.check(L.ktmi_moe_sort(None, 2, 0, 8, ids.data_ptr(), T, k, E, None, off.data_ptr(), perm.data_ptr(), pos.data_ptr(),
+                               ws.data_ptr(), need, _lib.stream_ptr(dev)))
+    for got, want in zip((off, perm, pos.reshape(T, k)), plain_order(ids, E)):
+        assert np.array_equal(got.cpu().numpy(), want)
+    assert (ws[need:] == 93).all()
