@@ -253,7 +253,7 @@ __global__ __launch_bounds__(64 * KS * WR) void w4_mfma_kernel(W4Args a, W4Plan 
     } else if (a.offsets) {
       const int items = gridDim.x / p.blocks, begin = a.offsets[0], end = a.offsets[a.n_experts];
       for (int64_t r = item; r < begin && r < a.n_routes; r += items) zero(r);
-      for (int64_t r = (end > 0 ? end : 0) + item; r < a.n_routes; r += items) zero(a.perm ? ~a.perm[r] : r);
+      for (int64_t r = (end > 0 ? (int64_t)end : 0) + item; r < a.n_routes; r += items) zero(a.perm ? ~a.perm[r] : r);
     }
   };
   if (m == 0) return zero_rows();

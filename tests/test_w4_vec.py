@@ -449,3 +449,26 @@ def test_records_without_the_kernels_are_refused_on_the_gpu(dev, name):
     want = call(*tensors)
     check_refused_records(name, call, tensors)
     assert torch.equal(call(*tensors), want)
+
+
+# K, group: rows that end with a word of codes and rows that do not
+WIDE = [(128, 32), (130, 64), (256, 128), (192, 64), (131, 128)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N", [20, 17000])
+@pytest.mark.parametrize("K,G", WIDE)
+def test_ids_and_offsets_outside_the_range_on_the_matrix_cores(dev, K, G, N, dtype):
+    E = 3
+    q, s, z = make_weights((E,), N, K, G, True, dtype, 8, dev)
+    x = make_x(6, K, dtype, 9, dev)
+    ids = torch.tensor([0, 3, 2, -1, 2 ** 31 - 1, -2 ** 31], dtype=torch.int32, device=dev)
+    same(W.moe_w4_vec(x, q, s, ids, 1, z, G), routed(x, q, s, z, G, ids, 1)[0])
+    more = ids.repeat(12)  # past the ids that a wave holds
+    same(W.moe_w4_vec(x, q, s, more, 12, z, G), routed(x, q, s, z, G, more, 12)[0])
+    # segments past the rows are cut at them, rows in none are zeros
+    for offsets, of in [([-5, 2, 4, 900], [0, 0, 1, 1, 2, 2]), ([2, 2, 5, 5], [-1, -1, 1, 1, 1, -1]), ([9, 9, 9, 9], [-1] * 6),
+                        ([-9, -9, -9, -1], [-1] * 6), ([0, 6, 6, 2 ** 31 - 1], [0] * 6), ([-2 ** 31, 1, 1, 6], [0, 2, 2, 2, 2, 2])]:
+        y = W.moe_w4_sorted(x, q, s, torch.tensor(offsets, dtype=torch.int32, device=dev), z, G)
+        same(y, routed(x, q, s, z, G, torch.tensor(of, device=dev), 1)[0])
