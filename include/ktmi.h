@@ -142,7 +142,7 @@ int ktmi_moe_unsort_grad(const void* dy, int64_t dy_stride, const void* rows, in
 
 /* ---- products with 4-bit weights and group scales ---------------------------------
  * y[r, n] = sum_g scale[e, n, g] * sum_{c in group g} (code[e, n, c] - zero[e, n, g]) * x[r, c], summed
- * in fp32 and rounded once to x's type. For checkpoints of plain 4-bit codes (no ggml type); no
+ * in fp32 and rounded once to x's type (bits of fp32 x below 2^-133 may be left out). For checkpoints of plain 4-bit codes (no ggml type); no
  * counterpart in the reference.
  *   codes uint8 [n_experts, rows, ceil(cols/2)]: byte j of a row holds code 2j in its low and
  *         2j+1 in its high four bits (codes packed eight to an int32 along cols are the same bytes)
@@ -167,6 +167,17 @@ int ktmi_moe_w4_vec(const void* x, int x_dtype, int64_t x_stride, int64_t cols, 
 int ktmi_moe_w4_sorted(const void* x, int x_dtype, int64_t x_stride, int64_t cols, const void* codes,
                        const void* scales, int scale_dtype, const void* zeros, int64_t group, int64_t rows,
                        int64_t n_experts, const int32_t* offsets, int64_t n_rows, void* y, void* stream);
+/* The kernel that such a call takes: by = KTMI_W4_DENSE, _IDS or _SORTED for n_rows rows of y. */
+enum { KTMI_W4_DENSE = 0, KTMI_W4_IDS = 1, KTMI_W4_SORTED = 2 };
+typedef struct ktmi_w4_kernel {
+  int32_t x_rows;       /* rows of x a pass, at most; 1: the kernel of rows below 128 columns */
+  int32_t col_waves;    /* waves that share a row's columns */
+  int32_t weight_rows;  /* weight rows that a block works on at a time */
+  int32_t tiles;        /* of so many rows, after each other in a block, at most */
+  int32_t staged;       /* 1: x passes through LDS in more than one part */
+} ktmi_w4_kernel;
+int ktmi_w4_kernel_of(int by, int x_dtype, int64_t cols, int64_t group, int64_t rows, int64_t n_experts, int64_t n_rows,
+                      ktmi_w4_kernel* kernel);
 
 /* ---- one hot-expert MoE layer -----------------------------------------------------
  * The GPU half of a layer: routes (t, k) with slot_ids[t*top_k+k] >= 0 run the expert in

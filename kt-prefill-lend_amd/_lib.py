@@ -14,6 +14,7 @@ LIB_PATH = Path(os.environ.get("KTMI_LIB", Path(__file__).resolve().parent / "li
 
 KTMI_OK = 0
 KTMI_F32, KTMI_F16, KTMI_BF16 = 0, 1, 2
+W4_DENSE, W4_IDS, W4_SORTED = 0, 1, 2
 MODE_AUTO, MODE_GEMV, MODE_GROUPED, MODE_DECODE = 0, 1, 2, 3
 STAGE_EVENTS = 6
 NOALLOC_SCRATCH_BYTES = 64 << 20  # KTMI_NOALLOC_SCRATCH_BYTES
@@ -47,6 +48,16 @@ class ktmi_bank(C.Structure):
     ]
 
 
+class ktmi_w4_kernel(C.Structure):
+    _fields_ = [
+        ("x_rows", C.c_int32),
+        ("col_waves", C.c_int32),
+        ("weight_rows", C.c_int32),
+        ("tiles", C.c_int32),
+        ("staged", C.c_int32),
+    ]
+
+
 # name -> (restype, argtypes); every symbol declared in include/ktmi.h
 SIGNATURES = {
     "ktmi_last_error": (C.c_char_p, []),
@@ -70,6 +81,7 @@ SIGNATURES = {
     "ktmi_moe_w4_vec": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _i32, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp,
                                _i64, _vp]),
     "ktmi_moe_w4_sorted": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _i32, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
+    "ktmi_w4_kernel_of": (_i32, [_i32, _i32, _i64, _i64, _i64, _i64, _i64, C.POINTER(ktmi_w4_kernel)]),
     "ktmi_moe_layer_workspace": (_i64, [C.POINTER(ktmi_layer), _i64, _i64, _i32]),
     "ktmi_moe_layer": (_i32, [C.POINTER(ktmi_layer), _vp, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _i32, _vp]),
     "ktmi_moe_layer_mode": (_i32, [C.POINTER(ktmi_layer), _i64, _i64]),

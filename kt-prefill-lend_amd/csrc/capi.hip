@@ -296,6 +296,19 @@ int ktmi_moe_w4_sorted(const void* x, int x_dtype, int64_t x_stride, int64_t col
   return launch_w4(a, (hipStream_t)stream);
 }
 
+int ktmi_w4_kernel_of(int by, int x_dtype, int64_t cols, int64_t group, int64_t rows, int64_t n_experts, int64_t n_rows,
+                      ktmi_w4_kernel* kernel) {
+  g_err[0] = 0;
+  KTMI_REQUIRE(by >= KTMI_W4_DENSE && by <= KTMI_W4_SORTED && kernel && n_rows > 0, KTMI_EINVAL,
+               "w4_kernel_of: by %d, %lld rows, or a null pointer", by, (long long)n_rows);
+  static const int32_t named = 0;  // stands in for the tensors, which the choice does not read
+  const W4Args a = {&named, cols, cols, (const uint8_t*)&named, &named, nullptr, group, rows, by == KTMI_W4_DENSE ? 1 : n_experts,
+                    by == KTMI_W4_IDS ? &named : nullptr, by == KTMI_W4_SORTED ? &named : nullptr, 1, n_rows, (void*)&named,
+                    (uint8_t*)&named, x_dtype, KTMI_F32, nullptr};
+  int rc = check_w4("w4_kernel_of", a, n_rows);
+  return rc ? rc : launch_w4(a, nullptr, kernel);
+}
+
 // ---- scratch for ktmi_moe_layer_noalloc
 // A file-scope device array that stands in for the caller's workspace. In host code its
 // name is a host-side stand-in, not a device address: the address on each device comes

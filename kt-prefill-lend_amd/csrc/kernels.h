@@ -45,10 +45,12 @@ struct W4Args {
 };
 constexpr int W4_LDS_MOST = 152 << 10;
 int64_t w4_workspace(int64_t tokens, int64_t top_k, int64_t n_experts);
-int launch_w4(const W4Args& a, hipStream_t stream);
-int launch_w4_bf16(const W4Args& a, hipStream_t stream);  // by activation type: one pass without a sort
-int launch_w4_f16(const W4Args& a, hipStream_t stream);
-int launch_w4_f32(const W4Args& a, hipStream_t stream);
+// tell: takes what the call would launch, and nothing is launched
+int launch_w4(const W4Args& a, hipStream_t stream, ktmi_w4_kernel* tell = nullptr);
+// by activation type: one pass without a sort
+int launch_w4_bf16(const W4Args& a, hipStream_t stream, ktmi_w4_kernel* tell);
+int launch_w4_f16(const W4Args& a, hipStream_t stream, ktmi_w4_kernel* tell);
+int launch_w4_f32(const W4Args& a, hipStream_t stream, ktmi_w4_kernel* tell);
 constexpr int W4_STEP = 128;  // columns of a step: 16 bytes of codes a lane
 constexpr int64_t W4_ROUTES = 1 << 23;  // rows of y of a call, at most: a grid has below 2^32 threads
 constexpr int W4_IDS = 64;    // routes whose ids a wave holds one a lane

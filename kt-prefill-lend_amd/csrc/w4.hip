@@ -6,9 +6,10 @@ namespace ktmi {
 
 namespace {
 
-int launch_any(const W4Args& a, hipStream_t stream) {
-  return a.x_dtype == KTMI_F32 ? launch_w4_f32(a, stream)
-         : a.x_dtype == KTMI_F16 ? launch_w4_f16(a, stream) : launch_w4_bf16(a, stream);
+int launch_any(const W4Args& a, hipStream_t stream, ktmi_w4_kernel* tell) {
+  return a.x_dtype == KTMI_F32   ? launch_w4_f32(a, stream, tell)
+         : a.x_dtype == KTMI_F16 ? launch_w4_f16(a, stream, tell)
+                                 : launch_w4_bf16(a, stream, tell);
 }
 
 // workspace of a call with more ids than a wave holds: the routes' order (offsets, perm, pos) and the
@@ -23,22 +24,23 @@ int64_t w4_workspace(int64_t tokens, int64_t top_k, int64_t E) {
   return 4 * (ints(E + 1) + 2 * ints(R) + ints(moe_sort_counts(tokens, top_k) * (E + 1)));
 }
 
-int launch_w4(const W4Args& a, hipStream_t stream) {
+int launch_w4(const W4Args& a, hipStream_t stream, ktmi_w4_kernel* tell) {
   int rc;
   if (a.ids && a.n_routes > W4_IDS && a.cols >= W4_STEP) {
     int* offsets = (int*)a.ws;
     int* perm = offsets + ints(a.n_experts + 1);
     int* pos = perm + ints(a.n_routes);
-    rc = launch_moe_sort(nullptr, 2, 0, 0, a.ids, a.n_routes / a.top_k, a.top_k, a.n_experts, nullptr, offsets, perm, pos,
-                         pos + ints(a.n_routes), stream);
+    rc = tell ? KTMI_OK
+              : launch_moe_sort(nullptr, 2, 0, 0, a.ids, a.n_routes / a.top_k, a.top_k, a.n_experts, nullptr, offsets, perm,
+                                pos, pos + ints(a.n_routes), stream);
     if (rc) return rc;
     W4Args b = a;
     b.ids = nullptr, b.offsets = offsets, b.perm = perm;
-    rc = launch_any(b, stream);
+    rc = launch_any(b, stream, tell);
   } else {
-    rc = launch_any(a, stream);
+    rc = launch_any(a, stream, tell);
   }
-  if (rc) return rc;
+  if (rc || tell) return rc;
   KTMI_HIP_TRY(hipGetLastError());
   return KTMI_OK;
 }

@@ -3,6 +3,6 @@
 
 namespace ktmi {
 
-int launch_w4_f16(const W4Args& a, hipStream_t stream) { return launch_t<_Float16>(a, stream); }
+int launch_w4_f16(const W4Args& a, hipStream_t stream, ktmi_w4_kernel* tell) { return launch_t<_Float16>(a, stream, tell); }
 
 }  // namespace ktmi

@@ -677,8 +677,9 @@ __global__ __launch_bounds__(256) void w4_short_kernel(W4Args a) {
   }
 }
 
+// The launches; with tell, what they would launch instead.
 template <typename T, int SPS, bool S4, bool Z, int MT, int KS, int WR>
-int launch_as(const W4Args& a, int64_t items, int64_t expected, hipStream_t stream) {
+int launch_as(const W4Args& a, int64_t items, int64_t expected, hipStream_t stream, ktmi_w4_kernel* tell) {
   constexpr int PLANES = std::is_same<T, float>::value ? 3 : 1, RB = 16 * WR, UNIT = W4_STEP * KS;
   const int64_t tiles = (a.rows + RB - 1) / RB;
   W4Plan p;
@@ -706,21 +707,25 @@ int launch_as(const W4Args& a, int64_t items, int64_t expected, hipStream_t stre
                (long long)(items * p.blocks), 64 * KS * WR);
   auto kernel = w4_mfma_kernel<T, SPS, S4, Z, MT, KS, WR>;
   KTMI_REQUIRE(bytes <= W4_LDS_MOST, KTMI_EINVAL, "w4: %lld bytes of LDS", (long long)bytes);
+  if (tell) {
+    *tell = {16 * MT, KS, 16 * WR, p.deep, whole > x_bytes};
+    return KTMI_OK;
+  }
   kernel<<<(unsigned)(items * p.blocks), 64 * KS * WR, bytes, stream>>>(a, p);
   return KTMI_OK;
 }
 
 template <typename T, int SPS, int MT, int KS, int WR>
-int launch_one(const W4Args& a, int64_t items, int64_t expected, hipStream_t stream) {
+int launch_one(const W4Args& a, int64_t items, int64_t expected, hipStream_t stream, ktmi_w4_kernel* tell) {
   if (a.scale_dtype == KTMI_F32)
-    return a.zeros ? launch_as<T, SPS, true, true, MT, KS, WR>(a, items, expected, stream)
-                   : launch_as<T, SPS, true, false, MT, KS, WR>(a, items, expected, stream);
-  return a.zeros ? launch_as<T, SPS, false, true, MT, KS, WR>(a, items, expected, stream)
-                 : launch_as<T, SPS, false, false, MT, KS, WR>(a, items, expected, stream);
+    return a.zeros ? launch_as<T, SPS, true, true, MT, KS, WR>(a, items, expected, stream, tell)
+                   : launch_as<T, SPS, true, false, MT, KS, WR>(a, items, expected, stream, tell);
+  return a.zeros ? launch_as<T, SPS, false, true, MT, KS, WR>(a, items, expected, stream, tell)
+                 : launch_as<T, SPS, false, false, MT, KS, WR>(a, items, expected, stream, tell);
 }
 
 template <typename T, int SPS>
-int launch_sps(const W4Args& a, hipStream_t stream) {
+int launch_sps(const W4Args& a, hipStream_t stream, ktmi_w4_kernel* tell) {
   constexpr bool F32 = std::is_same<T, float>::value;
   // rows of an expert, about: 16 a pass, or 32 where there are more (dense 4096 x 7168, bf16: 32 rows 26 us
   // in one pass of 32, 64 rows 27 in two; in one of 64 with its shorter stages 71)
@@ -740,23 +745,29 @@ int launch_sps(const W4Args& a, hipStream_t stream) {
   const bool wide = expected * ((a.rows + 31) / 32) > 256;
   if constexpr (!F32)
     if (many)
-      return !split ? launch_one<T, SPS, 2, 1, 4>(a, items, expected, stream)
-             : wide ? launch_one<T, SPS, 2, 2, 4>(a, items, expected, stream)
-                    : launch_one<T, SPS, 2, 4, 2>(a, items, expected, stream);
-  return split ? launch_one<T, SPS, 1, 4, 1>(a, items, expected, stream) : launch_one<T, SPS, 1, 1, 4>(a, items, expected, stream);
+      return !split ? launch_one<T, SPS, 2, 1, 4>(a, items, expected, stream, tell)
+             : wide ? launch_one<T, SPS, 2, 2, 4>(a, items, expected, stream, tell)
+                    : launch_one<T, SPS, 2, 4, 2>(a, items, expected, stream, tell);
+  return split ? launch_one<T, SPS, 1, 4, 1>(a, items, expected, stream, tell) : launch_one<T, SPS, 1, 1, 4>(a, items, expected, stream, tell);
 }
 
 template <typename T>
-int launch_t(const W4Args& a, hipStream_t stream) {
+int launch_t(const W4Args& a, hipStream_t stream, ktmi_w4_kernel* tell) {
   W4Args b = a;
   if (a.group >= a.cols) b.group = (a.cols + W4_STEP - 1) / W4_STEP * W4_STEP;  // one group of whole steps
   if (a.cols < W4_STEP) {
+    if (tell) {
+      *tell = {1, 1, 4, 1, 0};
+      return KTMI_OK;
+    }
     const int64_t quads = (a.rows + 3) / 4;
     const dim3 grid((unsigned)a.n_routes, (unsigned)(quads < 65535 ? quads : 65535));
     w4_short_kernel<T><<<grid, 256, 0, stream>>>(b);
     return KTMI_OK;
   }
-  return b.group == 32 ? launch_sps<T, 4>(b, stream) : b.group == 64 ? launch_sps<T, 2>(b, stream) : launch_sps<T, 1>(b, stream);
+  return b.group == 32   ? launch_sps<T, 4>(b, stream, tell)
+         : b.group == 64 ? launch_sps<T, 2>(b, stream, tell)
+                         : launch_sps<T, 1>(b, stream, tell);
 }
 
 }  // namespace

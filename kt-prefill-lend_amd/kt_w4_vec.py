@@ -13,9 +13,10 @@ codes: uint8, byte j of a row holds code 2j in its low and code 2j + 1 in its hi
 same bytes as int32 [.., K/8]; scales: bf16, f16 or f32 [.., ceil(K/group_size)]; zeros: uint8 of that
 shape, or None for 8 everywhere; group_size: 32, 64, a multiple of 128, or at least K (one group a
 row). x: bf16, f16 or f32; the weights' values are exact, sums are in fp32 and rounded once to x's
-type. Any K and N (to 2^24), at most 2^23 rows of y. They run on the current stream of x's device, allocate from torch's caching
-allocator, never synchronise and can be captured into a HIP graph. No gradient: inputs that require
-one are refused while gradients are recorded (RuntimeError), inputs with a forward-mode tangent always
+type (of f32 x the bits below 2^-133 may be left out). Any K and N (to 2^24), at most 2^23 rows of y.
+They run on the current stream of x's device, allocate from torch's caching allocator, never
+synchronise and can be captured into a HIP graph. No gradient: inputs that require one are refused
+while gradients are recorded (RuntimeError), inputs with a forward-mode tangent always
 (NotImplementedError), and so are traces by torch.jit.trace or make_fx (RuntimeError).
 """
 from __future__ import annotations

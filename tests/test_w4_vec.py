@@ -3,6 +3,7 @@
 Most cases use small integers for x and powers of two for the scales: every product and partial sum
 is then exact in fp32 whatever the order of the sums, so the only rounding is the last one and the
 outputs have to be equal bit for bit. Others use general values against 64 bits."""
+import ctypes
 import math
 
 import pytest
@@ -451,8 +452,175 @@ def test_records_without_the_kernels_are_refused_on_the_gpu(dev, name):
     assert torch.equal(call(*tensors), want)
 
 
+# ---------------------------------------------------------------- every kernel shape of the products
+
+
+def kernel_of(by, dtype, K, G, N, E, R):
+    """(x_rows, col_waves, weight_rows, tiles, staged) of the kernel that the call takes."""
+    k = _lib.ktmi_w4_kernel()
+    _lib.check(_lib.lib().ktmi_w4_kernel_of(by, _lib.dtype_code(dtype), K, G, N, E, R, ctypes.byref(k)), "w4_kernel_of")
+    return tuple(getattr(k, name) for name, _ in k._fields_)
+
+
+def test_kernel_of_refusals():
+    L, k = _lib.lib(), _lib.ktmi_w4_kernel()
+    good = dict(by=_lib.W4_SORTED, dt=2, K=256, G=128, N=64, E=4, R=8)
+    for kw in [dict(), dict(by=3), dict(by=-1), dict(dt=5), dict(K=0), dict(G=48), dict(N=0), dict(E=0), dict(R=0), dict(R=1 << 24)]:
+        a = good | kw
+        rc = L.ktmi_w4_kernel_of(a["by"], a["dt"], a["K"], a["G"], a["N"], a["E"], a["R"], ctypes.byref(k))
+        assert rc == (-1 if kw else 0), kw
+    assert L.ktmi_w4_kernel_of(0, 2, 256, 128, 64, 1, 8, None) == -1
+
+
+# rows of x, N, K, group; with the shapes above: the kernel that bf16 rows take
+DENSE_SHAPES = [
+    (16, 20000, 2080, 32, (16, 1, 64, 1, 1)), (64, 40000, 2080, 32, (32, 1, 64, 2, 1)), (1, 16390, 2048, 128, (16, 1, 64, 1, 0)),
+    (33, 16400, 768, 64, (32, 1, 64, 1, 0)), (2, 100000, 1280, 256, (16, 1, 64, 2, 0)), (5, 1030, 2080, 32, (16, 4, 16, 1, 0)),
+    (40, 1030, 2080, 64, (32, 4, 32, 1, 1)), (40, 1030, 768, 64, (32, 4, 32, 1, 0)), (64, 6000, 768, 128, (32, 2, 64, 1, 0)),
+    (64, 6000, 7168, 128, (32, 2, 64, 1, 1)), (64, 6000, 2080, 32, (32, 2, 64, 1, 1)),
+]
+# mean rows of an expert, experts, N, K, group: uneven counts, some none
+SORTED_SHAPES = [
+    (8, 48, 2050, 768, 128, (16, 1, 64, 2, 0)), (3, 128, 1050, 4480, 32, (16, 1, 64, 4, 1)), (20, 64, 1050, 4096, 64, (32, 1, 64, 2, 1)),
+    (2, 400, 1030, 640, 128, (16, 1, 64, 8, 0)), (21, 150, 520, 1280, 256, (32, 1, 64, 2, 1)), (24, 90, 2050, 2080, 32, (32, 1, 64, 5, 1)),
+    (2, 300, 33, 384, 64, (16, 1, 64, 1, 0)), (1, 140, 20, 256, 32, (16, 4, 16, 1, 0)), (25, 130, 20, 640, 128, (32, 4, 32, 1, 0)),
+]
+# tokens, routes of each, experts, N, K, group: up to 64 ids looked at by every wave, more ordered in one launch,
+# in chunks, in more chunks than add up their counts by themselves
+ROUTED_SHAPES = [
+    (8, 8, 200, 2050, 768, 128, (16, 1, 64, 2, 0)), (13, 8, 18, 3000, 4096, 64, (16, 1, 64, 1, 1)),
+    (625, 8, 200, 200, 256, 32, (32, 1, 64, 1, 0)), (17000, 8, 130, 40, 128, 128, (32, 2, 64, 1, 0)),
+    (60, 17, 150, 130, 384, 64, (16, 1, 64, 1, 0)), (5000, 1, 300, 70, 256, 64, (16, 1, 64, 1, 0)),
+]
+
+
+def test_kernel_shapes_are_all_reached():
+    """The lists hold every split of the waves, several row tiles a block, and stages, for each group size class."""
+    bf16, reached = torch.bfloat16, set()
+    for T, N, K, G, want in DENSE_SHAPES:
+        assert kernel_of(_lib.W4_DENSE, bf16, K, G, N, 1, T) == want, (T, N, K, G)
+        reached.add((min(G, 128), *want))
+    for n, E, N, K, G, want in SORTED_SHAPES:
+        assert kernel_of(_lib.W4_SORTED, bf16, K, G, N, E, n * E) == want, (n, E, N, K, G)
+        reached.add((min(G, 128), *want))
+    for T, k, E, N, K, G, want in ROUTED_SHAPES:
+        assert kernel_of(_lib.W4_IDS, bf16, K, G, N, E, T * k) == want, (T, k, E, N, K, G)
+        reached.add((min(G, 128), *want))
+    splits = {(rows, waves, at_once) for _, rows, waves, at_once, _, _ in reached}
+    assert splits == {(16, 1, 64), (16, 4, 16), (32, 1, 64), (32, 4, 32), (32, 2, 64)}
+    for G in (32, 64, 128):
+        whole = [r for r in reached if r[0] == G and r[2] == 1]
+        assert {r[1] for r in whole} == {16, 32} and any(r[4] > 1 for r in whole)
+    assert any(r[5] and r[4] > 1 and r[1] == 16 for r in reached) and any(r[5] and r[4] > 1 and r[1] == 32 for r in reached)
+
+
+def uneven(mean, E, seed):
+    """Rows of each of E experts, mean * E in all."""
+    g = torch.Generator().manual_seed(seed)
+    at = torch.multinomial(torch.rand(E, generator=g) ** 2, mean * E, replacement=True, generator=g)
+    return torch.bincount(at, minlength=E)
+
+
+def scale_types(dtype):
+    return {"own": dtype, "other": torch.bfloat16 if dtype == torch.float32 else torch.float32}
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("stype", ["own", "other"])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("T,N,K,G,shape", DENSE_SHAPES)
+def test_dense_shapes_exact(dev, T, N, K, G, shape, zeros, stype, dtype):
+    q, s, z = make_weights((), N, K, G, zeros, scale_types(dtype)[stype], N + K, dev)
+    x = make_x(T, K, dtype, T, dev)
+    same(W.w4_vec(x, q, s, z, G), x.double() @ matrix(q, s, z, G, K)[0].t())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("stype", ["own", "other"])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("n,E,N,K,G,shape", SORTED_SHAPES)
+def test_sorted_shapes_exact(dev, n, E, N, K, G, shape, zeros, stype, dtype):
+    """Rows before the first segment and behind the last are zeros."""
+    before, after = 3, 2
+    counts = uneven(n, E, N)
+    R = before + int(counts.sum()) + after
+    q, s, z = make_weights((E,), N, K, G, zeros, scale_types(dtype)[stype], N + K, dev)
+    ids = torch.full((R,), -1)
+    ids[before:R - after] = torch.repeat_interleave(torch.arange(E), counts)
+    offsets = (before + torch.cat([torch.zeros(1, dtype=torch.int64), counts.cumsum(0)])).to(torch.int32).to(dev)
+    x = make_x(R, K, dtype, 5, dev)
+    y = W.moe_w4_sorted(x, q, s, offsets, z, G)
+    same(y, routed(x, q, s, z, G, ids.to(dev), 1)[0])
+    assert (y[:before] == 0).all() and (y[R - after:] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("stype", ["own", "other"])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("T,k,E,N,K,G,shape", ROUTED_SHAPES)
+def test_routed_shapes_exact(dev, T, k, E, N, K, G, shape, zeros, stype, dtype):
+    q, s, z = make_weights((E,), N, K, G, zeros, scale_types(dtype)[stype], N + K, dev)
+    x, ids = make_x(T, K, dtype, T, dev), routes(T, k, E, 0.2, T, dev)
+    same(W.moe_w4_vec(x, q, s, ids, k, z, G), routed(x, q, s, z, G, ids, k)[0])
+
+
 # K, group: rows that end with a word of codes and rows that do not
 WIDE = [(128, 32), (130, 64), (256, 128), (192, 64), (131, 128)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("again", [False, True])
+@pytest.mark.parametrize("K,G", WIDE)
+def test_every_code_and_zero_point_on_the_matrix_cores(dev, K, G, again, dtype):
+    """Each of the 256 bytes of codes against each of the 256 zero points, at every place of a step. With an
+    infinity in another row of the block its sums are made again another way."""
+    N, groups = 256, groups_of(K, G)
+    half = (K + 1) // 2
+    n, j = torch.arange(N)[:, None], torch.arange(half)[None]
+    x = torch.eye(K).to(dtype).to(dev)
+    if again:
+        x = torch.cat([x, torch.full((1, K), float("inf")).to(dtype).to(dev)])
+        x = x[torch.randperm(K + 1, generator=torch.Generator().manual_seed(2)).to(dev)]
+    s = torch.ones((N, groups), dtype=dtype, device=dev)
+    finite = torch.isfinite(x).all(1)
+    for shift in range(0, 256, 16):
+        q = ((j * 16 + n * 1 + n * shift) % 256).to(torch.uint8).to(dev)
+        z = ((n * 3 + torch.arange(groups)[None] * 85 + shift) % 256).to(torch.uint8).to(dev)
+        y = W.w4_vec(x, q, s, z, G)
+        w = matrix(q, s, z, G, K)[0]
+        same(y[finite], x[finite].double() @ w.t())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("large", [False, True])
+@pytest.mark.parametrize("K,G", WIDE)
+def test_large_and_small_values_on_the_matrix_cores(dev, K, G, large, dtype):
+    """Values near the ends of x's range keep their bits, subnormal ones too: each output is one product. Large
+    ones times a code pass fp32, times the code less the zero point they do not."""
+    f = torch.finfo(dtype)
+    vals = [f.max / 8, -f.max / 16, f.max / 16, -f.max / 8] if large else []
+    vals = torch.tensor(vals + [f.tiny, -f.tiny * 1.5, f.tiny / 2, -f.tiny / 4, 1.0, f.eps, 1 + f.eps, -f.tiny * (1 + f.eps)],
+                        dtype=dtype)
+    n = vals.numel()
+    x = torch.zeros((n, K), dtype=dtype)
+    x[torch.arange(n), torch.arange(n) * 10] = vals
+    x = x.to(dev)
+    q = torch.full((4, (K + 1) // 2), 0x99, dtype=torch.uint8, device=dev)  # code 9, weight 1
+    q[1] = 0x77  # weight -1
+    q[2] = 0x88  # weight 0
+    q[3] = 0xCC  # weight 4
+    s = torch.ones((4, groups_of(K, G)), dtype=dtype, device=dev)
+    y = W.w4_vec(x, q, s, None, G)
+    weight = torch.tensor([1.0, -1.0, 0.0, 4.0], dtype=torch.float64)
+    want, off = (vals.double()[:, None] * weight).to(dev), torch.zeros(n, 4, dtype=torch.float64)
+    if dtype == torch.float32:  # its three bf16 parts end at 2^-133: what is below is less than one such step
+        off[vals.abs() < 2.0 ** -109] = 2.0 ** -133 * weight.abs()
+    assert ((y.double() - want).abs() <= off.to(dev)).all()
 
 
 @gpu
