@@ -6,6 +6,7 @@
   between an MFMA and the reader of its result: within 12 wait states of the last MFMA of a chain, none.
 * No kernel spills vector registers.
 """
+import importlib.util
 import os
 import re
 import shutil
@@ -73,3 +74,25 @@ def test_mfma_results_are_read_before_a_branch(tmp_path):
     assert not found, found[:5]
     spills = [int(l.split(":")[1]) for l in lines if ".vgpr_spill_count:" in l]
     assert len(spills) > 40 and not any(spills)
+
+
+def _build_flags():
+    """The flags that the library is built with."""
+    spec = importlib.util.spec_from_file_location("ktmi_build", CSRC.parent / "build.py")
+    build = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(build)
+    return build.HIP_FLAGS
+
+
+# fp32 rows take three products an operand, but have no passes of 32 rows: fewer kernels
+@pytest.mark.parametrize("name,mfmas,kernels", [("w4_f16", 5000, 60), ("w4_f32", 4000, 24)])
+def test_mfma_results_are_read_before_a_branch_in_the_other_types(tmp_path, name, mfmas, kernels):
+    out = tmp_path / (name + ".s")
+    cmd = [HIPCC, *_build_flags(), "--cuda-device-only", "-S", str(CSRC / (name + ".hip")), "-o", str(out)]
+    subprocess.run(cmd, check=True, capture_output=True, timeout=900)
+    lines = out.read_text().split("\n")
+    total, found = branches_after_mfma(lines)
+    assert total > mfmas
+    assert not found, found[:5]
+    spills = [int(l.split(":")[1]) for l in lines if ".vgpr_spill_count:" in l]
+    assert len(spills) > kernels and not any(spills)
