@@ -12,7 +12,8 @@
 // activations with the constant -z, so the group's sum D = sum (q - z) x is exact but for fp32 sums, and
 // acc += s D: no rounding of a weight. Infinite or NaN
 // activations (and products past fp32) make that inf - inf: a block whose sums are not all finite
-// runs again with q - z as the operand, which gives the plain sum's infinities and NaN.
+// runs again with q - z as the operand, which gives the plain sum's infinities and NaN. It takes the rows of x
+// that had such sums from there, the others from the first run: what one row holds changes no bit of another's.
 //
 // fp32 activations are three bf16 parts (8 + 8 + 8 bits of the significand, cut, so that nothing
 // overflows), each with a product of its own: exact but for parts below bf16's smallest number.
@@ -235,6 +236,7 @@ __global__ __launch_bounds__(64 * KS * WR) void w4_mfma_kernel(W4Args a, W4Plan 
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   __shared__ const T* src[16 * MT];
   __shared__ T* dst[16 * MT];
+  __shared__ uint32_t again;  // rows of x whose sums were not all finite, one a bit
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int item = blockIdx.x / p.blocks, n0 = (blockIdx.x - item * p.blocks) * p.deep * RB;
   const int rows_left = (int)(a.rows - n0 < RB * p.deep ? a.rows - n0 : RB * p.deep);
@@ -452,7 +454,7 @@ __global__ __launch_bounds__(64 * KS * WR) void w4_mfma_kernel(W4Args a, W4Plan 
     }
   };
 
-  f32x4_t acc[MT];
+  f32x4_t acc[MT] = {};
   // step s, the at-th of the stage
   auto compute = [&](auto plain, const u32x4_t& raw, const float* scale, const uint32_t (&zz)[SPS], int at) {
     constexpr bool PLAIN = decltype(plain)::value;
@@ -493,25 +495,27 @@ __global__ __launch_bounds__(64 * KS * WR) void w4_mfma_kernel(W4Args a, W4Plan 
   };
   const bool staged = per_stage < p.steps;  // in more than one stage: sums wait in LDS between them
   f32x4_t* sums = (f32x4_t*)(lds + p.x_bytes) + wave * MT * 64 + lane;
-  auto out = [&](int t) {  // the sums of row tile t
+  uint32_t only = ~0u;  // rows of x whose sums are the plain run's
+  auto out = [&](auto plain, int t) {  // the sums of row tile t
     if (t * RB + rb < rows_left)
 #pragma unroll
       for (int q = 0; q < MT; ++q)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int r = 16 * q + 4 * g + i;
-          if (r < m) *(__attribute__((address_space(1))) T*)(dst[r] + n0 + t * RB + rb) = (T)acc[q][i];  // global: a flat store drains the ring
+          if (r < m && (!decltype(plain)::value || (only >> r & 1)))
+            *(__attribute__((address_space(1))) T*)(dst[r] + n0 + t * RB + rb) = (T)acc[q][i];  // global: a flat store drains the ring
         }
   };
+  uint32_t bad = 0;  // the lane's sums that are not finite: 4 t + i of acc[t][i]
   auto run = [&](auto plain) {
     constexpr bool PLAIN = decltype(plain)::value;
     const int tiles = (rows_left + RB - 1) / RB;
-    bool bad = false;
     auto check = [&]() {
 #pragma unroll
       for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) bad |= !(fabsf(acc[t][i]) < __builtin_inff());
+        for (int i = 0; i < 4; ++i) bad |= fabsf(acc[t][i]) < __builtin_inff() ? 0u : 1u << (4 * t + i);
     };
     auto clear = [&]() {
 #pragma unroll
@@ -612,17 +616,34 @@ __global__ __launch_bounds__(64 * KS * WR) void w4_mfma_kernel(W4Args a, W4Plan 
             }
           }
           if (i0 + n == p.steps) {
-            check();
-            out(t);
+            if constexpr (!PLAIN) check();
+            out(plain, t);
           }
           clear();
         }
       }
     }
-    if constexpr (KS > 1) check();
-    return __syncthreads_or(bad);
+    if constexpr (KS > 1 && !PLAIN) check();
+    return __syncthreads_or(bad != 0);
   };
-  if (ragged || run(std::false_type{})) run(std::true_type{});
+  if (ragged || run(std::false_type{})) {
+    f32x4_t first[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) first[t] = acc[t];
+    if (!ragged) {
+      if (threadIdx.x == 0) again = 0;
+      __syncthreads();
+      if (bad) atomicOr(&again, (bad & 15u) << (4 * g) | (bad >> 4) << (16 + 4 * g));
+      __syncthreads();
+      only = again;
+    }
+    run(std::true_type{});
+    if constexpr (KS > 1)
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[t][i] = only >> (16 * t + 4 * g + i) & 1 ? acc[t][i] : first[t][i];
+  }
 
   // the waves' sums over their columns meet in LDS, in the order of the columns' parts
   if constexpr (KS > 1) {
@@ -635,7 +656,7 @@ __global__ __launch_bounds__(64 * KS * WR) void w4_mfma_kernel(W4Args a, W4Plan 
 #pragma unroll
       for (int t = 0; t < MT; ++t)
         for (int w = 0; w < KS - 1; ++w) acc[t] += part[(w * MT + t) * 64 + lane];
-      out(0);
+      out(std::false_type{}, 0);
     }
   }
   zero_rows();

@@ -620,6 +620,11 @@ def test_large_and_small_values_on_the_matrix_cores(dev, K, G, large, dtype):
     want, off = (vals.double()[:, None] * weight).to(dev), torch.zeros(n, 4, dtype=torch.float64)
     if dtype == torch.float32:  # its three bf16 parts end at 2^-133: what is below is less than one such step
         off[vals.abs() < 2.0 ** -109] = 2.0 ** -133 * weight.abs()
+        # Values of 24 bits: of the parts h, m, l (|m| < 2^-7 |v|, |l| < 2^-15 |v|) the sum runs over c h, -8 h (both
+        # exact: 8 bits times 4), c m, -8 m, c l, -8 l, whose partial sums are at most (|c - 8| + 12 2^-7) |v|, below
+        # 1.1 |c - 8| |v| (all of it exact for c = 8): four additions, each off by 2^-24 of that.
+        full = vals.abs() > 1e30
+        off[full] = 4 * 2.0 ** -24 * 1.1 * vals.double().abs()[full, None] * weight.abs()
     assert ((y.double() - want).abs() <= off.to(dev)).all()
 
 
@@ -640,3 +645,44 @@ def test_ids_and_offsets_outside_the_range_on_the_matrix_cores(dev, K, G, N, dty
                         ([-9, -9, -9, -1], [-1] * 6), ([0, 6, 6, 2 ** 31 - 1], [0] * 6), ([-2 ** 31, 1, 1, 6], [0, 2, 2, 2, 2, 2])]:
         y = W.moe_w4_sorted(x, q, s, torch.tensor(offsets, dtype=torch.int32, device=dev), z, G)
         same(y, routed(x, q, s, z, G, torch.tensor(of, device=dev), 1)[0])
+
+
+# rows of x, N, K, group: the columns shared by four waves, by two, whole rows a wave, several row tiles, stages
+NEIGHBOURS = [(5, 40, 384, 64), (20, 70, 640, 128), (64, 6000, 768, 128), (7, 20000, 2080, 32), (24, 40000, 2080, 64), (9, 40, 130, 64)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("T,N,K,G", NEIGHBOURS)
+def test_rows_beside_one_that_is_not_finite_keep_their_bits(dev, T, N, K, G, zeros, dtype):
+    """General values: a row's sums do not depend on what another row of the call holds, by a bit."""
+    q, s, z = make_weights((), N, K, G, zeros, dtype, 3, dev, exact=False)
+    x = make_x(T, K, dtype, 4, dev, exact=False)
+    clean = W.w4_vec(x, q, s, z, G)
+    f = torch.finfo(dtype)
+    w, m = matrix(q, s, z, G, K)
+    for bad in (float("inf"), float("nan"), f.max, f.max / 12):
+        other = x.clone()
+        other[2, K - 2] = other[T - 1, 1] = bad
+        got = W.w4_vec(other, q, s, z, G)
+        rest = [t for t in range(T) if t not in (2, T - 1)]
+        assert torch.equal(got[rest], clean[rest])
+        ids = torch.zeros(T, dtype=torch.int32, device=dev)
+        again = W.moe_w4_vec(other, q[None], s[None], ids, 1, None if z is None else z[None], G)
+        first = W.moe_w4_vec(x, q[None], s[None], ids, 1, None if z is None else z[None], G)
+        assert torch.equal(again[rest], first[rest])
+        # the rows themselves: what 64 bits give where they are not finite; else, where the groups' sums
+        # stay within fp32, as near as a plain sum
+        plain = matrix(q, torch.ones_like(s), z, G, K)[0].abs()
+        for t in (2, T - 1):
+            want = other[t].double() @ w.t()
+            if abs(bad) < float("inf"):
+                near = (other[t].double().abs() @ plain.t() < 2.0 ** 127) & (want.abs() < 0.9 * f.max)
+                size = other[t].double().abs() @ m.t()
+                tol = f.eps / 2 * want.abs() + (1 + f.eps / 2) * (2 * K + 4) * 2.0 ** -24 * size
+                tol += 2.0 ** -25 if dtype == torch.float16 else 0.0  # half a step below f16's normal numbers
+                assert near.any() and ((got[t].double() - want).abs() <= tol)[near].all()
+            else:
+                assert torch.equal(got[t].isnan(), want.isnan())
+                assert torch.equal(got[t][~want.isnan()].double(), want[~want.isnan()])
