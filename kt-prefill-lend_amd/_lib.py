@@ -146,36 +146,53 @@ def stream_ptr(device=None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def _refuse_records(what, tensors):
-    """Refuses calls that torch would record without what the library computes in them: tensors with a
-    forward-mode tangent (the result would have none, a derivative of 0), and traces of torch's own operations
-    (they would hold the outputs' allocations alone)."""
+_torch = None  # what on_device_of takes from torch, bound by its first call (looked up anew they take 0.6 us a call)
+
+
+def _bind_torch():
+    global _torch
     import torch
 
-    if torch.autograd.forward_ad._current_level >= 0:
-        for t in tensors:
-            if isinstance(t, torch.Tensor) and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
-                raise NotImplementedError(f"{what} has no forward-mode derivative: call it on the primal tensors")
-    if torch._C._is_tracing():
-        raise RuntimeError(f"{what} cannot be traced: its kernels are no torch operations")
-    if torch._C._len_torch_dispatch_stack() or torch._ops._len_torch_dispatch_stack_pre_dispatch():
-        from torch.fx.experimental.proxy_tensor import get_proxy_mode
+    c = torch._C
+    pre_dispatch = c._dispatch_tls_is_dispatch_key_included
+    _torch = (torch.autograd.forward_ad, c._is_tracing, c._len_torch_dispatch_stack, pre_dispatch, c.DispatchKey.PreDispatch,
+              c._cuda_getDevice, c._cuda_getCurrentRawStream)
+    return _torch
 
-        if get_proxy_mode() is not None:
-            raise RuntimeError(f"{what} cannot be traced: its kernels are no torch operations")
+
+def _refuse_tangents(what, tensors):
+    """Refuses tensors with a forward-mode tangent: the result would have none, that is a derivative of 0."""
+    import torch
+
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what} has no forward-mode derivative: call it on the primal tensors")
+
+
+def _refuse_traces(what):
+    """Refuses traces of torch's operations: they would hold the outputs' allocations alone."""
+    import torch
+    from torch.fx.experimental.proxy_tensor import get_proxy_mode
+
+    if torch.jit.is_tracing() or get_proxy_mode() is not None:
+        raise RuntimeError(f"{what} cannot be traced: its kernels are no torch operations")
 
 
 def on_device_of(what, t, fn, *args):
     """fn(stream handle, *args) with t's device current: the current stream of that device, on which the
     call's launches and its tensors' allocations are ordered. what: the call's name in errors."""
+    forward_ad, tracing, modes, included, pre_dispatch, current_device, stream = _torch or _bind_torch()
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(what, args)
+    if tracing() or modes() or included(pre_dispatch):
+        _refuse_traces(what)
+    index = t.get_device()
+    if current_device() == index:
+        return fn(stream(index), *args)
     import torch
 
-    _refuse_records(what, args)
-    index = t.get_device()
-    if torch._C._cuda_getDevice() == index:
-        return fn(torch._C._cuda_getCurrentRawStream(index), *args)
     with torch.cuda.device(index):
-        return fn(torch._C._cuda_getCurrentRawStream(index), *args)
+        return fn(stream(index), *args)
 
 
 def dtype_code(dtype) -> int:
