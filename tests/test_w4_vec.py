@@ -686,3 +686,21 @@ def test_rows_beside_one_that_is_not_finite_keep_their_bits(dev, T, N, K, G, zer
             else:
                 assert torch.equal(got[t].isnan(), want.isnan())
                 assert torch.equal(got[t][~want.isnan()].double(), want[~want.isnan()])
+
+
+@gpu
+@pytest.mark.parametrize("E", [1, 2, 63, 64, 65, 127, 640, 2047, 2048])
+@pytest.mark.parametrize("K", [1, 96, 127, 130])
+def test_sorted_exact_of_many_experts(dev, E, K):
+    """Empty segments in front, between and behind, a first segment past row 0, offsets past the rows."""
+    g = torch.Generator().manual_seed(E + K)
+    R, N, G = 301, 3, 32
+    q, s, z = make_weights((E,), N, K, G, True, torch.bfloat16, 8, dev)
+    x = make_x(R, K, torch.bfloat16, 9, dev)
+    for offsets in (torch.sort(torch.randint(-20, R + 20, (E + 1,), generator=g)).values,
+                    torch.sort(torch.randint(7, R - 7, (E + 1,), generator=g) // 40 * 40).values,
+                    torch.full((E + 1,), R // 2), torch.arange(E + 1) - 3, R - E - 1 + torch.arange(E + 1)):
+        ids = torch.searchsorted(offsets, torch.arange(R), right=True) - 1
+        ids[ids >= E] = -1
+        y = W.moe_w4_sorted(x, q, s, offsets.to(torch.int32).to(dev), z, G)
+        same(y, routed(x, q, s, z, G, ids.to(dev), 1)[0])
