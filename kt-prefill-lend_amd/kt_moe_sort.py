@@ -39,6 +39,14 @@ def _rows_of(t):
     return t if t.is_contiguous() or (t.stride(1) == 1 and t.stride(0) >= t.shape[1]) else t.contiguous()
 
 
+def _address(what, t):
+    """t's first element, where the library takes a null pointer for an argument left out."""
+    p = t.data_ptr()
+    if p == 0 and t.numel():
+        raise TypeError(f"{what}: a {type(t).__name__} holds no memory of its own: pass its local tensor")
+    return p
+
+
 def _check_gpu(what, *tensors):
     """Refuses tensors that are not all on one GPU (None: an argument left out)."""
     index = tensors[0].get_device()  # -1 on the CPU
@@ -85,7 +93,7 @@ def _launch_sort(stream, x, ids, n_experts):
     pos = ids.new_empty((T, k))
     need = L.ktmi_moe_sort_workspace(T, k, n_experts)
     ws = ids.new_empty((need,), dtype=torch.uint8) if need else None
-    rc = L.ktmi_moe_sort(x.data_ptr(), _CODES[x.dtype], x.stride(0), K, ids.data_ptr(), T, k, n_experts,
+    rc = L.ktmi_moe_sort(_address("moe_sort", x), _CODES[x.dtype], x.stride(0), K, ids.data_ptr(), T, k, n_experts,
                          rows.data_ptr(), offsets.data_ptr(), perm.data_ptr(), pos.data_ptr(),
                          ws.data_ptr() if need else None, need, stream)
     if rc:
@@ -101,8 +109,8 @@ def _launch_unsort(stream, rows, topk_w, pos):
         topk_w = topk_w.contiguous()
     y = rows.new_empty((T, K))
     rc = _lib.lib().ktmi_moe_unsort(rows.data_ptr(), _CODES[rows.dtype], rows.stride(0), K,
-                                    None if topk_w is None else topk_w.data_ptr(), pos.data_ptr(), T, k, y.data_ptr(),
-                                    stream)
+                                    None if topk_w is None else _address("moe_unsort", topk_w), pos.data_ptr(), T, k,
+                                    y.data_ptr(), stream)
     if rc:
         _lib.check(rc, "moe_unsort")
     return y
@@ -117,9 +125,10 @@ def _launch_unsort_grad(stream, dy, rows, topk_w, pos, want_rows, want_w):
         topk_w = topk_w.contiguous()
     drows = dy.new_empty((T * k, K)) if want_rows else None
     dw = dy.new_empty((T, k), dtype=torch.float32) if want_w else None
-    rc = _lib.lib().ktmi_moe_unsort_grad(dy.data_ptr(), dy.stride(0), rows.data_ptr() if want_w else None,
+    what = "moe_unsort's gradient"
+    rc = _lib.lib().ktmi_moe_unsort_grad(_address(what, dy), dy.stride(0), rows.data_ptr() if want_w else None,
                                          rows.stride(0) if want_w else K, _CODES[dy.dtype], K,
-                                         None if topk_w is None else topk_w.data_ptr(), pos.data_ptr(), T, k,
+                                         None if topk_w is None else _address(what, topk_w), pos.data_ptr(), T, k,
                                          drows.data_ptr() if want_rows else None, dw.data_ptr() if want_w else None,
                                          stream)
     if rc:

@@ -24,7 +24,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .kt_moe_sort import _CODES, MAX_EXPERTS, _check_gpu, _rows_of
+from .kt_moe_sort import _CODES, MAX_EXPERTS, _address, _check_gpu, _rows_of
 
 
 def _check(what, x, codes, scales, zeros, group, lead):
@@ -67,7 +67,7 @@ def _args(x, codes, scales, zeros, group):
     zeros = None if zeros is None else zeros.contiguous()
     return (x, codes, scales, zeros), (x.data_ptr(), _CODES[x.dtype], x.stride(0), x.shape[1], codes.data_ptr(),
                                        scales.data_ptr(), _CODES[scales.dtype],
-                                       None if zeros is None else zeros.data_ptr(), group)
+                                       None if zeros is None else _address("zeros", zeros), group)
 
 
 def _launch_dense(stream, x, codes, scales, zeros, group):

@@ -101,3 +101,27 @@ def check_refused_records(name, call, tensors):
     for pre in (False, True):
         with pytest.raises(RuntimeError, match=f"{name} cannot be traced"):
             make_fx(call, pre_dispatch=pre)(*tensors)
+
+
+def wrapped(t):
+    """t in a tensor subclass that holds it, without memory of its own (as distributed tensors are)."""
+    import torch
+
+    class Wrapped(torch.Tensor):
+        @staticmethod
+        def __new__(cls, inner):
+            return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device=inner.device,
+                                                       strides=inner.stride())
+
+        def __init__(self, inner):
+            self.inner = inner
+
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            def plain(a):
+                return a.inner if isinstance(a, cls) else a
+
+            out = func(*[plain(a) for a in args], **(kwargs or {}))
+            return cls(out) if isinstance(out, torch.Tensor) else out
+
+    return Wrapped(t)

@@ -552,3 +552,18 @@ def test_order_alone(dev, T, k):
     for got, want in zip((off, perm, pos.reshape(T, k)), plain_order(ids, E)):
         assert np.array_equal(got.cpu().numpy(), want)
     assert (ws[need:] == 93).all()
+
+
+def test_tensors_without_memory_are_refused():
+    """Where the library takes a null pointer for an argument left out, a wrapper's must not pass for one."""
+    from helpers import wrapped
+
+    x, w, ids = torch.ones(2, 4), torch.ones(2, 2), torch.zeros(2, 2, dtype=torch.int32)
+    rows, pos = torch.ones(4, 4), torch.arange(4, dtype=torch.int32).reshape(2, 2)
+    with pytest.raises(TypeError, match="moe_sort: a Wrapped"):
+        S._launch_sort(0, wrapped(x), ids, 3)
+    with pytest.raises(TypeError, match="moe_unsort: a Wrapped"):
+        S._launch_unsort(0, rows, wrapped(w), pos)
+    for dy, v in [(wrapped(x), w), (x, wrapped(w))]:
+        with pytest.raises(TypeError, match="moe_unsort's gradient: a Wrapped"):
+            S._launch_unsort_grad(0, dy, rows, v, pos, True, True)

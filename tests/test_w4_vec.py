@@ -704,3 +704,11 @@ def test_sorted_exact_of_many_experts(dev, E, K):
         ids[ids >= E] = -1
         y = W.moe_w4_sorted(x, q, s, offsets.to(torch.int32).to(dev), z, G)
         same(y, routed(x, q, s, z, G, ids.to(dev), 1)[0])
+
+
+def test_zeros_without_memory_are_refused():
+    from helpers import wrapped
+
+    x, q, s = torch.ones(2, 64), torch.zeros((3, 32), dtype=torch.uint8), torch.ones(3, 2)
+    with pytest.raises(TypeError, match="zeros: a Wrapped"):
+        W._args(x, q, s, wrapped(torch.zeros((3, 2), dtype=torch.uint8)), 32)
