@@ -146,17 +146,16 @@ def stream_ptr(device=None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-_torch = None  # what on_device_of takes from torch, bound by its first call (looked up anew they take 0.6 us a call)
+_torch = None  # what on_device_of takes from torch, bound by its first call (looked up anew it takes 0.5 us a call)
 
 
 def _bind_torch():
     global _torch
     import torch
+    import torch.fx
 
     c = torch._C
-    pre_dispatch = c._dispatch_tls_is_dispatch_key_included
-    _torch = (torch.autograd.forward_ad, c._is_tracing, c._len_torch_dispatch_stack, pre_dispatch, c.DispatchKey.PreDispatch,
-              c._cuda_getDevice, c._cuda_getCurrentRawStream)
+    _torch = torch.autograd.forward_ad, torch.fx._symbolic_trace, c._is_tracing, c._cuda_getDevice, c._cuda_getCurrentRawStream
     return _torch
 
 
@@ -172,7 +171,7 @@ def _refuse_tangents(what, tensors):
 def _refuse_traces(what):
     """Refuses traces of torch's operations: they would hold the outputs' allocations alone."""
     import torch
-    from torch.fx.experimental.proxy_tensor import get_proxy_mode
+    from torch.fx.experimental.proxy_tensor import get_proxy_mode  # this thread's
 
     if torch.jit.is_tracing() or get_proxy_mode() is not None:
         raise RuntimeError(f"{what} cannot be traced: its kernels are no torch operations")
@@ -181,10 +180,10 @@ def _refuse_traces(what):
 def on_device_of(what, t, fn, *args):
     """fn(stream handle, *args) with t's device current: the current stream of that device, on which the
     call's launches and its tensors' allocations are ordered. what: the call's name in errors."""
-    forward_ad, tracing, modes, included, pre_dispatch, current_device, stream = _torch or _bind_torch()
+    forward_ad, fx, jit_tracing, current_device, stream = _torch or _bind_torch()
     if forward_ad._current_level >= 0:
         _refuse_tangents(what, args)
-    if tracing() or modes() or included(pre_dispatch):
+    if fx._is_fx_tracing_flag or jit_tracing():
         _refuse_traces(what)
     index = t.get_device()
     if current_device() == index:

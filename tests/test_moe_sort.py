@@ -567,3 +567,82 @@ def test_tensors_without_memory_are_refused():
     for dy, v in [(wrapped(x), w), (x, wrapped(w))]:
         with pytest.raises(TypeError, match="moe_unsort's gradient: a Wrapped"):
             S._launch_unsort_grad(0, dy, rows, v, pos, True, True)
+
+
+# ---------------------------------------------------------------- compiled, checkpointed, from several threads
+
+def a_run(dev, ids, E):
+    """A sort, an operation on the rows and the way back, as a function of (x, w), with its gradients."""
+    def forward(x, w):
+        s = S.moe_sort(x * 1, ids, E)
+        return S.moe_unsort(s.rows * 2, w, s.pos) + 1
+
+    def all_of(fn, x, w):
+        y = fn(x, w)
+        return [y.detach(), *torch.autograd.grad(y, (x, w), torch.ones_like(y))]
+
+    return forward, all_of
+
+
+@gpu
+@pytest.mark.parametrize("how", ["eager", "aot_eager", "checkpoint"])
+def test_compiled_and_checkpointed(dev, how):
+    T, k, E, K = 77, 8, 16, 256
+    ids = make_ids(T, k, E, 0.1, 1, dev)
+    x, w = make_x((T, K), torch.bfloat16, 2, dev).requires_grad_(True), make_x((T, k), torch.float32, 3, dev).requires_grad_(True)
+    forward, all_of = a_run(dev, ids, E)
+    want = all_of(forward, x, w)
+    if how == "checkpoint":
+        from torch.utils.checkpoint import checkpoint
+
+        other = lambda x, w: checkpoint(forward, x, w, use_reentrant=False)  # noqa: E731
+    else:
+        torch._dynamo.reset()
+        other = torch.compile(forward, backend=how)
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(want, all_of(other, x, w)))
+
+
+@gpu
+def test_threads(dev):
+    """Calls of several host threads, each on a stream of its own, with refusals between them."""
+    import threading
+
+    import kt_prefill_lend_amd.kt_w4_vec as W
+
+    T, k, E, K, N = 77, 8, 16, 256, 128
+    ids = make_ids(T, k, E, 0.1, 1, dev)
+    x, w = make_x((T, K), torch.bfloat16, 2, dev).requires_grad_(True), make_x((T, k), torch.float32, 3, dev).requires_grad_(True)
+    g = torch.Generator().manual_seed(4)
+    q = torch.randint(0, 256, (E, N, K // 2), generator=g, dtype=torch.uint8).to(dev)
+    sc = torch.rand((E, N, K // 128), generator=g).to(torch.bfloat16).to(dev)
+    forward, all_of = a_run(dev, ids, E)
+
+    def step():
+        with torch.no_grad():
+            y = W.moe_w4_vec(x, q, sc, ids.reshape(-1), k)
+        return [y, *all_of(forward, x, w)]
+
+    want, wrong = step(), []
+    torch.cuda.synchronize()
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for n in range(20):
+                    got = step()
+                    stream.synchronize()
+                    if not all(torch.equal(a, b) for a, b in zip(want, got)):
+                        wrong.append((i, n))
+                    with pytest.raises(ValueError, match="4000 experts"):
+                        S.moe_sort(x.detach(), ids, 4000)
+        except BaseException as e:  # a thread's failure is the test's
+            wrong.append((i, repr(e)))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong
