@@ -8,9 +8,9 @@
 // and its routes' places are wave-uniform.
 //
 // HBM bounds the long calls and launches the short ones. 16384 tokens of 2048 bf16 columns, 8 routes
-// each: the order 17 us (two launches), the copies 103 us for 604 MB (5.8 TB/s; a large copy on this
-// card moves 5.0 read and written, a fill 6.9); 4096 tokens: the sums back 24 us, their gradients 43 us for
-// 257 MB (6.0 TB/s). One token: one launch of 4 us. The order could be one launch less with blocks that
+// each: the order 17 us (two launches), the copies 102 us for 604 MB (5.9 TB/s; a large copy on this
+// card moves 5.0 read and written, a fill 6.9); 4096 tokens, a fifth of the routes without an expert: the sums back
+// 23 us, their gradients 42 us for 257 MB (6.1 TB/s). One token: one launch of 4 us. The order could be one launch less with blocks that
 // wait for each other's counts; that is left out, as a wait between blocks ends only if all of them run.
 #include <type_traits>
 

@@ -1,7 +1,8 @@
 """Tokens sorted by expert and back, with the route weights applied, and the gradients of both.
 
 For expert products outside the built-in layer (`kt_gguf_hot.moe_layer`): other weight formats
-(`kt_w4_vec.moe_w4_sorted`), adapters, ranks that hold part of the experts, training.
+(`kt_w4_vec.moe_w4_sorted`, which has no gradient), adapters, ranks that hold part of the experts,
+training.
 
     s = moe_sort(x, topk_ids, n_experts)          # s.rows[s.offsets[e]:s.offsets[e + 1]] are expert e's
     y = moe_unsort(experts(s.rows), topk_w, s.pos)  # the weighted sum over each token's routes
