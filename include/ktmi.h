@@ -142,8 +142,8 @@ int ktmi_moe_unsort_grad(const void* dy, int64_t dy_stride, const void* rows, in
 
 /* ---- products with 4-bit weights and group scales ---------------------------------
  * y[r, n] = sum_g scale[e, n, g] * sum_{c in group g} (code[e, n, c] - zero[e, n, g]) * x[r, c], summed
- * in fp32 and rounded once to x's type (bits of fp32 x below 2^-133 may be left out). For checkpoints of plain 4-bit codes (no ggml type); no
- * counterpart in the reference.
+ * in fp32 and rounded once to x's type (bits of fp32 x below 2^-133 may be left out). For checkpoints
+ * of plain 4-bit codes (no ggml type); no counterpart in the reference.
  *   codes uint8 [n_experts, rows, ceil(cols/2)]: byte j of a row holds code 2j in its low and
  *         2j+1 in its high four bits (codes packed eight to an int32 along cols are the same bytes)
  *   scales [n_experts, rows, ceil(cols/group)] in scale_dtype; zeros uint8 of that shape, or NULL: 8
