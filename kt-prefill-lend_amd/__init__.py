@@ -13,6 +13,7 @@ The directory name is not a Python identifier; load it as `kt_prefill_lend_amd` 
 from __future__ import annotations
 
 __all__ = ["gguf", "kt_gguf_moe_multi", "kt_gguf_dequant", "kt_gguf_hot", "kt_hot_cache", "kt_ep_wrapper", "kt_moe_sort",
+           "kt_fp8_block", "kt_gated",
            "kt_w4_vec", "synth"]
 
 

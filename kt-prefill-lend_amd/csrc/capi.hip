@@ -309,6 +309,168 @@ int ktmi_w4_kernel_of(int by, int x_dtype, int64_t cols, int64_t group, int64_t 
   return rc ? rc : launch_w4(a, nullptr, kernel);
 }
 
+// ---- products in 8-bit floating point
+
+static constexpr int64_t MAX_ROWS = 0x7fffff00;  // of x or y: 31 bits hold a row past the last tile's
+
+static int check_fp8(const char* what, const Fp8Args& a, int64_t need, int64_t ws_bytes) {
+  KTMI_REQUIRE(dtype_ok(a.dtype), KTMI_EINVAL, "%s: x dtype %d", what, a.dtype);
+  KTMI_REQUIRE(a.cols > 0 && a.cols <= (1 << 24) && a.rows > 0 && a.rows <= (1 << 24), KTMI_EINVAL,
+               "%s: cols %lld rows %lld (1 to 2^24)", what, (long long)a.cols, (long long)a.rows);
+  KTMI_REQUIRE(a.n_experts > 0 && a.n_experts <= SORT_MAX_EXPERTS, KTMI_EINVAL, "%s: %lld experts (1 to %lld)", what,
+               (long long)a.n_experts, (long long)SORT_MAX_EXPERTS);
+  KTMI_REQUIRE(a.x_rows >= 0 && a.top_k > 0 && a.top_k <= 65535 && a.x_rows <= MAX_ROWS / a.top_k, KTMI_EINVAL,
+               "%s: %lld rows of x, top_k %lld (at most 65535, and %lld rows of y)", what, (long long)a.x_rows,
+               (long long)a.top_k, (long long)MAX_ROWS);
+  if (a.x_rows == 0) return KTMI_OK;
+  const int es = a.dtype == KTMI_F32 ? 4 : 2;
+  KTMI_REQUIRE(a.x && a.w && a.scales && a.y, KTMI_EINVAL, "%s: null pointer", what);
+  KTMI_REQUIRE(aligned(a.x, es) && aligned(a.y, es) && aligned(a.scales, 4), KTMI_EINVAL,
+               "%s: x, y and scales must be aligned to their types", what);
+  KTMI_REQUIRE(a.x_stride >= a.cols || a.x_rows <= 1, KTMI_EINVAL, "%s: x_stride %lld below cols %lld", what,
+               (long long)a.x_stride, (long long)a.cols);
+  KTMI_REQUIRE(need == 0 || (a.ws && ws_bytes >= need && aligned(a.ws, 16)), KTMI_ESPACE,
+               "%s: workspace %lld < %lld bytes, or not aligned to 16", what, (long long)ws_bytes, (long long)need);
+  return KTMI_OK;
+}
+
+static bool fp8_shape(int64_t cols, int64_t rows, int64_t n_experts, int64_t top_k) {
+  return cols > 0 && cols <= (1 << 24) && rows > 0 && n_experts > 0 && n_experts <= SORT_MAX_EXPERTS && top_k > 0 &&
+         top_k <= 65535 && rows <= MAX_ROWS / top_k;
+}
+
+int64_t ktmi_fp8_linear_workspace(int64_t cols, int64_t tokens) {
+  return fp8_shape(cols, tokens, 1, 1) ? fp8_workspace(cols, tokens, 1, 1, false) : 0;
+}
+
+int ktmi_fp8_linear(const void* x, int x_dtype, int64_t x_stride, int64_t cols, const void* w, const float* scales,
+                    int64_t rows, int64_t tokens, void* y, void* workspace, int64_t ws_bytes, void* stream) {
+  g_err[0] = 0;
+  const Fp8Args a = {x_dtype, x, x_stride, tokens, (const uint8_t*)w, scales, rows, cols, 1, nullptr, 1, nullptr, y,
+                     (uint8_t*)workspace};
+  int rc = check_fp8("fp8_linear", a, ktmi_fp8_linear_workspace(cols, tokens), ws_bytes);
+  return rc || tokens == 0 ? rc : launch_fp8(a, (hipStream_t)stream);
+}
+
+int64_t ktmi_moe_fp8_vec_workspace(int64_t cols, int64_t tokens, int64_t top_k, int64_t n_experts) {
+  return fp8_shape(cols, tokens, n_experts, top_k) ? fp8_workspace(cols, tokens, n_experts, top_k, true) : 0;
+}
+
+int ktmi_moe_fp8_vec(const void* x, int x_dtype, int64_t x_stride, int64_t cols, const void* w, const float* scales,
+                     int64_t rows, int64_t n_experts, const int32_t* ids, int64_t top_k, int64_t tokens, void* y,
+                     void* workspace, int64_t ws_bytes, void* stream) {
+  g_err[0] = 0;
+  const Fp8Args a = {x_dtype, x, x_stride, tokens, (const uint8_t*)w, scales, rows, cols, n_experts, ids, top_k, nullptr, y,
+                     (uint8_t*)workspace};
+  int rc = check_fp8("moe_fp8_vec", a, ktmi_moe_fp8_vec_workspace(cols, tokens, top_k, n_experts), ws_bytes);
+  if (rc || tokens == 0) return rc;
+  KTMI_REQUIRE(ids, KTMI_EINVAL, "moe_fp8_vec: null pointer");
+  return launch_fp8(a, (hipStream_t)stream);
+}
+
+int64_t ktmi_moe_fp8_sorted_workspace(int64_t cols, int64_t n_experts, int64_t n_rows) {
+  return fp8_shape(cols, n_rows, n_experts, 1) ? fp8_workspace(cols, n_rows, n_experts, 1, false) : 0;
+}
+
+int ktmi_moe_fp8_sorted(const void* x, int x_dtype, int64_t x_stride, int64_t cols, const void* w, const float* scales,
+                        int64_t rows, int64_t n_experts, const int32_t* offsets, int64_t n_rows, void* y, void* workspace,
+                        int64_t ws_bytes, void* stream) {
+  g_err[0] = 0;
+  const Fp8Args a = {x_dtype, x, x_stride, n_rows, (const uint8_t*)w, scales, rows, cols, n_experts, nullptr, 1, offsets, y,
+                     (uint8_t*)workspace};
+  int rc = check_fp8("moe_fp8_sorted", a, ktmi_moe_fp8_sorted_workspace(cols, n_experts, n_rows), ws_bytes);
+  if (rc || n_rows == 0) return rc;
+  KTMI_REQUIRE(offsets, KTMI_EINVAL, "moe_fp8_sorted: null pointer");
+  return launch_fp8(a, (hipStream_t)stream);
+}
+
+// ---- gated and linear products with gradients
+
+static int check_prod(const char* what, const ProdArgs& a) {
+  KTMI_REQUIRE(dtype_ok(a.dtype), KTMI_EINVAL, "%s: dtype %d", what, a.dtype);
+  KTMI_REQUIRE(a.cols > 0 && a.cols <= (1 << 24) && a.rows > 0 && a.rows <= (1 << 24), KTMI_EINVAL,
+               "%s: cols %lld rows %lld (1 to 2^24)", what, (long long)a.cols, (long long)a.rows);
+  KTMI_REQUIRE(a.n_experts > 0 && a.n_experts <= SORT_MAX_EXPERTS && (a.offsets || a.n_experts == 1), KTMI_EINVAL,
+               "%s: %lld experts (1 to %lld; without offsets 1)", what, (long long)a.n_experts, (long long)SORT_MAX_EXPERTS);
+  KTMI_REQUIRE(a.n_rows >= 0 && a.n_rows <= MAX_ROWS, KTMI_EINVAL, "%s: %lld rows (at most %lld)", what, (long long)a.n_rows,
+               (long long)MAX_ROWS);
+  const int es = a.dtype == KTMI_F32 ? 4 : 2;
+  KTMI_REQUIRE(aligned(a.x, es) && aligned(a.dy, es) && aligned(a.w, es) && aligned(a.y, es) && aligned(a.sums, 16), KTMI_EINVAL,
+               "%s: tensors must be aligned to their types, sums to 16 bytes", what);
+  return KTMI_OK;
+}
+
+static int check_stride(const char* what, const char* name, int64_t stride, int64_t width, int64_t rows) {
+  KTMI_REQUIRE(stride >= width || rows <= 1, KTMI_EINVAL, "%s: %s %lld below the row's %lld", what, name, (long long)stride,
+               (long long)width);
+  return KTMI_OK;
+}
+
+static int check_act(const char* what, int act) {
+  KTMI_REQUIRE(act == KTMI_ACT_SILU || act == KTMI_ACT_GELU_TANH, KTMI_EINVAL, "%s: act %d", what, act);
+  return KTMI_OK;
+}
+
+int ktmi_gated(const void* x, int dtype, int64_t x_stride, int64_t cols, const void* w13, int64_t inter, int64_t n_experts,
+               const int32_t* offsets, int64_t n_rows, int act, void* h, float* sums, void* stream) {
+  g_err[0] = 0;
+  const ProdArgs a = {dtype, x, x_stride, nullptr, 0, w13, inter, cols, n_experts, offsets, n_rows, act, h, sums};
+  int rc = check_prod("gated", a);
+  if (!rc) rc = check_act("gated", act);
+  if (!rc) rc = check_stride("gated", "x_stride", x_stride, cols, n_rows);
+  KTMI_REQUIRE(rc || inter <= (1 << 23), KTMI_EINVAL, "gated: inter %lld (at most 2^23)", (long long)inter);
+  if (rc || n_rows == 0) return rc;
+  KTMI_REQUIRE(x && w13 && h, KTMI_EINVAL, "gated: null pointer");
+  return launch_prod_fwd(a, true, (hipStream_t)stream);
+}
+
+int ktmi_gated_grad(const float* sums, const void* dh, int dtype, int64_t dh_stride, int64_t inter, int64_t n_rows, int act,
+                    void* dsums, void* stream) {
+  g_err[0] = 0;
+  const ProdArgs a = {dtype, nullptr, 0, dh, dh_stride, nullptr, inter, 1, 1, nullptr, n_rows, act, dsums, (float*)sums};
+  int rc = check_prod("gated_grad", a);
+  if (!rc) rc = check_act("gated_grad", act);
+  if (!rc) rc = check_stride("gated_grad", "dh_stride", dh_stride, inter, n_rows);
+  KTMI_REQUIRE(rc || inter <= (1 << 23), KTMI_EINVAL, "gated_grad: inter %lld (at most 2^23)", (long long)inter);
+  if (rc || n_rows == 0) return rc;
+  KTMI_REQUIRE(sums && dh && dsums, KTMI_EINVAL, "gated_grad: null pointer");
+  return launch_gated_grad(sums, dh, dtype, dh_stride, inter, n_rows, act, dsums, (hipStream_t)stream);
+}
+
+int ktmi_linear(const void* x, int dtype, int64_t x_stride, int64_t cols, const void* w, int64_t rows, int64_t n_experts,
+                const int32_t* offsets, int64_t n_rows, void* y, void* stream) {
+  g_err[0] = 0;
+  const ProdArgs a = {dtype, x, x_stride, nullptr, 0, w, rows, cols, n_experts, offsets, n_rows, 0, y, nullptr};
+  int rc = check_prod("linear", a);
+  if (!rc) rc = check_stride("linear", "x_stride", x_stride, cols, n_rows);
+  if (rc || n_rows == 0) return rc;
+  KTMI_REQUIRE(x && w && y, KTMI_EINVAL, "linear: null pointer");
+  return launch_prod_fwd(a, false, (hipStream_t)stream);
+}
+
+int ktmi_linear_grad_x(const void* dy, int dtype, int64_t dy_stride, int64_t rows, const void* w, int64_t cols,
+                       int64_t n_experts, const int32_t* offsets, int64_t n_rows, void* dx, void* stream) {
+  g_err[0] = 0;
+  const ProdArgs a = {dtype, nullptr, 0, dy, dy_stride, w, rows, cols, n_experts, offsets, n_rows, 0, dx, nullptr};
+  int rc = check_prod("linear_grad_x", a);
+  if (!rc) rc = check_stride("linear_grad_x", "dy_stride", dy_stride, rows, n_rows);
+  if (rc || n_rows == 0) return rc;
+  KTMI_REQUIRE(dy && w && dx, KTMI_EINVAL, "linear_grad_x: null pointer");
+  return launch_prod_dx(a, (hipStream_t)stream);
+}
+
+int ktmi_linear_grad_w(const void* dy, int dtype, int64_t dy_stride, int64_t rows, const void* x, int64_t x_stride,
+                       int64_t cols, int64_t n_experts, const int32_t* offsets, int64_t n_rows, void* dw, void* stream) {
+  g_err[0] = 0;
+  const ProdArgs a = {dtype, x, x_stride, dy, dy_stride, nullptr, rows, cols, n_experts, offsets, n_rows, 0, dw, nullptr};
+  int rc = check_prod("linear_grad_w", a);
+  if (!rc) rc = check_stride("linear_grad_w", "dy_stride", dy_stride, rows, n_rows);
+  if (!rc) rc = check_stride("linear_grad_w", "x_stride", x_stride, cols, n_rows);
+  if (rc) return rc;
+  KTMI_REQUIRE(dw && (n_rows == 0 || (dy && x)), KTMI_EINVAL, "linear_grad_w: null pointer");
+  return launch_prod_dw(a, (hipStream_t)stream);
+}
+
 // ---- scratch for ktmi_moe_layer_noalloc
 // A file-scope device array that stands in for the caller's workspace. In host code its
 // name is a host-side stand-in, not a device address: the address on each device comes

@@ -55,6 +55,45 @@ constexpr int W4_STEP = 128;  // columns of a step: 16 bytes of codes a lane
 constexpr int64_t W4_ROUTES = 1 << 23;  // rows of y of a call, at most: a grid has below 2^32 threads
 constexpr int W4_IDS = 64;    // routes whose ids a wave holds one a lane
 
+// Products by expert (prod.hip): rows of x or dy by the matrix of their expert, w [n_experts, rows, cols] (gated: [2 rows,
+// cols]); offsets NULL: one matrix. y: the products, or the gradient asked for. Strides in elements.
+struct ProdArgs {
+  int dtype;
+  const void* x;
+  int64_t x_stride;
+  const void* dy;
+  int64_t dy_stride;
+  const void* w;
+  int64_t rows, cols, n_experts;
+  const int32_t* offsets;
+  int64_t n_rows;
+  int act;
+  void* y;
+  float* sums;
+};
+int launch_prod_fwd(const ProdArgs& a, bool gated, hipStream_t stream);
+int launch_prod_dx(const ProdArgs& a, hipStream_t stream);
+int launch_prod_dw(const ProdArgs& a, hipStream_t stream);
+int launch_gated_grad(const float* sums, const void* dh, int dtype, int64_t dh_stride, int64_t inter, int64_t n_rows, int act,
+                      void* dsums, hipStream_t stream);
+// Products in 8-bit floating point: x [x_rows, cols] by e4m3 matrices with a scale for each block of 128 x 128; route r's
+// row of x is r / top_k and its expert ids[r], or that of the segment that holds row r, or the one matrix.
+struct Fp8Args {
+  int dtype;
+  const void* x;
+  int64_t x_stride, x_rows;
+  const uint8_t* w;
+  const float* scales;
+  int64_t rows, cols, n_experts;
+  const int32_t* ids;
+  int64_t top_k;
+  const int32_t* offsets;
+  void* y;
+  uint8_t* ws;
+};
+int64_t fp8_workspace(int64_t cols, int64_t x_rows, int64_t n_experts, int64_t top_k, bool ids);
+int launch_fp8(const Fp8Args& a, hipStream_t stream);
+
 // GEMV over raw GGUF rows against q8_1 activations (the decode-window kernel).
 // xq: q8_1 rows of the tokens, xq_stride bytes apart. W: slot tensor (w_is_table = 0,
 // experts w_expert_stride bytes apart) or int64 table of per-slot addresses. Expert ids

@@ -1,0 +1,217 @@
+// Products in 8-bit floating point (e4m3) of many rows: y[m, n] = sum over blocks g of 128 k of xs[m, g] ws[n / 128, g]
+// sum over k in g of x[m, k] w[n, k], on v_mfma_f32_16x16x128, whose k is one block.
+//
+// The matrix cores add e4m3 products of one instruction with about 16 bits below the largest (measured:
+// codes of normal values 1.5e-5 of the sums' norm, any codes 1.1e-4 of the terms' sum at worst). For y in 16 bits, rounded
+// at 2^-9 or 2^-12, that is enough; for y in fp32 the codes become bf16, which holds them exactly, and
+// the sums are those of v_mfma_f32_16x16x32_bf16.
+#pragma once
+#include "prod_tile.h"
+
+namespace ktmi {
+
+struct E4M3 {
+  using S = uint8_t;
+  static constexpr int ES = 1, EPC = 16;
+};
+
+// codes 8 hi .. 8 hi + 7 of a chunk's 16 as bf16, whose bits are the high half of the fp32 value's
+__device__ __forceinline__ bf16x8_t e4m3_to_bf16(u32x4_t c, int hi) {
+  u32x4_t v;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int d = (int)c[2 * hi + i];
+    const u32x2_t a = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_cvt_pk_f32_fp8(d, false));
+    const u32x2_t b = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_cvt_pk_f32_fp8(d, true));
+    v[2 * i] = __builtin_amdgcn_perm(a[1], a[0], 0x07060302);
+    v[2 * i + 1] = __builtin_amdgcn_perm(b[1], b[0], 0x07060302);
+  }
+  return __builtin_bit_cast(bf16x8_t, v);
+}
+
+// The products of 16 rows by 16 over one block: lane l holds chunks l / 16 and 4 + l / 16 of row l % 16.
+template <bool EXACT>
+__device__ __forceinline__ f32x4_t mma_block(const u32x4_t a[2], const u32x4_t b[2]) {
+  f32x4_t c = {0, 0, 0, 0};
+  if constexpr (EXACT) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e4m3_to_bf16(a[i / 2], i & 1), e4m3_to_bf16(b[i / 2], i & 1), c, 0, 0, 0);
+  } else {
+    const i32x8_t x = {(int)a[0][0], (int)a[0][1], (int)a[0][2], (int)a[0][3], (int)a[1][0], (int)a[1][1], (int)a[1][2], (int)a[1][3]};
+    const i32x8_t y = {(int)b[0][0], (int)b[0][1], (int)b[0][2], (int)b[0][3], (int)b[1][0], (int)b[1][1], (int)b[1][2], (int)b[1][3]};
+    c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 0, 0, 0, 0, 0, 0);  // no scales: their operands 0
+  }
+  return c;
+}
+
+// Chunks of X's as fp32 values.
+template <typename X, int XC>
+__device__ __forceinline__ void unpack_chunks(const u32x4_t (&x)[XC], float (&v)[XC * X::EPC]) {
+#pragma unroll
+  for (int c = 0; c < XC; ++c)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t d = x[c][i];  // (a bit cast of a vector's element takes its first one)
+      if constexpr (X::ES == 4) {
+        v[4 * c + i] = __builtin_bit_cast(float, d);
+      } else if constexpr (std::is_same<X, F16>::value) {
+        v[8 * c + 2 * i] = half_bits_to_float((uint16_t)d);
+        v[8 * c + 2 * i + 1] = half_bits_to_float((uint16_t)(d >> 16));
+      } else {
+        v[8 * c + 2 * i] = __builtin_bit_cast(float, d << 16);
+        v[8 * c + 2 * i + 1] = __builtin_bit_cast(float, d & 0xffff0000u);
+      }
+    }
+}
+
+// four values as e4m3 codes, to nearest, ties to even
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+  int u = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, u, true);
+}
+
+struct Fp8TileArgs {
+  const uint8_t* x;         // codes [rows, x_stride], quantised rows padded with zeros to whole blocks
+  const float* xs;          // scales [blocks, xs_stride]
+  int64_t x_stride, xs_stride, x_rows;
+  const uint8_t* w;         // codes [experts, N, K]
+  const float* ws;          // scales [experts, ceil(N / 128), blocks]
+  void* y;                  // [M, N]
+  int M, N, K;
+  Segments seg;             // offsets NULL: one matrix for all rows
+  const int32_t* perm;      // sorted routes: row p's codes are row perm[p] / top_k, its place in y perm[p] (its
+  int top_k;                // complement without an expert); NULL: row p
+};
+
+template <typename S, bool EXACT, bool DIRECT, int WM, int WN, int MF, int NF>
+__global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile(Fp8TileArgs a) {
+  constexpr int THREADS = 64 * WM * WN, BM = 16 * WM * MF, BN = 16 * WN * NF;
+  using P = TileOperand<E4M3, false, true, BM, THREADS>;
+  using Q = TileOperand<E4M3, false, DIRECT, BN, THREADS>;
+  constexpr int BUF = P::BYTES + Q::BYTES + BM * 4;
+  static_assert(BM % 64 == 0 && BM <= THREADS && 128 % (16 * NF) == 0 && BN % 128 == 0, "a wave's columns lie in one block");
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * BUF];
+
+  Place pl;
+  TileArgs t = {};
+  t.M = a.M, t.N = a.N, t.seg = a.seg;
+  if (!place_of<PROD_FWD, BM, BN>(t, pl)) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave % WM, wn = wave / WM, l16 = lane & 15, q4 = lane >> 4;
+  const int blocks = (a.K + 127) / 128;
+
+  f32x4_t acc[NF][MF] = {};
+  if (pl.expert >= 0) {
+    const int last = pl.rows - 1;
+    const uint8_t* pb = a.x;
+    int64_t pbytes = a.x_rows * a.x_stride;
+    int64_t sbase = 0;
+    if (!a.perm) pb += pl.m0 * a.x_stride, pbytes -= pl.m0 * a.x_stride, sbase = pl.m0;
+    auto row_of = [&](int i) {
+      const int r = min(i, last);
+      return a.perm ? a.perm[pl.m0 + r] / a.top_k : r;
+    };
+    P p;
+    Q q;
+    p.init(tid, a.x_stride, 0, row_of);
+    const uint8_t* qb = a.w + ((int64_t)pl.expert * a.N + pl.n0) * a.K;
+    const int64_t qbytes = (int64_t)(a.N - pl.n0) * a.K;
+    const int end = a.N - 1 - pl.n0;
+    q.init(tid, a.K, 0, [&](int i) { return min(i, end); });
+    const float* ws = a.ws + ((int64_t)pl.expert * ((a.N + 127) / 128) + min(pl.n0 + 16 * NF * wn, a.N - 1) / 128) * blocks;
+    const float* xs = a.xs + sbase + (tid < BM ? row_of(tid) : 0);
+    float xs_reg = 0;
+    auto load = [&](int k, int buf) {
+      uint8_t* b = lds + buf * BUF;
+      if (tid < BM) xs_reg = xs[k * a.xs_stride];
+      p.load(pb, pbytes, a.x_stride, k, blocks * 128, 0, b, tid);
+      q.load(qb, qbytes, a.K, k, a.K, 0, b + P::BYTES, tid);
+    };
+    auto put = [&](int buf) {
+      uint8_t* b = lds + buf * BUF;
+      if (tid < BM) *(float*)(b + P::BYTES + Q::BYTES + 4 * tid) = xs_reg;
+      q.put(b + P::BYTES, tid);
+    };
+    static_assert(MF % 2 == 0, "");
+    u32x4_t pf[2][2], qf[NF][2];
+    float sx[2];
+    auto read_row = [&](const uint8_t* src, int row, u32x4_t to[2]) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) to[c] = *(const u32x4_t*)(src + row * STEP_BYTES + 16 * row_slot(row, 4 * c + q4));
+    };
+    auto read_p = [&](int buf, int j, int to) {
+      const uint8_t* b = lds + buf * BUF;
+      const int row = 16 * (MF * wm + j) + l16;
+      read_row(b, row, pf[to]);
+      sx[to] = *(const float*)(b + P::BYTES + Q::BYTES + 4 * row);
+    };
+    auto read_q = [&](int buf) {
+#pragma unroll
+      for (int i = 0; i < NF; ++i) read_row(lds + buf * BUF + P::BYTES, 16 * (NF * wn + i) + l16, qf[i]);
+    };
+    load(0, 0);
+    put(0);
+    __builtin_amdgcn_s_waitcnt(WAIT_ALL);
+    block_barrier();
+    float sw = ws[0], sw_next = sw;
+    if (blocks > 1) load(1, 1), sw_next = ws[1];
+    read_q(0);
+    read_p(0, 0, 0);
+    // a block's sums are scaled and added while the matrix cores work on the next rows'
+    f32x4_t c[2][NF] = {};
+    float s[2] = {0, 0};
+    auto add = [&](int j) {
+#pragma unroll
+      for (int i = 0; i < NF; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(c[j & 1][i][r], s[j & 1], acc[i][j][r]);
+    };
+    for (int k = 0; k < blocks; ++k) {
+      const int buf = k & 1;
+#pragma unroll
+      for (int j = 0; j < MF; ++j) {
+        if (j + 1 < MF) {
+          read_p(buf, j + 1, (j + 1) & 1);
+        } else {
+          // the step's last rows are in registers, and its columns too: the buffer is free for step k + 2 once
+          // every wave is here, and step k + 1's loads, on their way since the last such place, have to be there
+          if (k + 1 < blocks) put(buf ^ 1);
+          __builtin_amdgcn_s_waitcnt(WAIT_ALL);
+          block_barrier();
+          if (k + 2 < blocks) load(k + 2, buf);
+        }
+        s[j & 1] = sx[j & 1] * sw;
+#pragma unroll
+        for (int i = 0; i < NF; ++i) c[j & 1][i] = mma_block<EXACT>(qf[i], pf[j & 1]);
+        add((j + MF - 1) % MF);  // of the step before at first: zeros before the first step
+      }
+      if (k + 1 < blocks) {
+        sw = sw_next;
+        if (k + 2 < blocks) sw_next = ws[k + 2];
+        read_q(buf ^ 1);
+        read_p(buf ^ 1, 0, 0);
+      }
+    }
+    settle(c);
+    add(MF - 1);
+  }
+
+  // fragment (i, j): the lane holds row 16 j + lane % 16 of x's, rows 4 (lane / 16) + r of w's
+  const bool vec = a.N % 4 == 0 && (uintptr_t)a.y % (4 * sizeof(S)) == 0;
+#pragma unroll
+  for (int j = 0; j < MF; ++j) {
+    const int m = 16 * (MF * wm + j) + l16;
+    if (m >= pl.rows) continue;
+    int at = pl.m0 + m;
+    if (a.perm) at = pl.expert >= 0 ? a.perm[at] : ~a.perm[at];
+    S* row = (S*)a.y + (int64_t)at * a.N;
+#pragma unroll
+    for (int i = 0; i < NF; ++i) {
+      const int n = pl.n0 + 16 * (NF * wn + i) + 4 * q4;
+      if (n < a.N) store4(row, n, a.N, vec, acc[i][j]);
+    }
+  }
+}
+
+}  // namespace ktmi

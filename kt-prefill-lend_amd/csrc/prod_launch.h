@@ -1,0 +1,182 @@
+// The choice of kernels of the products by expert, compiled once for each element type (prod_bf16.hip and its like).
+#pragma once
+#include "prod_rows.h"
+
+namespace ktmi {
+
+// Tiles of 256 x 256 by 8 waves, or 128 x 128 by 4, of which two share a CU.
+template <typename T, int MODE, bool GATED, bool DIRECT, bool LARGE>
+int launch_tile_of(const TileArgs& a, hipStream_t stream) {
+  constexpr int BM = LARGE ? 256 : 128, BN = (LARGE ? 256 : 128) / (GATED ? 2 : 1), THREADS = LARGE ? 512 : 256;
+  const int64_t nt = (a.N + BN - 1) / BN;
+  int64_t mt = (a.M + BM - 1) / BM;
+  if (a.seg.offsets) mt = MODE == PROD_DW ? mt * a.seg.E : a.M / BM + a.seg.E + 2;
+  const int64_t grid = (mt * nt + 7) / 8 * 8;
+  KTMI_REQUIRE(grid < (int64_t)0xffffffff / THREADS, KTMI_EINVAL, "a grid of %lld blocks (below 2^32 threads)", (long long)grid);
+  if constexpr (LARGE) prod_tile<T, MODE, GATED, DIRECT, 2, 4, 4, 2><<<(unsigned)grid, THREADS, 0, stream>>>(a);
+  else prod_tile<T, MODE, GATED, DIRECT, 2, 2, 2, 2><<<(unsigned)grid, THREADS, 0, stream>>>(a);
+  KTMI_HIP_TRY(hipGetLastError());
+  return KTMI_OK;
+}
+
+// Rows at multiples of 16 bytes, whose tiles 32-bit offsets reach.
+inline bool rows_direct(const void* p, int64_t stride, int64_t span) {
+  return ((uintptr_t)p | (uintptr_t)stride) % 16 == 0 && span * stride < 0x7fffffff;
+}
+
+template <typename T, int MODE, bool GATED>
+int launch_tile(const TileArgs& a, hipStream_t stream) {
+  const int64_t wide = MODE == PROD_FWD && GATED ? 2 * (int64_t)a.N : 256;
+  // k past the operands' ends comes in whole chunks where it runs along the rows; across them rows end anywhere
+  const bool ends = MODE == PROD_DW || a.K % T::EPC == 0;
+  const bool direct = ends && rows_direct(a.p, a.p_stride, 256) && rows_direct(a.q, a.q_stride, wide) && a.q_expert % 16 == 0;
+  if (!direct) return launch_tile_of<T, MODE, GATED, false, false>(a, stream);
+  const int64_t parts = a.seg.offsets ? a.seg.E : 1;
+  const int64_t m = MODE == PROD_DW ? a.M : a.M / parts;
+  const int64_t tiles = (m + 255) / 256 * ((a.N * (GATED ? 2 : 1) + 255) / 256) * parts;
+  if (m >= 192 && tiles >= 192) return launch_tile_of<T, MODE, GATED, true, true>(a, stream);
+  return launch_tile_of<T, MODE, GATED, true, false>(a, stream);
+}
+
+template <typename X, bool FP8, bool GATED, int CT, int NRF>
+int launch_rows_of(RowsArgs a, hipStream_t stream) {
+  constexpr int WAVES = 8, OUT = (GATED ? 8 : 16) * NRF;
+  a.row_tiles = (a.N + OUT - 1) / OUT;
+  int64_t tiles = (a.R + 16 * CT - 1) / (16 * CT);
+  if (a.ids) tiles = a.R;
+  else if (a.seg.offsets) tiles = a.R / (16 * CT) + min(a.seg.E + 2, a.R);
+  const int64_t grid = tiles * a.row_tiles;
+  KTMI_REQUIRE(grid < (int64_t)0xffffffff / (64 * WAVES), KTMI_EINVAL, "a grid of %lld blocks (below 2^32 threads)",
+               (long long)grid);
+  prod_rows<X, FP8, GATED, CT, NRF, WAVES><<<(unsigned)grid, 64 * WAVES, 0, stream>>>(a);
+  KTMI_HIP_TRY(hipGetLastError());
+  return KTMI_OK;
+}
+
+template <typename X, bool FP8, bool GATED>
+int launch_rows(const RowsArgs& a, int mean, hipStream_t stream) {
+  if (mean <= 16) return launch_rows_of<X, FP8, GATED, 1, 1>(a, stream);
+  if (mean <= 32) return launch_rows_of<X, FP8, GATED, 2, 1>(a, stream);
+  return launch_rows_of<X, FP8, GATED, 4, 2>(a, stream);
+}
+
+template <typename X>
+int launch_fp8_tile(const Fp8TileArgs& a, hipStream_t stream) {
+  using S = typename X::S;
+  constexpr bool EXACT = std::is_same<X, F32>::value;
+  const bool direct = rows_direct(a.w, a.K, 256);
+  const int64_t mean = a.seg.offsets ? a.M / a.seg.E : a.M;
+  const bool large = direct && mean >= 192 && (mean + 255) / 256 * ((a.N + 255) / 256) * (a.seg.offsets ? a.seg.E : 1) >= 192;
+  const int64_t bm = large ? 256 : 128, bn = large ? 256 : 128, threads = large ? 512 : 256;
+  const int64_t mt = a.seg.offsets ? a.M / bm + a.seg.E + 2 : (a.M + bm - 1) / bm;
+  const int64_t grid = (mt * ((a.N + bn - 1) / bn) + 7) / 8 * 8;
+  KTMI_REQUIRE(grid < (int64_t)0xffffffff / threads, KTMI_EINVAL, "a grid of %lld blocks (below 2^32 threads)", (long long)grid);
+  if (large) fp8_tile<S, EXACT, true, 2, 4, 8, 4><<<(unsigned)grid, 512, 0, stream>>>(a);
+  else if (direct) fp8_tile<S, EXACT, true, 2, 2, 4, 4><<<(unsigned)grid, 256, 0, stream>>>(a);
+  else fp8_tile<S, EXACT, false, 2, 2, 4, 4><<<(unsigned)grid, 256, 0, stream>>>(a);
+  KTMI_HIP_TRY(hipGetLastError());
+  return KTMI_OK;
+}
+
+// ---- one group of 16 lanes a group of 128 values: codes [rows, blocks * 128], scales [blocks, rows]
+template <typename X>
+__global__ __launch_bounds__(256) void fp8_quantise(const uint8_t* x, int64_t stride, int K, int64_t rows, uint8_t* codes,
+                                                    float* scales) {
+  const int blocks = (K + 127) / 128;
+  const int64_t g = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+  const int i = threadIdx.x & 15;
+  // sixteen rows of a column of groups after each other, then the next column's
+  const int64_t band = g / (16 * (int64_t)blocks);
+  const int in = (int)(g - band * 16 * blocks);
+  const int64_t row = band * 16 + in % 16;
+  const int b = in / 16;
+  if (row >= rows) return;  // the whole group
+  constexpr int XC = 8 / X::EPC;
+  u32x4_t c[XC];
+  const uint8_t* r = x + row * stride * X::ES;
+#pragma unroll
+  for (int j = 0; j < XC; ++j) c[j] = load_chunk<X::ES>(r, (int64_t)b * 128 + 8 * i + X::EPC * j, K);
+  float v[8];
+  unpack_chunks<X>(c, v);
+  float top = 0x1p-116f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[j]));
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+  const float inv = 448.0f / top;
+  const u32x2_t q = {e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv), e4m3x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv)};
+  *(u32x2_t*)(codes + (row * blocks + b) * 128 + 8 * i) = q;
+  if (i == 0) scales[b * rows + row] = top / 448.0f;
+}
+
+template <typename X>
+int launch_quantise(const void* x, int64_t stride, int64_t K, int64_t rows, uint8_t* codes, float* scales, hipStream_t stream) {
+  const int64_t groups = (rows + 15) / 16 * 16 * ((K + 127) / 128);
+  KTMI_REQUIRE(groups / 16 < (int64_t)0xffffffff / 256, KTMI_EINVAL, "fp8: %lld groups of 128 values (below 2^28)",
+               (long long)groups);
+  fp8_quantise<X><<<(unsigned)(groups / 16), 256, 0, stream>>>((const uint8_t*)x, stride, (int)K, rows, codes, scales);
+  KTMI_HIP_TRY(hipGetLastError());
+  return KTMI_OK;
+}
+
+// ---- the gradients of the sums from that of h = act(g) u: dg = dh u act'(g), du = dh act(g)
+template <typename T>
+__global__ __launch_bounds__(256) void gated_grad(const float* gu, const uint8_t* dh, int64_t dh_stride, int N, int64_t rows,
+                                                  int act, uint8_t* dgu) {
+  using S = typename T::S;
+  const int64_t n4 = (N + 3) / 4, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = at / n4;
+  const int n = 4 * (int)(at - row * n4);
+  if (row >= rows) return;
+  const float *g = gu + row * 2 * N + n, *u = g + N;
+  const S* d = (const S*)dh + row * dh_stride + n;
+  S *dg = (S*)dgu + row * 2 * N + n, *du = dg + N;
+  typedef typename vec4_of<S>::type V;
+  // vectors of four where every row starts at one
+  if (N % 4 == 0 && dh_stride % 4 == 0 && ((uintptr_t)dh | (uintptr_t)dgu) % sizeof(V) == 0) {
+    const f32x4_t gv = gload<f32x4_t>(g), uv = gload<f32x4_t>(u);
+    const V dv = gload<V>(d);
+    V a, b;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float f, df;
+      act_grad(act, gv[i], f, df);
+      a[i] = (S)((float)dv[i] * uv[i] * df);
+      b[i] = (S)((float)dv[i] * f);
+    }
+    *(V*)dg = a;
+    *(V*)du = b;
+  } else {
+    for (int i = 0; i < 4 && n + i < N; ++i) {
+      float f, df;
+      act_grad(act, g[i], f, df);
+      dg[i] = (S)((float)d[i] * u[i] * df);
+      du[i] = (S)((float)d[i] * f);
+    }
+  }
+}
+
+template <typename T>
+int launch_gated_grad(const float* gu, const void* dh, int64_t dh_stride, int64_t N, int64_t rows, int act, void* dgu,
+                      hipStream_t stream) {
+  const int64_t grid = ((N + 3) / 4 * rows + 255) / 256;
+  KTMI_REQUIRE(grid < (int64_t)0xffffffff / 256, KTMI_EINVAL, "gated_grad: %lld values (below 2^34)", (long long)(N * rows));
+  gated_grad<T><<<(unsigned)grid, 256, 0, stream>>>(gu, (const uint8_t*)dh, dh_stride, (int)N, rows, act, (uint8_t*)dgu);
+  KTMI_HIP_TRY(hipGetLastError());
+  return KTMI_OK;
+}
+
+template <typename T>
+struct ProdOps {
+  static int tile(int mode, bool gated, const TileArgs& a, hipStream_t s) {
+    if (mode == PROD_DX) return launch_tile<T, PROD_DX, false>(a, s);
+    if (mode == PROD_DW) return launch_tile<T, PROD_DW, false>(a, s);
+    return gated ? launch_tile<T, PROD_FWD, true>(a, s) : launch_tile<T, PROD_FWD, false>(a, s);
+  }
+  static int rows(bool fp8, bool gated, const RowsArgs& a, int mean, hipStream_t s) {
+    if (fp8) return launch_rows<T, true, false>(a, mean, s);
+    return gated ? launch_rows<T, false, true>(a, mean, s) : launch_rows<T, false, false>(a, mean, s);
+  }
+};
+
+}  // namespace ktmi
