@@ -106,7 +106,7 @@ static int launch_fp8_slice(const Fp8Args& a, hipStream_t stream) {
   }
   float* xs = (float*)ws;
   uint8_t* codes = ws + 4 * ints(blocks * a.x_rows);
-  const int rc = t.quantise(a.x, a.x_stride, a.cols, a.x_rows, codes, xs, stream);
+  const int rc = t.quantise(a.x, a.x_stride, a.cols, a.x_rows, a.offsets ? a.offsets + a.n_experts : nullptr, codes, xs, stream);
   if (rc) return rc;
   Fp8TileArgs f = {};
   f.x = codes, f.xs = xs, f.x_stride = blocks * 128, f.xs_stride = a.x_rows, f.x_rows = a.x_rows;

@@ -124,31 +124,33 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile(Fp8TileArgs a) {
     float xs_reg = 0;
     auto load = [&](int k, int buf) {
       uint8_t* b = lds + buf * BUF;
-      if (tid < BM) xs_reg = xs[k * a.xs_stride];
+      if (wave < BM / 64) xs_reg = xs[k * a.xs_stride];
       p.load(pb, pbytes, a.x_stride, k, blocks * 128, 0, b, tid);
       q.load(qb, qbytes, a.K, k, a.K, 0, b + P::BYTES, tid);
     };
     auto put = [&](int buf) {
       uint8_t* b = lds + buf * BUF;
-      if (tid < BM) *(float*)(b + P::BYTES + Q::BYTES + 4 * tid) = xs_reg;
+      if (wave < BM / 64) *(float*)(b + P::BYTES + Q::BYTES + 4 * tid) = xs_reg;
       q.put(b + P::BYTES, tid);
     };
     static_assert(MF % 2 == 0, "");
     u32x4_t pf[2][2], qf[NF][2];
     float sx[2];
-    auto read_row = [&](const uint8_t* src, int row, u32x4_t to[2]) {
-#pragma unroll
-      for (int c = 0; c < 2; ++c) to[c] = *(const u32x4_t*)(src + row * STEP_BYTES + 16 * row_slot(row, 4 * c + q4));
-    };
+    // a lane's chunks of fragment 0 of x's and w's rows (fragment j is 16 rows on, with the same slots), its scale
+    const int slot[2] = {16 * row_slot(l16, q4), 16 * row_slot(l16, 4 + q4)};
+    const int p_at = (16 * MF * wm + l16) * STEP_BYTES, q_at = P::BYTES + (16 * NF * wn + l16) * STEP_BYTES;
+    const int s_at = P::BYTES + Q::BYTES + 4 * (16 * MF * wm + l16);
     auto read_p = [&](int buf, int j, int to) {
       const uint8_t* b = lds + buf * BUF;
-      const int row = 16 * (MF * wm + j) + l16;
-      read_row(b, row, pf[to]);
-      sx[to] = *(const float*)(b + P::BYTES + Q::BYTES + 4 * row);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) pf[to][c] = *(const u32x4_t*)(b + p_at + slot[c] + 16 * j * STEP_BYTES);
+      sx[to] = *(const float*)(b + s_at + 64 * j);
     };
     auto read_q = [&](int buf) {
 #pragma unroll
-      for (int i = 0; i < NF; ++i) read_row(lds + buf * BUF + P::BYTES, 16 * (NF * wn + i) + l16, qf[i]);
+      for (int i = 0; i < NF; ++i)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) qf[i][c] = *(const u32x4_t*)(lds + buf * BUF + q_at + slot[c] + 16 * i * STEP_BYTES);
     };
     load(0, 0);
     put(0);
@@ -158,15 +160,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile(Fp8TileArgs a) {
     if (blocks > 1) load(1, 1), sw_next = ws[1];
     read_q(0);
     read_p(0, 0, 0);
-    // a block's sums are scaled and added while the matrix cores work on the next rows'
-    f32x4_t c[2][NF] = {};
-    float s[2] = {0, 0};
-    auto add = [&](int j) {
-#pragma unroll
-      for (int i = 0; i < NF; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(c[j & 1][i][r], s[j & 1], acc[i][j][r]);
-    };
     for (int k = 0; k < blocks; ++k) {
       const int buf = k & 1;
 #pragma unroll
@@ -181,10 +174,20 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile(Fp8TileArgs a) {
           block_barrier();
           if (k + 2 < blocks) load(k + 2, buf);
         }
-        s[j & 1] = sx[j & 1] * sw;
+        // scaled and added right behind the products (the asm keeps the compiler from moving that past the branches
+        // below, see settle(), with every block's sums in registers till then): the SIMD's other wave has the matrix cores
+        // meanwhile
+        const float s = sx[j & 1] * sw;
+        f32x4_t c[NF];
 #pragma unroll
-        for (int i = 0; i < NF; ++i) c[j & 1][i] = mma_block<EXACT>(qf[i], pf[j & 1]);
-        add((j + MF - 1) % MF);  // of the step before at first: zeros before the first step
+        for (int i = 0; i < NF; ++i) c[i] = mma_block<EXACT>(qf[i], pf[j & 1]);
+#pragma unroll
+        for (int i = 0; i < NF; ++i) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(c[i][r], s, acc[i][j][r]);
+          asm volatile("" : "+v"(acc[i][j]));
+        }
+        __builtin_amdgcn_sched_barrier(0);  // reads moved further ahead than one fragment cost more registers than there are
       }
       if (k + 1 < blocks) {
         sw = sw_next;
@@ -193,8 +196,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile(Fp8TileArgs a) {
         read_p(buf ^ 1, 0, 0);
       }
     }
-    settle(c);
-    add(MF - 1);
   }
 
   // fragment (i, j): the lane holds row 16 j + lane % 16 of x's, rows 4 (lane / 16) + r of w's

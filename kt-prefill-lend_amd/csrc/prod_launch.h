@@ -38,9 +38,9 @@ int launch_tile(const TileArgs& a, hipStream_t stream) {
   return launch_tile_of<T, MODE, GATED, true, false>(a, stream);
 }
 
-template <typename X, bool FP8, bool GATED, int CT, int NRF>
+template <typename X, bool FP8, bool GATED, int CT, int NRF, int WK>
 int launch_rows_of(RowsArgs a, hipStream_t stream) {
-  constexpr int WAVES = 8, OUT = (GATED ? 8 : 16) * NRF;
+  constexpr int WAVES = 8, OUT = (GATED ? 8 : 16) * NRF * (WAVES / WK);
   a.row_tiles = (a.N + OUT - 1) / OUT;
   int64_t tiles = (a.R + 16 * CT - 1) / (16 * CT);
   if (a.ids) tiles = a.R;
@@ -48,16 +48,30 @@ int launch_rows_of(RowsArgs a, hipStream_t stream) {
   const int64_t grid = tiles * a.row_tiles;
   KTMI_REQUIRE(grid < (int64_t)0xffffffff / (64 * WAVES), KTMI_EINVAL, "a grid of %lld blocks (below 2^32 threads)",
                (long long)grid);
-  prod_rows<X, FP8, GATED, CT, NRF, WAVES><<<(unsigned)grid, 64 * WAVES, 0, stream>>>(a);
+  prod_rows<X, FP8, GATED, CT, NRF, WK, WAVES / WK><<<(unsigned)grid, 64 * WAVES, 0, stream>>>(a);
   KTMI_HIP_TRY(hipGetLastError());
   return KTMI_OK;
 }
 
+// mean: rows of a matrix. Rows of w a wave: 16 where more would leave CUs without a block, else 64 (32 against 64 rows of
+// x), which share the rows of x and, of e4m3, their quantisation. Rows of w below 16 units are too short for eight
+// waves: two share one.
 template <typename X, bool FP8, bool GATED>
 int launch_rows(const RowsArgs& a, int mean, hipStream_t stream) {
-  if (mean <= 16) return launch_rows_of<X, FP8, GATED, 1, 1>(a, stream);
-  if (mean <= 32) return launch_rows_of<X, FP8, GATED, 2, 1>(a, stream);
-  return launch_rows_of<X, FP8, GATED, 4, 2>(a, stream);
+  constexpr int UE = 128 / (FP8 ? 1 : X::ES);
+  const bool shorter = a.K < 16 * UE;
+  const int64_t cols = mean <= 16 ? 16 : mean <= 32 ? 32 : 64;
+  const int64_t parts = a.ids || a.seg.offsets ? min((int64_t)a.seg.E, (int64_t)a.R) : (a.R + cols - 1) / cols;
+  const int64_t frags = parts * (GATED ? 2 : 1) * a.N / 16;
+  if (cols == 16) {
+    if (frags < 4 * 512) return launch_rows_of<X, FP8, GATED, 1, 1, 8>(a, stream);
+    return shorter ? launch_rows_of<X, FP8, GATED, 1, 2, 2>(a, stream) : launch_rows_of<X, FP8, GATED, 1, 4, 8>(a, stream);
+  }
+  if (cols == 32) {
+    if (frags < 4 * 512) return launch_rows_of<X, FP8, GATED, 2, 1, 8>(a, stream);
+    return shorter ? launch_rows_of<X, FP8, GATED, 2, 2, 2>(a, stream) : launch_rows_of<X, FP8, GATED, 2, 2, 8>(a, stream);
+  }
+  return shorter ? launch_rows_of<X, FP8, GATED, 4, 2, 2>(a, stream) : launch_rows_of<X, FP8, GATED, 4, 2, 8>(a, stream);
 }
 
 template <typename X>
@@ -66,12 +80,15 @@ int launch_fp8_tile(const Fp8TileArgs& a, hipStream_t stream) {
   constexpr bool EXACT = std::is_same<X, F32>::value;
   const bool direct = rows_direct(a.w, a.K, 256);
   const int64_t mean = a.seg.offsets ? a.M / a.seg.E : a.M;
-  const bool large = direct && mean >= 192 && (mean + 255) / 256 * ((a.N + 255) / 256) * (a.seg.offsets ? a.seg.E : 1) >= 192;
+  const bool large = direct && !EXACT && mean >= 192 && (mean + 255) / 256 * ((a.N + 255) / 256) * (a.seg.offsets ? a.seg.E : 1) >= 192;
   const int64_t bm = large ? 256 : 128, bn = large ? 256 : 128, threads = large ? 512 : 256;
   const int64_t mt = a.seg.offsets ? a.M / bm + a.seg.E + 2 : (a.M + bm - 1) / bm;
   const int64_t grid = (mt * ((a.N + bn - 1) / bn) + 7) / 8 * 8;
   KTMI_REQUIRE(grid < (int64_t)0xffffffff / threads, KTMI_EINVAL, "a grid of %lld blocks (below 2^32 threads)", (long long)grid);
-  if (large) fp8_tile<S, EXACT, true, 2, 4, 8, 4><<<(unsigned)grid, 512, 0, stream>>>(a);
+  if constexpr (!EXACT) {
+    if (large) fp8_tile<S, EXACT, true, 2, 4, 8, 4><<<(unsigned)grid, 512, 0, stream>>>(a);
+  }
+  if (large) ;
   else if (direct) fp8_tile<S, EXACT, true, 2, 2, 4, 4><<<(unsigned)grid, 256, 0, stream>>>(a);
   else fp8_tile<S, EXACT, false, 2, 2, 4, 4><<<(unsigned)grid, 256, 0, stream>>>(a);
   KTMI_HIP_TRY(hipGetLastError());
@@ -80,8 +97,8 @@ int launch_fp8_tile(const Fp8TileArgs& a, hipStream_t stream) {
 
 // ---- one group of 16 lanes a group of 128 values: codes [rows, blocks * 128], scales [blocks, rows]
 template <typename X>
-__global__ __launch_bounds__(256) void fp8_quantise(const uint8_t* x, int64_t stride, int K, int64_t rows, uint8_t* codes,
-                                                    float* scales) {
+__global__ __launch_bounds__(256) void fp8_quantise(const uint8_t* x, int64_t stride, int K, int64_t rows, const int32_t* end,
+                                                    uint8_t* codes, float* scales) {
   const int blocks = (K + 127) / 128;
   const int64_t g = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
   const int i = threadIdx.x & 15;
@@ -90,7 +107,7 @@ __global__ __launch_bounds__(256) void fp8_quantise(const uint8_t* x, int64_t st
   const int in = (int)(g - band * 16 * blocks);
   const int64_t row = band * 16 + in % 16;
   const int b = in / 16;
-  if (row >= rows) return;  // the whole group
+  if (row >= rows || (end && row >= *end)) return;  // the whole group; end: rows behind the last segment have no product
   constexpr int XC = 8 / X::EPC;
   u32x4_t c[XC];
   const uint8_t* r = x + row * stride * X::ES;
@@ -110,11 +127,12 @@ __global__ __launch_bounds__(256) void fp8_quantise(const uint8_t* x, int64_t st
 }
 
 template <typename X>
-int launch_quantise(const void* x, int64_t stride, int64_t K, int64_t rows, uint8_t* codes, float* scales, hipStream_t stream) {
+int launch_quantise(const void* x, int64_t stride, int64_t K, int64_t rows, const int32_t* end, uint8_t* codes, float* scales,
+                    hipStream_t stream) {
   const int64_t groups = (rows + 15) / 16 * 16 * ((K + 127) / 128);
   KTMI_REQUIRE(groups / 16 < (int64_t)0xffffffff / 256, KTMI_EINVAL, "fp8: %lld groups of 128 values (below 2^28)",
                (long long)groups);
-  fp8_quantise<X><<<(unsigned)(groups / 16), 256, 0, stream>>>((const uint8_t*)x, stride, (int)K, rows, codes, scales);
+  fp8_quantise<X><<<(unsigned)(groups / 16), 256, 0, stream>>>((const uint8_t*)x, stride, (int)K, rows, end, codes, scales);
   KTMI_HIP_TRY(hipGetLastError());
   return KTMI_OK;
 }

@@ -1,9 +1,9 @@
 // Products of few rows: y[r, n] = sum over k of x[r, k] w[n, k], for decode windows, bound by the bytes of w.
 //
-// A block takes 16 NRF rows of w (gated: 8 of the gate and the 8 rows of up beside them, for each 16) and at most 16 CT rows of
-// x, which are the columns of the matrix cores' tiles. Its WAVES waves share the k: wave i takes the 128-byte units
-// i, i + WAVES, .. of the rows, so that they read neighbouring bytes, and each unit of x is read by
-// one wave only, straight into the operands' registers. The waves' sums meet in LDS.
+// A wave takes 16 NRF rows of w (gated: 8 of the gate and the 8 rows of up beside them, for each 16) and at most 16 CT rows of
+// x, which are the columns of the matrix cores' tiles. WK waves of a block share the k: wave i takes the 128-byte units
+// i, i + WK, .. of the rows, so that they read neighbouring bytes, and each unit of x is read by one of them
+// only, straight into the operands' registers; their sums meet in LDS. The block's other waves take the rows behind.
 #pragma once
 #include "prod_fp8.h"
 
@@ -45,21 +45,21 @@ __device__ __forceinline__ float quantise_unit(const u32x4_t (&x)[XC], u32x4_t c
 }
 
 // FP8: e4m3 rows of w against rows of type X, quantised on the way; else rows of X's type.
-template <typename X, bool FP8, bool GATED, int CT, int NRF, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void prod_rows(RowsArgs a) {
+template <typename X, bool FP8, bool GATED, int CT, int NRF, int WK, int WR>
+__global__ __launch_bounds__(64 * WK * WR) void prod_rows(RowsArgs a) {
   using S = typename X::S;
   static_assert(!FP8 || !GATED, "");
   constexpr int ES = FP8 ? 1 : X::ES;                 // bytes of an element of w
   constexpr int UE = 128 / ES;                        // elements of a unit
   constexpr int XC = UE * X::ES / 64;                 // chunks of x a lane a unit
-  constexpr int COLS = 16 * CT, OUT = GATED ? 8 * NRF : 16 * NRF;
-  constexpr int DEPTH = FP8 ? 2 : CT * NRF <= 2 ? 4 : 2;  // units on their way at once
-  __shared__ float red[WAVES][NRF * CT * 4][64];
+  constexpr int COLS = 16 * CT, MINE = GATED ? 8 * NRF : 16 * NRF, OUT = MINE * WR;  // rows of y a wave, a block
+  constexpr int DEPTH = CT * NRF == 1 ? 4 : 2;        // units on their way at once
+  __shared__ float red[WK][WR * NRF * CT * 4][64];
   __shared__ int list[64];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int l16 = lane & 15, q4 = lane >> 4;
-  const int tile = blockIdx.x / a.row_tiles, n0 = (blockIdx.x - tile * a.row_tiles) * OUT;
+  const int l16 = lane & 15, q4 = lane >> 4, wk = wave % WK, wr = wave / WK;
+  const int tile = blockIdx.x / a.row_tiles, n0 = (blockIdx.x - tile * a.row_tiles) * OUT, nw = n0 + wr * MINE;
 
   // the block's expert and rows
   int expert, row0 = 0, rows;
@@ -104,16 +104,16 @@ __global__ __launch_bounds__(64 * WAVES) void prod_rows(RowsArgs a) {
       const int r = out_row(min(16 * t + l16, rows - 1));
       xr[t] = (const uint8_t*)a.x + (int64_t)(a.ids || a.perm ? r / a.top_k : r) * a.x_stride * X::ES;
     }
-    const uint8_t* wr[NRF];
+    const uint8_t* rows_w[NRF];
     const float* ws[NRF];
     const int units = (a.K + UE - 1) / UE;
 #pragma unroll
     for (int f = 0; f < NRF; ++f) {
       int n;
-      if constexpr (GATED) n = min(n0 + 8 * f + (l16 & 7), a.N - 1) + (l16 >> 3) * a.N;
-      else n = min(n0 + 16 * f + l16, a.N - 1);
-      wr[f] = a.w + expert * a.w_expert + (int64_t)n * a.K * ES;
-      if constexpr (FP8) ws[f] = a.ws + ((int64_t)expert * ((a.N + 127) / 128) + min(n0 + 16 * f, a.N - 1) / 128) * units;
+      if constexpr (GATED) n = min(nw + 8 * f + (l16 & 7), a.N - 1) + (l16 >> 3) * a.N;
+      else n = min(nw + 16 * f + l16, a.N - 1);
+      rows_w[f] = a.w + expert * a.w_expert + (int64_t)n * a.K * ES;
+      if constexpr (FP8) ws[f] = a.ws + ((int64_t)expert * ((a.N + 127) / 128) + min(nw + 16 * f, a.N - 1) / 128) * units;
     }
     struct Unit {
       u32x4_t w[NRF][2], x[CT][XC];
@@ -127,7 +127,7 @@ __global__ __launch_bounds__(64 * WAVES) void prod_rows(RowsArgs a) {
 #pragma unroll
         for (int f = 0; f < NRF; ++f)
 #pragma unroll
-          for (int c = 0; c < 2; ++c) v.w[f][c] = gload<u32x4_a1_t>(wr[f] + (k + 4 * CE * c + CE * q4) * ES);
+          for (int c = 0; c < 2; ++c) v.w[f][c] = gload<u32x4_a1_t>(rows_w[f] + (k + 4 * CE * c + CE * q4) * ES);
 #pragma unroll
         for (int t = 0; t < CT; ++t)
 #pragma unroll
@@ -137,7 +137,7 @@ __global__ __launch_bounds__(64 * WAVES) void prod_rows(RowsArgs a) {
 #pragma unroll
         for (int f = 0; f < NRF; ++f)
 #pragma unroll
-          for (int c = 0; c < 2; ++c) v.w[f][c] = load_chunk<ES>(wr[f], k + 4 * CE * c + CE * q4, a.K);
+          for (int c = 0; c < 2; ++c) v.w[f][c] = load_chunk<ES>(rows_w[f], k + 4 * CE * c + CE * q4, a.K);
 #pragma unroll
         for (int t = 0; t < CT; ++t)
 #pragma unroll
@@ -174,17 +174,17 @@ __global__ __launch_bounds__(64 * WAVES) void prod_rows(RowsArgs a) {
       }
     };
     // the wave's units, DEPTH of them on their way
-    const int mine = units > wave ? (units - wave + WAVES - 1) / WAVES : 0;
+    const int mine = units > wk ? (units - wk + WK - 1) / WK : 0;
     Unit ring[DEPTH];
 #pragma unroll
     for (int i = 0; i < DEPTH; ++i)
-      if (i < mine) load(wave + WAVES * i, ring[i]);
+      if (i < mine) load(wk + WK * i, ring[i]);
     for (int i = 0; i < mine; i += DEPTH) {
 #pragma unroll
       for (int d = 0; d < DEPTH; ++d) {
         if (i + d >= mine) break;
         compute(ring[d]);
-        if (i + d + DEPTH < mine) load(wave + WAVES * (i + d + DEPTH), ring[d]);
+        if (i + d + DEPTH < mine) load(wk + WK * (i + d + DEPTH), ring[d]);
       }
     }
     settle(acc);
@@ -193,7 +193,7 @@ __global__ __launch_bounds__(64 * WAVES) void prod_rows(RowsArgs a) {
 #pragma unroll
       for (int t = 0; t < CT; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) red[wave][(f * CT + t) * 4 + r][lane] = acc[f][t][r];
+        for (int r = 0; r < 4; ++r) red[wk][((wr * NRF + f) * CT + t) * 4 + r][lane] = acc[f][t][r];
   }
   __syncthreads();
 
@@ -202,10 +202,10 @@ __global__ __launch_bounds__(64 * WAVES) void prod_rows(RowsArgs a) {
     const int at = (f * CT + (c >> 4)) * 4 + (row & 3), l = 16 * (row >> 2) + (c & 15);
     float s = 0;
 #pragma unroll
-    for (int i = 0; i < WAVES; ++i) s += red[i][at][l];
+    for (int i = 0; i < WK; ++i) s += red[i][at][l];
     return s;
   };
-  for (int o = tid; o < OUT * rows; o += 64 * WAVES) {
+  for (int o = tid; o < OUT * rows; o += 64 * WK * WR) {
     const int c = o / OUT, n = o - c * OUT;
     if (n0 + n >= a.N) continue;
     const int64_t at = out_row(c);
@@ -229,7 +229,8 @@ struct ProdTable {
   int (*tile)(int mode, bool gated, const TileArgs& a, hipStream_t stream);
   int (*rows)(bool fp8, bool gated, const RowsArgs& a, int mean, hipStream_t stream);
   int (*fp8_tile)(const Fp8TileArgs& a, hipStream_t stream);
-  int (*quantise)(const void* x, int64_t stride, int64_t K, int64_t rows, uint8_t* codes, float* scales, hipStream_t stream);
+  int (*quantise)(const void* x, int64_t stride, int64_t K, int64_t rows, const int32_t* end, uint8_t* codes, float* scales,
+                  hipStream_t stream);
   int (*gated_grad)(const float* gu, const void* dh, int64_t dh_stride, int64_t N, int64_t rows, int act, void* dgu,
                     hipStream_t stream);
 };
