@@ -125,7 +125,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile(Fp8TileArgs a) {
     auto load = [&](int k, int buf) {
       uint8_t* b = lds + buf * BUF;
       if (wave < BM / 64) xs_reg = xs[k * a.xs_stride];
-      p.load(pb, pbytes, a.x_stride, k, blocks * 128, 0, b, tid);
+      p.template load<false>(pb, pbytes, a.x_stride, k, blocks * 128, 0, b, tid);
       q.load(qb, qbytes, a.K, k, a.K, 0, b + P::BYTES, tid);
     };
     auto put = [&](int buf) {
@@ -146,56 +146,69 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile(Fp8TileArgs a) {
       for (int c = 0; c < 2; ++c) pf[to][c] = *(const u32x4_t*)(b + p_at + slot[c] + 16 * j * STEP_BYTES);
       sx[to] = *(const float*)(b + s_at + 64 * j);
     };
-    auto read_q = [&](int buf) {
+    auto read_q = [&](int buf, int i) {
 #pragma unroll
-      for (int i = 0; i < NF; ++i)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) qf[i][c] = *(const u32x4_t*)(lds + buf * BUF + q_at + slot[c] + 16 * i * STEP_BYTES);
+      for (int c = 0; c < 2; ++c) qf[i][c] = *(const u32x4_t*)(lds + buf * BUF + q_at + slot[c] + 16 * i * STEP_BYTES);
     };
     load(0, 0);
     put(0);
     __builtin_amdgcn_s_waitcnt(WAIT_ALL);
     block_barrier();
-    float sw = ws[0], sw_next = sw;
-    if (blocks > 1) load(1, 1), sw_next = ws[1];
-    read_q(0);
+    // loads past the last step read that one again, into the buffer that is free: the loop has no branches
+    const int end_k = blocks - 1;
+    float sw = ws[0], sw_next = ws[min(1, end_k)];
+    load(min(1, end_k), 1);
+#pragma unroll
+    for (int i = 0; i < NF; ++i) read_q(0, i);
     read_p(0, 0, 0);
+    // The products of 16 rows of x go to c[0] and c[1] in turn: while the matrix cores work on one, the other's are
+    // scaled and added, four instructions behind each of theirs. The asm keeps the compiler from moving that past
+    // the branches below, with every block's sums in registers till then. A c is read behind the four products of the other,
+    // which follow one another in the matrix cores' pipe, so it is there, past a branch too (see settle()).
+    f32x4_t c[2][NF] = {};
+    float s[2] = {0, 0};
+    auto products = [&](int j, auto between) {
+      const int cur = j & 1, prev = cur ^ 1, jp = (j + MF - 1) % MF;  // jp of the step before at first
+      s[cur] = sx[cur] * sw;
+#pragma unroll
+      for (int i = 0; i < NF; ++i) {
+        c[cur][i] = mma_block<EXACT>(qf[i], pf[cur]);
+        __builtin_amdgcn_sched_barrier(0);
+        between(i);
+        if (i > 0) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[i - 1][jp][r] = __builtin_fmaf(c[prev][i - 1][r], s[prev], acc[i - 1][jp][r]);
+          asm volatile("" : "+v"(acc[i - 1][jp]));
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[NF - 1][jp][r] = __builtin_fmaf(c[prev][NF - 1][r], s[prev], acc[NF - 1][jp][r]);
+      asm volatile("" : "+v"(acc[NF - 1][jp]));
+    };
     for (int k = 0; k < blocks; ++k) {
       const int buf = k & 1;
 #pragma unroll
-      for (int j = 0; j < MF; ++j) {
-        if (j + 1 < MF) {
-          read_p(buf, j + 1, (j + 1) & 1);
-        } else {
-          // the step's last rows are in registers, and its columns too: the buffer is free for step k + 2 once
-          // every wave is here, and step k + 1's loads, on their way since the last such place, have to be there
-          if (k + 1 < blocks) put(buf ^ 1);
-          __builtin_amdgcn_s_waitcnt(WAIT_ALL);
-          block_barrier();
-          if (k + 2 < blocks) load(k + 2, buf);
-        }
-        // scaled and added right behind the products (the asm keeps the compiler from moving that past the branches
-        // below, see settle(), with every block's sums in registers till then): the SIMD's other wave has the matrix cores
-        // meanwhile
-        const float s = sx[j & 1] * sw;
-        f32x4_t c[NF];
-#pragma unroll
-        for (int i = 0; i < NF; ++i) c[i] = mma_block<EXACT>(qf[i], pf[j & 1]);
-#pragma unroll
-        for (int i = 0; i < NF; ++i) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(c[i][r], s, acc[i][j][r]);
-          asm volatile("" : "+v"(acc[i][j]));
-        }
-        __builtin_amdgcn_sched_barrier(0);  // reads moved further ahead than one fragment cost more registers than there are
+      for (int j = 0; j + 1 < MF; ++j) {
+        read_p(buf, j + 1, (j + 1) & 1);
+        products(j, [](int) {});
       }
-      if (k + 1 < blocks) {
-        sw = sw_next;
-        if (k + 2 < blocks) sw_next = ws[k + 2];
-        read_q(buf ^ 1);
-        read_p(buf ^ 1, 0, 0);
-      }
+      // the step's last rows are in registers, and its columns too: the buffer is free for step k + 2 once
+      // every wave is here, and step k + 1's loads, on their way since the last such place, have to be there
+      put(buf ^ 1);
+      __builtin_amdgcn_s_waitcnt(WAIT_ALL);
+      block_barrier();
+      load(min(k + 2, end_k), buf);
+      products(MF - 1, [&](int i) { read_q(buf ^ 1, i); });
+      sw = sw_next;
+      sw_next = ws[min(k + 2, end_k)];
+      read_p(buf ^ 1, 0, 0);
     }
+    settle(c);
+#pragma unroll
+    for (int i = 0; i < NF; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[i][MF - 1][r] = __builtin_fmaf(c[1][i][r], s[1], acc[i][MF - 1][r]);
   }
 
   // fragment (i, j): the lane holds row 16 j + lane % 16 of x's, rows 4 (lane / 16) + r of w's

@@ -85,22 +85,23 @@ struct TileOperand {
   }
 
   // Loads step `step` of the k up to kend into dst (DIRECT) or registers. base: row 0, k = 0; bytes: from there
-  // to the operand's end; width: elements of a row in memory (TR). Chunks past kend become zeros.
+  // to the operand's end; width: elements of a row in memory (TR). Chunks past kend become zeros (ENDS: there are some).
+  template <bool ENDS = true>
   __device__ __forceinline__ void load(const uint8_t* base, int64_t bytes, int64_t stride, int step, int kend, int width,
                                        uint8_t* dst, int tid) {
     const int k0 = step * BK;
     if constexpr (DIRECT) {
       const int64_t at = TR ? (int64_t)k0 * stride : (int64_t)k0 * ES;
-      const int64_t left = bytes - at;
-      const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
-          (void*)(base + at), (short)0, (int)(left < 0x7fffffff ? left : 0x7fffffff), 0x00020000);
+      const uint64_t left = (uint64_t)(bytes - at);  // at most 2^31 - 1 of them, in scalar instructions
+      const uint32_t records = (uint32_t)(left >> 32) ? 0x7fffffffu : min((uint32_t)left, 0x7fffffffu);
+      const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(base + at), (short)0, (int)records, 0x00020000);
       const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
       const bool whole = k0 + BK <= kend;
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
         uint32_t o = off[j];
         // past the operand's end, where a buffer load gives zeros
-        if (!whole && k0 + first + (TR ? j * ROWS : 0) >= kend) o = 0x80000000u;
+        if (ENDS && !whole && k0 + first + (TR ? j * ROWS : 0) >= kend) o = 0x80000000u;
         __builtin_amdgcn_raw_ptr_buffer_load_lds(
             rsrc, (__attribute__((address_space(3))) void*)(dst + (j * THREADS + wave * 64) * 16), 16, (int)o, 0, 0, 0);
       }
@@ -305,11 +306,13 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void prod_tile(TileArgs a) {
         for (int i = 0; i < NF; ++i) acc[i][j] = T::mma32(qf[from][i], pf[from][j], acc[i][j]);
     };
     if (steps > 0) {
+      // loads past the last step read that one again, into the buffer that is free: the loop has no branches
+      const int last = steps - 1;
       load(0, 0);
       put(0);
       __builtin_amdgcn_s_waitcnt(WAIT_ALL);
       block_barrier();
-      if (steps > 1) load(1, 1);
+      load(min(1, last), 1);
       read(0, 0, 0);
       for (int k = 0; k < steps; ++k) {
         const int buf = k & 1;
@@ -320,13 +323,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void prod_tile(TileArgs a) {
         }
         // this step's last operands are in registers: its buffer is free for step k + 2 once every wave
         // is here, and step k + 1's loads, on their way since the last such place, have to be there
-        if (k + 1 < steps) put(buf ^ 1);
+        put(buf ^ 1);
         __builtin_amdgcn_s_waitcnt(WAIT_ALL);
         block_barrier();
-        if (k + 1 < steps) {
-          if (k + 2 < steps) load(k + 2, buf);
-          read(buf ^ 1, 0, 0);
-        }
+        load(min(k + 2, last), buf);
+        read(buf ^ 1, 0, 0);
         mma((SUBS - 1) & 1);
       }
       settle(acc);
