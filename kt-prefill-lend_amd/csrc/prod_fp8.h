@@ -89,7 +89,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile(Fp8TileArgs a) {
   constexpr int THREADS = 64 * WM * WN, BM = 16 * WM * MF, BN = 16 * WN * NF;
   using P = TileOperand<E4M3, false, true, BM, THREADS>;
   using Q = TileOperand<E4M3, false, DIRECT, BN, THREADS>;
-  constexpr int BUF = P::BYTES + Q::BYTES + BM * 4;
+  constexpr int BUF = P::BYTES + Q::BYTES + BM * 4 + 256;  // rows, their scales, those of the columns' blocks
+
   static_assert(BM % 64 == 0 && BM <= THREADS && 128 % (16 * NF) == 0 && BN % 128 == 0, "a wave's columns lie in one block");
   __shared__ __attribute__((aligned(16))) uint8_t lds[2 * BUF];
 
@@ -119,27 +120,33 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile(Fp8TileArgs a) {
     const int64_t qbytes = (int64_t)(a.N - pl.n0) * a.K;
     const int end = a.N - 1 - pl.n0;
     q.init(tid, a.K, 0, [&](int i) { return min(i, end); });
-    const float* ws = a.ws + ((int64_t)pl.expert * ((a.N + 127) / 128) + min(pl.n0 + 16 * NF * wn, a.N - 1) / 128) * blocks;
-    const float* xs = a.xs + sbase + (tid < BM ? row_of(tid) : 0);
-    float xs_reg = 0;
+    // The scales of a step go to LDS too: wave i < BM / 64 takes those of 64 rows, the next one those of the columns'
+    // blocks (by scalar loads, which count with the LDS reads, every step waited for them)
+    constexpr int SW = BM / 64;
+    static_assert(SW < WM * WN, "");
+    const int col_blocks = (a.N + 127) / 128;
+    const float* sp = wave < SW ? a.xs + sbase + row_of(tid)
+                                : a.ws + ((int64_t)pl.expert * col_blocks + min(pl.n0 / 128 + (lane & (BN / 128 - 1)), col_blocks - 1)) * blocks;
+    const int64_t sp_step = wave < SW ? a.xs_stride : 1;
+    float s_reg = 0;
     auto load = [&](int k, int buf) {
       uint8_t* b = lds + buf * BUF;
-      if (wave < BM / 64) xs_reg = xs[k * a.xs_stride];
+      if (wave <= SW) s_reg = gload<float>(sp + k * sp_step);
       p.template load<false>(pb, pbytes, a.x_stride, k, blocks * 128, 0, b, tid);
       q.load(qb, qbytes, a.K, k, a.K, 0, b + P::BYTES, tid);
     };
     auto put = [&](int buf) {
       uint8_t* b = lds + buf * BUF;
-      if (wave < BM / 64) *(float*)(b + P::BYTES + Q::BYTES + 4 * tid) = xs_reg;
+      if (wave <= SW) *(float*)(b + P::BYTES + Q::BYTES + 4 * tid) = s_reg;
       q.put(b + P::BYTES, tid);
     };
-    static_assert(MF % 2 == 0, "");
     u32x4_t pf[2][2], qf[NF][2];
     float sx[2];
     // a lane's chunks of fragment 0 of x's and w's rows (fragment j is 16 rows on, with the same slots), its scale
-    const int slot[2] = {16 * row_slot(l16, q4), 16 * row_slot(l16, 4 + q4)};
+    const int slot[2] = {16 * row_slot<1>(l16, q4), 16 * row_slot<1>(l16, 4 + q4)};
     const int p_at = (16 * MF * wm + l16) * STEP_BYTES, q_at = P::BYTES + (16 * NF * wn + l16) * STEP_BYTES;
     const int s_at = P::BYTES + Q::BYTES + 4 * (16 * MF * wm + l16);
+    const int sw_at = P::BYTES + Q::BYTES + 4 * BM + 4 * (16 * NF * wn / 128);
     auto read_p = [&](int buf, int j, int to) {
       const uint8_t* b = lds + buf * BUF;
 #pragma unroll
@@ -156,11 +163,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile(Fp8TileArgs a) {
     block_barrier();
     // loads past the last step read that one again, into the buffer that is free: the loop has no branches
     const int end_k = blocks - 1;
-    float sw = ws[0], sw_next = ws[min(1, end_k)];
     load(min(1, end_k), 1);
 #pragma unroll
     for (int i = 0; i < NF; ++i) read_q(0, i);
     read_p(0, 0, 0);
+    float sw = *(const float*)(lds + sw_at);
     // The products of 16 rows of x go to c[0] and c[1] in turn: while the matrix cores work on one, the other's are
     // scaled and added, four instructions behind each of theirs. The asm keeps the compiler from moving that past
     // the branches below, with every block's sums in registers till then. A c is read behind the four products of the other,
@@ -200,9 +207,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile(Fp8TileArgs a) {
       block_barrier();
       load(min(k + 2, end_k), buf);
       products(MF - 1, [&](int i) { read_q(buf ^ 1, i); });
-      sw = sw_next;
-      sw_next = ws[min(k + 2, end_k)];
       read_p(buf ^ 1, 0, 0);
+      sw = *(const float*)(lds + (buf ^ 1) * BUF + sw_at);
     }
     settle(c);
 #pragma unroll
