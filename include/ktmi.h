@@ -186,17 +186,17 @@ int ktmi_w4_kernel_of(int by, int x_dtype, int64_t cols, int64_t group, int64_t 
  * xs = f32(a / 448); a value that is not finite makes its row NaN. Sums in fp32, rounded once to x's type. Any cols and
  * rows (to 2^24), any alignment of the codes; rows of x that start at multiples of 16 bytes and cols that are multiples of 16 are
  * the fast case. No counterpart in the reference. */
-int64_t ktmi_fp8_linear_workspace(int64_t cols, int64_t tokens);
+int64_t ktmi_fp8_linear_workspace(int64_t rows, int64_t cols, int64_t tokens);
 int ktmi_fp8_linear(const void* x, int x_dtype, int64_t x_stride, int64_t cols, const void* w, const float* scales,
                     int64_t rows, int64_t tokens, void* y, void* workspace, int64_t ws_bytes, void* stream);
 /* by route: y[r] = W[ids[r]] x[r / top_k], y [tokens*top_k, rows]; ids outside [0, n_experts) give zero rows. */
-int64_t ktmi_moe_fp8_vec_workspace(int64_t cols, int64_t tokens, int64_t top_k, int64_t n_experts);
+int64_t ktmi_moe_fp8_vec_workspace(int64_t rows, int64_t cols, int64_t tokens, int64_t top_k, int64_t n_experts);
 int ktmi_moe_fp8_vec(const void* x, int x_dtype, int64_t x_stride, int64_t cols, const void* w, const float* scales,
                      int64_t rows, int64_t n_experts, const int32_t* ids, int64_t top_k, int64_t tokens, void* y,
                      void* workspace, int64_t ws_bytes, void* stream);
 /* rows sorted by expert (ktmi_moe_sort): y[p] = W[e] x[p] for offsets[e] <= p < offsets[e+1], y [n_rows, rows]; rows in
  * no segment give zero rows. offsets must ascend within [0, n_rows]; values outside are clamped to it. */
-int64_t ktmi_moe_fp8_sorted_workspace(int64_t cols, int64_t n_experts, int64_t n_rows);
+int64_t ktmi_moe_fp8_sorted_workspace(int64_t rows, int64_t cols, int64_t n_experts, int64_t n_rows);
 int ktmi_moe_fp8_sorted(const void* x, int x_dtype, int64_t x_stride, int64_t cols, const void* w, const float* scales,
                         int64_t rows, int64_t n_experts, const int32_t* offsets, int64_t n_rows, void* y, void* workspace,
                         int64_t ws_bytes, void* stream);
@@ -208,22 +208,29 @@ int ktmi_moe_fp8_sorted(const void* x, int x_dtype, int64_t x_stride, int64_t co
  * alignment; rows at multiples of 16 bytes are the fast case. No counterpart in the reference. */
 #define KTMI_ACT_SILU 0
 #define KTMI_ACT_GELU_TANH 1
+/* Workspace of a call (0: none is needed), for sums of a long k shared by several blocks. rows, cols: those of w (GATED: rows
+ * = inter). */
+enum { KTMI_PROD_GATED = 0, KTMI_PROD_LINEAR = 1, KTMI_PROD_GRAD_X = 2, KTMI_PROD_GRAD_W = 3 };
+int64_t ktmi_linear_workspace(int what, int dtype, int64_t rows, int64_t cols, int64_t n_experts, int64_t n_rows);
 /* h = act(x Wg^T) * (x Wu^T), w13 [n_experts, 2 inter, cols] = rows [gate; up], h [n_rows, inter]. sums fp32 [n_rows, 2 inter]
  * takes both projections before the activation, which the gradient needs (NULL: not kept). */
 int ktmi_gated(const void* x, int dtype, int64_t x_stride, int64_t cols, const void* w13, int64_t inter, int64_t n_experts,
-               const int32_t* offsets, int64_t n_rows, int act, void* h, float* sums, void* stream);
+               const int32_t* offsets, int64_t n_rows, int act, void* h, float* sums, void* workspace,
+               int64_t ws_bytes, void* stream);
 /* dsums [n_rows, 2 inter] = [dh * u * act'(g); dh * act(g)], of x's type, from sums = [g; u]: the dy of the two below. */
 int ktmi_gated_grad(const float* sums, const void* dh, int dtype, int64_t dh_stride, int64_t inter, int64_t n_rows, int act,
                     void* dsums, void* stream);
 /* y = x W^T, w [n_experts, rows, cols], y [n_rows, rows] */
 int ktmi_linear(const void* x, int dtype, int64_t x_stride, int64_t cols, const void* w, int64_t rows, int64_t n_experts,
-                const int32_t* offsets, int64_t n_rows, void* y, void* stream);
+                const int32_t* offsets, int64_t n_rows, void* y, void* workspace, int64_t ws_bytes, void* stream);
 /* dx = dy W [n_rows, cols], zeros for rows in no segment */
 int ktmi_linear_grad_x(const void* dy, int dtype, int64_t dy_stride, int64_t rows, const void* w, int64_t cols,
-                       int64_t n_experts, const int32_t* offsets, int64_t n_rows, void* dx, void* stream);
+                       int64_t n_experts, const int32_t* offsets, int64_t n_rows, void* dx, void* workspace, int64_t ws_bytes,
+                       void* stream);
 /* dw[e] = dy_e^T x_e over expert e's rows, [n_experts, rows, cols], zeros for an expert without rows */
 int ktmi_linear_grad_w(const void* dy, int dtype, int64_t dy_stride, int64_t rows, const void* x, int64_t x_stride,
-                       int64_t cols, int64_t n_experts, const int32_t* offsets, int64_t n_rows, void* dw, void* stream);
+                       int64_t cols, int64_t n_experts, const int32_t* offsets, int64_t n_rows, void* dw, void* workspace,
+                       int64_t ws_bytes, void* stream);
 
 /* ---- one hot-expert MoE layer -----------------------------------------------------
  * The GPU half of a layer: routes (t, k) with slot_ids[t*top_k+k] >= 0 run the expert in

@@ -15,6 +15,7 @@ LIB_PATH = Path(os.environ.get("KTMI_LIB", Path(__file__).resolve().parent / "li
 KTMI_OK = 0
 KTMI_F32, KTMI_F16, KTMI_BF16 = 0, 1, 2
 ACT_SILU, ACT_GELU_TANH = 0, 1
+PROD_GATED, PROD_LINEAR, PROD_GRAD_X, PROD_GRAD_W = 0, 1, 2, 3
 W4_DENSE, W4_IDS, W4_SORTED = 0, 1, 2
 MODE_AUTO, MODE_GEMV, MODE_GROUPED, MODE_DECODE = 0, 1, 2, 3
 STAGE_EVENTS = 6
@@ -83,17 +84,18 @@ SIGNATURES = {
                                _i64, _vp]),
     "ktmi_moe_w4_sorted": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _i32, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
     "ktmi_w4_kernel_of": (_i32, [_i32, _i32, _i64, _i64, _i64, _i64, _i64, C.POINTER(ktmi_w4_kernel)]),
-    "ktmi_fp8_linear_workspace": (_i64, [_i64, _i64]),
+    "ktmi_fp8_linear_workspace": (_i64, [_i64, _i64, _i64]),
     "ktmi_fp8_linear": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _vp]),
-    "ktmi_moe_fp8_vec_workspace": (_i64, [_i64, _i64, _i64, _i64]),
+    "ktmi_moe_fp8_vec_workspace": (_i64, [_i64, _i64, _i64, _i64, _i64]),
     "ktmi_moe_fp8_vec": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _vp]),
-    "ktmi_moe_fp8_sorted_workspace": (_i64, [_i64, _i64, _i64]),
+    "ktmi_moe_fp8_sorted_workspace": (_i64, [_i64, _i64, _i64, _i64]),
     "ktmi_moe_fp8_sorted": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp]),
-    "ktmi_gated": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i32, _vp, _vp, _vp]),
+    "ktmi_linear_workspace": (_i64, [_i32, _i32, _i64, _i64, _i64, _i64]),
+    "ktmi_gated": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i32, _vp, _vp, _vp, _i64, _vp]),
     "ktmi_gated_grad": (_i32, [_vp, _vp, _i32, _i64, _i64, _i64, _i32, _vp, _vp]),
-    "ktmi_linear": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _vp]),
-    "ktmi_linear_grad_x": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _vp]),
-    "ktmi_linear_grad_w": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
+    "ktmi_linear": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp]),
+    "ktmi_linear_grad_x": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp]),
+    "ktmi_linear_grad_w": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp]),
     "ktmi_moe_layer_workspace": (_i64, [C.POINTER(ktmi_layer), _i64, _i64, _i32]),
     "ktmi_moe_layer": (_i32, [C.POINTER(ktmi_layer), _vp, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _i32, _vp]),
     "ktmi_moe_layer_mode": (_i32, [C.POINTER(ktmi_layer), _i64, _i64]),

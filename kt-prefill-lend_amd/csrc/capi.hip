@@ -334,13 +334,13 @@ static int check_fp8(const char* what, const Fp8Args& a, int64_t need, int64_t w
   return KTMI_OK;
 }
 
-static bool fp8_shape(int64_t cols, int64_t rows, int64_t n_experts, int64_t top_k) {
-  return cols > 0 && cols <= (1 << 24) && rows > 0 && n_experts > 0 && n_experts <= SORT_MAX_EXPERTS && top_k > 0 &&
-         top_k <= 65535 && rows <= MAX_ROWS / top_k;
+static bool fp8_shape(int64_t rows, int64_t cols, int64_t x_rows, int64_t n_experts, int64_t top_k) {
+  return rows > 0 && rows <= (1 << 24) && cols > 0 && cols <= (1 << 24) && x_rows > 0 && n_experts > 0 && n_experts <= SORT_MAX_EXPERTS && top_k > 0 &&
+         top_k <= 65535 && x_rows <= MAX_ROWS / top_k;
 }
 
-int64_t ktmi_fp8_linear_workspace(int64_t cols, int64_t tokens) {
-  return fp8_shape(cols, tokens, 1, 1) ? fp8_workspace(cols, tokens, 1, 1, false) : 0;
+int64_t ktmi_fp8_linear_workspace(int64_t rows, int64_t cols, int64_t tokens) {
+  return fp8_shape(rows, cols, tokens, 1, 1) ? fp8_workspace(rows, cols, tokens, 1, 1, false) : 0;
 }
 
 int ktmi_fp8_linear(const void* x, int x_dtype, int64_t x_stride, int64_t cols, const void* w, const float* scales,
@@ -348,12 +348,12 @@ int ktmi_fp8_linear(const void* x, int x_dtype, int64_t x_stride, int64_t cols, 
   g_err[0] = 0;
   const Fp8Args a = {x_dtype, x, x_stride, tokens, (const uint8_t*)w, scales, rows, cols, 1, nullptr, 1, nullptr, y,
                      (uint8_t*)workspace};
-  int rc = check_fp8("fp8_linear", a, ktmi_fp8_linear_workspace(cols, tokens), ws_bytes);
+  int rc = check_fp8("fp8_linear", a, ktmi_fp8_linear_workspace(rows, cols, tokens), ws_bytes);
   return rc || tokens == 0 ? rc : launch_fp8(a, (hipStream_t)stream);
 }
 
-int64_t ktmi_moe_fp8_vec_workspace(int64_t cols, int64_t tokens, int64_t top_k, int64_t n_experts) {
-  return fp8_shape(cols, tokens, n_experts, top_k) ? fp8_workspace(cols, tokens, n_experts, top_k, true) : 0;
+int64_t ktmi_moe_fp8_vec_workspace(int64_t rows, int64_t cols, int64_t tokens, int64_t top_k, int64_t n_experts) {
+  return fp8_shape(rows, cols, tokens, n_experts, top_k) ? fp8_workspace(rows, cols, tokens, n_experts, top_k, true) : 0;
 }
 
 int ktmi_moe_fp8_vec(const void* x, int x_dtype, int64_t x_stride, int64_t cols, const void* w, const float* scales,
@@ -362,14 +362,14 @@ int ktmi_moe_fp8_vec(const void* x, int x_dtype, int64_t x_stride, int64_t cols,
   g_err[0] = 0;
   const Fp8Args a = {x_dtype, x, x_stride, tokens, (const uint8_t*)w, scales, rows, cols, n_experts, ids, top_k, nullptr, y,
                      (uint8_t*)workspace};
-  int rc = check_fp8("moe_fp8_vec", a, ktmi_moe_fp8_vec_workspace(cols, tokens, top_k, n_experts), ws_bytes);
+  int rc = check_fp8("moe_fp8_vec", a, ktmi_moe_fp8_vec_workspace(rows, cols, tokens, top_k, n_experts), ws_bytes);
   if (rc || tokens == 0) return rc;
   KTMI_REQUIRE(ids, KTMI_EINVAL, "moe_fp8_vec: null pointer");
   return launch_fp8(a, (hipStream_t)stream);
 }
 
-int64_t ktmi_moe_fp8_sorted_workspace(int64_t cols, int64_t n_experts, int64_t n_rows) {
-  return fp8_shape(cols, n_rows, n_experts, 1) ? fp8_workspace(cols, n_rows, n_experts, 1, false) : 0;
+int64_t ktmi_moe_fp8_sorted_workspace(int64_t rows, int64_t cols, int64_t n_experts, int64_t n_rows) {
+  return fp8_shape(rows, cols, n_rows, n_experts, 1) ? fp8_workspace(rows, cols, n_rows, n_experts, 1, false) : 0;
 }
 
 int ktmi_moe_fp8_sorted(const void* x, int x_dtype, int64_t x_stride, int64_t cols, const void* w, const float* scales,
@@ -378,7 +378,7 @@ int ktmi_moe_fp8_sorted(const void* x, int x_dtype, int64_t x_stride, int64_t co
   g_err[0] = 0;
   const Fp8Args a = {x_dtype, x, x_stride, n_rows, (const uint8_t*)w, scales, rows, cols, n_experts, nullptr, 1, offsets, y,
                      (uint8_t*)workspace};
-  int rc = check_fp8("moe_fp8_sorted", a, ktmi_moe_fp8_sorted_workspace(cols, n_experts, n_rows), ws_bytes);
+  int rc = check_fp8("moe_fp8_sorted", a, ktmi_moe_fp8_sorted_workspace(rows, cols, n_experts, n_rows), ws_bytes);
   if (rc || n_rows == 0) return rc;
   KTMI_REQUIRE(offsets, KTMI_EINVAL, "moe_fp8_sorted: null pointer");
   return launch_fp8(a, (hipStream_t)stream);
@@ -406,28 +406,45 @@ static int check_stride(const char* what, const char* name, int64_t stride, int6
   return KTMI_OK;
 }
 
+int64_t ktmi_linear_workspace(int what, int dtype, int64_t rows, int64_t cols, int64_t n_experts, int64_t n_rows) {
+  if (what < KTMI_PROD_GATED || what > KTMI_PROD_GRAD_W || !dtype_ok(dtype) || rows <= 0 || rows > (1 << 24) || cols <= 0 ||
+      cols > (1 << 24) || n_experts <= 0 || n_experts > SORT_MAX_EXPERTS || n_rows <= 0 || n_rows > MAX_ROWS)
+    return 0;
+  return prod_workspace(what, dtype, rows, cols, n_experts, n_rows);
+}
+
+// the call's workspace is there; then it runs
+static int run_prod(const char* name, int what, const ProdArgs& a, int64_t ws_bytes, void* stream) {
+  const int64_t need = ktmi_linear_workspace(what, a.dtype, a.rows, a.cols, a.n_experts, a.n_rows);
+  KTMI_REQUIRE(need == 0 || (a.part && ws_bytes >= need && aligned(a.part, 16)), KTMI_ESPACE,
+               "%s: workspace %lld < %lld bytes, or not aligned to 16", name, (long long)ws_bytes, (long long)need);
+  return launch_prod(what, a, (hipStream_t)stream);
+}
+
 static int check_act(const char* what, int act) {
   KTMI_REQUIRE(act == KTMI_ACT_SILU || act == KTMI_ACT_GELU_TANH, KTMI_EINVAL, "%s: act %d", what, act);
   return KTMI_OK;
 }
 
 int ktmi_gated(const void* x, int dtype, int64_t x_stride, int64_t cols, const void* w13, int64_t inter, int64_t n_experts,
-               const int32_t* offsets, int64_t n_rows, int act, void* h, float* sums, void* stream) {
+               const int32_t* offsets, int64_t n_rows, int act, void* h, float* sums, void* workspace, int64_t ws_bytes,
+               void* stream) {
   g_err[0] = 0;
-  const ProdArgs a = {dtype, x, x_stride, nullptr, 0, w13, inter, cols, n_experts, offsets, n_rows, act, h, sums};
+  const ProdArgs a = {dtype, x, x_stride, nullptr, 0, w13, inter, cols, n_experts, offsets, n_rows, act, h, sums, (float*)workspace};
   int rc = check_prod("gated", a);
   if (!rc) rc = check_act("gated", act);
   if (!rc) rc = check_stride("gated", "x_stride", x_stride, cols, n_rows);
   KTMI_REQUIRE(rc || inter <= (1 << 23), KTMI_EINVAL, "gated: inter %lld (at most 2^23)", (long long)inter);
   if (rc || n_rows == 0) return rc;
   KTMI_REQUIRE(x && w13 && h, KTMI_EINVAL, "gated: null pointer");
-  return launch_prod_fwd(a, true, (hipStream_t)stream);
+  return run_prod("gated", KTMI_PROD_GATED, a, ws_bytes, stream);
 }
 
 int ktmi_gated_grad(const float* sums, const void* dh, int dtype, int64_t dh_stride, int64_t inter, int64_t n_rows, int act,
                     void* dsums, void* stream) {
   g_err[0] = 0;
-  const ProdArgs a = {dtype, nullptr, 0, dh, dh_stride, nullptr, inter, 1, 1, nullptr, n_rows, act, dsums, (float*)sums};
+  const ProdArgs a = {dtype, nullptr, 0, dh, dh_stride, nullptr, inter, 1, 1, nullptr, n_rows, act, dsums, (float*)sums,
+                      nullptr};
   int rc = check_prod("gated_grad", a);
   if (!rc) rc = check_act("gated_grad", act);
   if (!rc) rc = check_stride("gated_grad", "dh_stride", dh_stride, inter, n_rows);
@@ -438,37 +455,42 @@ int ktmi_gated_grad(const float* sums, const void* dh, int dtype, int64_t dh_str
 }
 
 int ktmi_linear(const void* x, int dtype, int64_t x_stride, int64_t cols, const void* w, int64_t rows, int64_t n_experts,
-                const int32_t* offsets, int64_t n_rows, void* y, void* stream) {
+                const int32_t* offsets, int64_t n_rows, void* y, void* workspace, int64_t ws_bytes, void* stream) {
   g_err[0] = 0;
-  const ProdArgs a = {dtype, x, x_stride, nullptr, 0, w, rows, cols, n_experts, offsets, n_rows, 0, y, nullptr};
+  const ProdArgs a = {dtype, x, x_stride, nullptr, 0, w, rows, cols, n_experts, offsets, n_rows, 0, y, nullptr,
+                      (float*)workspace};
   int rc = check_prod("linear", a);
   if (!rc) rc = check_stride("linear", "x_stride", x_stride, cols, n_rows);
   if (rc || n_rows == 0) return rc;
   KTMI_REQUIRE(x && w && y, KTMI_EINVAL, "linear: null pointer");
-  return launch_prod_fwd(a, false, (hipStream_t)stream);
+  return run_prod("linear", KTMI_PROD_LINEAR, a, ws_bytes, stream);
 }
 
 int ktmi_linear_grad_x(const void* dy, int dtype, int64_t dy_stride, int64_t rows, const void* w, int64_t cols,
-                       int64_t n_experts, const int32_t* offsets, int64_t n_rows, void* dx, void* stream) {
+                       int64_t n_experts, const int32_t* offsets, int64_t n_rows, void* dx, void* workspace, int64_t ws_bytes,
+                       void* stream) {
   g_err[0] = 0;
-  const ProdArgs a = {dtype, nullptr, 0, dy, dy_stride, w, rows, cols, n_experts, offsets, n_rows, 0, dx, nullptr};
+  const ProdArgs a = {dtype, nullptr, 0, dy, dy_stride, w, rows, cols, n_experts, offsets, n_rows, 0, dx, nullptr,
+                      (float*)workspace};
   int rc = check_prod("linear_grad_x", a);
   if (!rc) rc = check_stride("linear_grad_x", "dy_stride", dy_stride, rows, n_rows);
   if (rc || n_rows == 0) return rc;
   KTMI_REQUIRE(dy && w && dx, KTMI_EINVAL, "linear_grad_x: null pointer");
-  return launch_prod_dx(a, (hipStream_t)stream);
+  return run_prod("linear_grad_x", KTMI_PROD_GRAD_X, a, ws_bytes, stream);
 }
 
 int ktmi_linear_grad_w(const void* dy, int dtype, int64_t dy_stride, int64_t rows, const void* x, int64_t x_stride,
-                       int64_t cols, int64_t n_experts, const int32_t* offsets, int64_t n_rows, void* dw, void* stream) {
+                       int64_t cols, int64_t n_experts, const int32_t* offsets, int64_t n_rows, void* dw, void* workspace,
+                       int64_t ws_bytes, void* stream) {
   g_err[0] = 0;
-  const ProdArgs a = {dtype, x, x_stride, dy, dy_stride, nullptr, rows, cols, n_experts, offsets, n_rows, 0, dw, nullptr};
+  const ProdArgs a = {dtype, x, x_stride, dy, dy_stride, nullptr, rows, cols, n_experts, offsets, n_rows, 0, dw, nullptr,
+                      (float*)workspace};
   int rc = check_prod("linear_grad_w", a);
   if (!rc) rc = check_stride("linear_grad_w", "dy_stride", dy_stride, rows, n_rows);
   if (!rc) rc = check_stride("linear_grad_w", "x_stride", x_stride, cols, n_rows);
   if (rc) return rc;
   KTMI_REQUIRE(dw && (n_rows == 0 || (dy && x)), KTMI_EINVAL, "linear_grad_w: null pointer");
-  return launch_prod_dw(a, (hipStream_t)stream);
+  return run_prod("linear_grad_w", KTMI_PROD_GRAD_W, a, ws_bytes, stream);
 }
 
 // ---- scratch for ktmi_moe_layer_noalloc

@@ -70,10 +70,10 @@ struct ProdArgs {
   int act;
   void* y;
   float* sums;
+  float* part;  // workspace
 };
-int launch_prod_fwd(const ProdArgs& a, bool gated, hipStream_t stream);
-int launch_prod_dx(const ProdArgs& a, hipStream_t stream);
-int launch_prod_dw(const ProdArgs& a, hipStream_t stream);
+int64_t prod_workspace(int what, int dtype, int64_t rows, int64_t cols, int64_t n_experts, int64_t n_rows);
+int launch_prod(int what, const ProdArgs& a, hipStream_t stream);
 int launch_gated_grad(const float* sums, const void* dh, int dtype, int64_t dh_stride, int64_t inter, int64_t n_rows, int act,
                       void* dsums, hipStream_t stream);
 // Products in 8-bit floating point: x [x_rows, cols] by e4m3 matrices with a scale for each block of 128 x 128; route r's
@@ -91,7 +91,7 @@ struct Fp8Args {
   void* y;
   uint8_t* ws;
 };
-int64_t fp8_workspace(int64_t cols, int64_t x_rows, int64_t n_experts, int64_t top_k, bool ids);
+int64_t fp8_workspace(int64_t rows, int64_t cols, int64_t x_rows, int64_t n_experts, int64_t top_k, bool ids);
 int launch_fp8(const Fp8Args& a, hipStream_t stream);
 
 // GEMV over raw GGUF rows against q8_1 activations (the decode-window kernel).

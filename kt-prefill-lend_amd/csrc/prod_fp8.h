@@ -82,6 +82,9 @@ struct Fp8TileArgs {
   Segments seg;             // offsets NULL: one matrix for all rows
   const int32_t* perm;      // sorted routes: row p's codes are row perm[p] / top_k, its place in y perm[p] (its
   int top_k;                // complement without an expert); NULL: row p
+  int splits;               // as TileArgs'
+  float* part;
+  int64_t slice;
 };
 
 template <typename S, bool EXACT, bool DIRECT, int WM, int WN, int MF, int NF>
@@ -96,14 +99,15 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile(Fp8TileArgs a) {
 
   Place pl;
   TileArgs t = {};
-  t.M = a.M, t.N = a.N, t.seg = a.seg;
+  t.M = a.M, t.N = a.N, t.seg = a.seg, t.splits = a.splits;
   if (!place_of<PROD_FWD, BM, BN>(t, pl)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave % WM, wn = wave / WM, l16 = lane & 15, q4 = lane >> 4;
   const int blocks = (a.K + 127) / 128;
 
   f32x4_t acc[NF][MF] = {};
-  if (pl.expert >= 0) {
+  const int share = (blocks + a.splits - 1) / a.splits, begin = pl.split * share, end_k = min(blocks, begin + share) - 1;
+  if (pl.expert >= 0 && begin <= end_k) {
     const int last = pl.rows - 1;
     const uint8_t* pb = a.x;
     int64_t pbytes = a.x_rows * a.x_stride;
@@ -133,7 +137,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile(Fp8TileArgs a) {
       uint8_t* b = lds + buf * BUF;
       if (wave <= SW) s_reg = gload<float>(sp + k * sp_step);
       p.template load<false>(pb, pbytes, a.x_stride, k, blocks * 128, 0, b, tid);
-      q.load(qb, qbytes, a.K, k, a.K, 0, b + P::BYTES, tid);
+      q.template load<true>(qb, qbytes, a.K, k, a.K, 0, b + P::BYTES, tid);
     };
     auto put = [&](int buf) {
       uint8_t* b = lds + buf * BUF;
@@ -157,13 +161,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile(Fp8TileArgs a) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) qf[i][c] = *(const u32x4_t*)(lds + buf * BUF + q_at + slot[c] + 16 * i * STEP_BYTES);
     };
-    load(0, 0);
+    load(begin, 0);
     put(0);
     __builtin_amdgcn_s_waitcnt(WAIT_ALL);
     block_barrier();
     // loads past the last step read that one again, into the buffer that is free: the loop has no branches
-    const int end_k = blocks - 1;
-    load(min(1, end_k), 1);
+    load(min(begin + 1, end_k), 1);
 #pragma unroll
     for (int i = 0; i < NF; ++i) read_q(0, i);
     read_p(0, 0, 0);
@@ -193,8 +196,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile(Fp8TileArgs a) {
       for (int r = 0; r < 4; ++r) acc[NF - 1][jp][r] = __builtin_fmaf(c[prev][NF - 1][r], s[prev], acc[NF - 1][jp][r]);
       asm volatile("" : "+v"(acc[NF - 1][jp]));
     };
-    for (int k = 0; k < blocks; ++k) {
-      const int buf = k & 1;
+    for (int k = begin; k <= end_k; ++k) {
+      const int buf = (k - begin) & 1;
 #pragma unroll
       for (int j = 0; j + 1 < MF; ++j) {
         read_p(buf, j + 1, (j + 1) & 1);
@@ -218,19 +221,26 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile(Fp8TileArgs a) {
   }
 
   // fragment (i, j): the lane holds row 16 j + lane % 16 of x's, rows 4 (lane / 16) + r of w's
-  const bool vec = a.N % 4 == 0 && (uintptr_t)a.y % (4 * sizeof(S)) == 0;
+  const int n0 = pl.n0 + 16 * NF * wn;
+  auto place = [&](int m) {
+    const int p = pl.m0 + m;
+    return a.perm ? (pl.expert >= 0 ? a.perm[p] : ~a.perm[p]) : p;
+  };
+  const bool wide = ((uintptr_t)a.y | (a.N * sizeof(S))) % 16 == 0;
+  __builtin_amdgcn_s_waitcnt(WAIT_ALL);  // the last steps' loads, into the buffers that the waves stage their rows in
+  block_barrier();
+  uint8_t* stage = lds + wave * STAGE_BYTES;
 #pragma unroll
   for (int j = 0; j < MF; ++j) {
-    const int m = 16 * (MF * wm + j) + l16;
-    if (m >= pl.rows) continue;
-    int at = pl.m0 + m;
-    if (a.perm) at = pl.expert >= 0 ? a.perm[at] : ~a.perm[at];
-    S* row = (S*)a.y + (int64_t)at * a.N;
-#pragma unroll
-    for (int i = 0; i < NF; ++i) {
-      const int n = pl.n0 + 16 * (NF * wn + i) + 4 * q4;
-      if (n < a.N) store4(row, n, a.N, vec, acc[i][j]);
+    const int m = 16 * (MF * wm + j);
+    if (m >= pl.rows) break;
+    if (a.splits > 1) {  // (its rows in the order of y already)
+      store_rows<float, 16, NF>(stage, [&](int i, int r) { return acc[i][j][r]; }, a.part + pl.split * a.slice + n0,
+                                [&](int i) { return (int64_t)place(m + i) * a.N; }, pl.rows - m, a.N - n0, a.N % 4 == 0, lane);
+      continue;
     }
+    store_rows<S, 16, NF>(stage, [&](int i, int r) { return acc[i][j][r]; }, (S*)a.y + n0,
+                          [&](int i) { return (int64_t)place(m + i) * a.N; }, pl.rows - m, a.N - n0, wide, lane);
   }
 }
 

@@ -4,38 +4,91 @@
 
 namespace ktmi {
 
-// Tiles of 256 x 256 by 8 waves, or 128 x 128 by 4, of which two share a CU.
-template <typename T, int MODE, bool GATED, bool DIRECT, bool LARGE>
+template <typename T, int MODE, bool GATED, bool DIRECT, bool TAIL, int SIZE>
 int launch_tile_of(const TileArgs& a, hipStream_t stream) {
-  constexpr int BM = LARGE ? 256 : 128, BN = (LARGE ? 256 : 128) / (GATED ? 2 : 1), THREADS = LARGE ? 512 : 256;
+  constexpr bool FOUR = SIZE == TILE_SMALL || SIZE == TILE_LOW;  // waves
+  constexpr int BM = tile_m(SIZE), BN = tile_n(SIZE) / (GATED ? 2 : 1), THREADS = FOUR ? 256 : 512;
   const int64_t nt = (a.N + BN - 1) / BN;
   int64_t mt = (a.M + BM - 1) / BM;
   if (a.seg.offsets) mt = MODE == PROD_DW ? mt * a.seg.E : a.M / BM + a.seg.E + 2;
-  const int64_t grid = (mt * nt + 7) / 8 * 8;
+  const int64_t grid = (mt * nt * a.splits + 7) / 8 * 8;
   KTMI_REQUIRE(grid < (int64_t)0xffffffff / THREADS, KTMI_EINVAL, "a grid of %lld blocks (below 2^32 threads)", (long long)grid);
-  if constexpr (LARGE) prod_tile<T, MODE, GATED, DIRECT, 2, 4, 4, 2><<<(unsigned)grid, THREADS, 0, stream>>>(a);
-  else prod_tile<T, MODE, GATED, DIRECT, 2, 2, 2, 2><<<(unsigned)grid, THREADS, 0, stream>>>(a);
+  if constexpr (SIZE == TILE_LARGE) prod_tile<T, MODE, GATED, DIRECT, TAIL, 2, 4, 4, 2, 2><<<(unsigned)grid, THREADS, 0, stream>>>(a);
+  else if constexpr (SIZE == TILE_DEEP) prod_tile<T, MODE, GATED, DIRECT, TAIL, 2, 4, 2, 2, 3><<<(unsigned)grid, THREADS, 0, stream>>>(a);
+  else if constexpr (SIZE == TILE_LOW) prod_tile<T, MODE, GATED, DIRECT, TAIL, 2, 2, 1, 2, 2><<<(unsigned)grid, THREADS, 0, stream>>>(a);
+  else prod_tile<T, MODE, GATED, DIRECT, TAIL, 2, 2, 2, 2, 2><<<(unsigned)grid, THREADS, 0, stream>>>(a);
   KTMI_HIP_TRY(hipGetLastError());
   return KTMI_OK;
 }
 
-// Rows at multiples of 16 bytes, whose tiles 32-bit offsets reach.
+// Rows at multiples of 4 bytes, whose tiles 32-bit offsets reach.
 inline bool rows_direct(const void* p, int64_t stride, int64_t span) {
-  return ((uintptr_t)p | (uintptr_t)stride) % 16 == 0 && span * stride < 0x7fffffff;
+  return ((uintptr_t)p | (uintptr_t)stride) % 4 == 0 && span * stride < 0x7fffffff;
 }
 
 template <typename T, int MODE, bool GATED>
-int launch_tile(const TileArgs& a, hipStream_t stream) {
+int launch_tile(const TileArgs& a, int size, hipStream_t stream) {
   const int64_t wide = MODE == PROD_FWD && GATED ? 2 * (int64_t)a.N : 256;
-  // k past the operands' ends comes in whole chunks where it runs along the rows; across them rows end anywhere
-  const bool ends = MODE == PROD_DW || a.K % T::EPC == 0;
-  const bool direct = ends && rows_direct(a.p, a.p_stride, 256) && rows_direct(a.q, a.q_stride, wide) && a.q_expert % 16 == 0;
-  if (!direct) return launch_tile_of<T, MODE, GATED, false, false>(a, stream);
-  const int64_t parts = a.seg.offsets ? a.seg.E : 1;
-  const int64_t m = MODE == PROD_DW ? a.M : a.M / parts;
-  const int64_t tiles = (m + 255) / 256 * ((a.N * (GATED ? 2 : 1) + 255) / 256) * parts;
-  if (m >= 192 && tiles >= 192) return launch_tile_of<T, MODE, GATED, true, true>(a, stream);
-  return launch_tile_of<T, MODE, GATED, true, false>(a, stream);
+  const bool direct = rows_direct(a.p, a.p_stride, 256) && rows_direct(a.q, a.q_stride, wide) && a.q_expert % 4 == 0;
+  if constexpr (MODE != PROD_DW) {
+    if (direct && a.K % (STEP_BYTES / T::ES)) {
+      if (size == TILE_LOW) return launch_tile_of<T, MODE, GATED, true, true, TILE_LOW>(a, stream);
+      if (size == TILE_LARGE) return launch_tile_of<T, MODE, GATED, true, true, TILE_LARGE>(a, stream);
+      return launch_tile_of<T, MODE, GATED, true, true, TILE_SMALL>(a, stream);
+    }
+    if (size == TILE_LOW)
+      return direct ? launch_tile_of<T, MODE, GATED, true, false, TILE_LOW>(a, stream)
+                    : launch_tile_of<T, MODE, GATED, false, false, TILE_LOW>(a, stream);
+  }
+  if (!direct) return launch_tile_of<T, MODE, GATED, false, false, TILE_SMALL>(a, stream);
+  if constexpr (MODE == PROD_FWD) {
+    if (size == TILE_DEEP) return launch_tile_of<T, MODE, GATED, true, false, TILE_DEEP>(a, stream);
+  }
+  if (size == TILE_LARGE) return launch_tile_of<T, MODE, GATED, true, false, TILE_LARGE>(a, stream);
+  return launch_tile_of<T, MODE, GATED, true, false, TILE_SMALL>(a, stream);
+}
+
+// ---- the sums of a tile's k shared by `splits` blocks, in the blocks' order: four values a thread where rows
+// hold multiples of four (VEC), else one. gated: rows [g; u] of 2 N, h = act(g) u.
+template <typename T, bool GATED, bool VEC>
+__global__ __launch_bounds__(256) void sum_parts(const float* part, int splits, int64_t slice, int64_t rows, int N, int act,
+                                                 uint8_t* out, float* gu) {
+  using S = typename T::S;
+  constexpr int V = VEC ? 4 : 1;
+  const int64_t n = N / V, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows * n) return;
+  const int64_t row = i / n, col = (i - row * n) * V;
+  const float* p = part + row * (GATED ? 2 : 1) * N + col;
+  float g[V] = {}, u[V] = {};
+  for (int s = 0; s < splits; ++s, p += slice) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      g[v] += p[v];
+      if constexpr (GATED) u[v] += p[N + v];
+    }
+  }
+  S* o = (S*)out + row * N + col;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    if constexpr (GATED) {
+      o[v] = (S)(act_of(act, g[v]) * u[v]);
+      if (gu) gu[row * 2 * N + col + v] = g[v], gu[row * 2 * N + N + col + v] = u[v];
+    } else {
+      o[v] = (S)g[v];
+    }
+  }
+}
+
+template <typename T, bool GATED>
+int launch_sum_parts(const float* part, int splits, int64_t slice, int64_t rows, int64_t N, int act, void* out, float* gu,
+                     hipStream_t stream) {
+  const bool vec = N % 4 == 0;
+  const int64_t grid = (rows * (vec ? N / 4 : N) + 255) / 256;
+  KTMI_REQUIRE(grid < (int64_t)0xffffffff / 256, KTMI_EINVAL, "a grid of %lld blocks (below 2^32 threads)", (long long)grid);
+  if (vec) sum_parts<T, GATED, true><<<(unsigned)grid, 256, 0, stream>>>(part, splits, slice, rows, (int)N, act, (uint8_t*)out, gu);
+  else sum_parts<T, GATED, false><<<(unsigned)grid, 256, 0, stream>>>(part, splits, slice, rows, (int)N, act, (uint8_t*)out, gu);
+  KTMI_HIP_TRY(hipGetLastError());
+  return KTMI_OK;
 }
 
 template <typename X, bool FP8, bool GATED, int CT, int NRF, int WK>
@@ -53,46 +106,48 @@ int launch_rows_of(RowsArgs a, hipStream_t stream) {
   return KTMI_OK;
 }
 
-// mean: rows of a matrix. Rows of w a wave: 16 where more would leave CUs without a block, else 64 (32 against 64 rows of
+// mean: rows of a matrix. Rows of w a wave: 16 where more would leave CUs without a block, else 64 (32 against 32 rows of
 // x), which share the rows of x and, of e4m3, their quantisation. Rows of w below 16 units are too short for eight
 // waves: two share one.
 template <typename X, bool FP8, bool GATED>
 int launch_rows(const RowsArgs& a, int mean, hipStream_t stream) {
   constexpr int UE = 128 / (FP8 ? 1 : X::ES);
   const bool shorter = a.K < 16 * UE;
-  const int64_t cols = mean <= 16 ? 16 : mean <= 32 ? 32 : 64;
+  const int64_t cols = mean <= 16 ? 16 : 32;
   const int64_t parts = a.ids || a.seg.offsets ? min((int64_t)a.seg.E, (int64_t)a.R) : (a.R + cols - 1) / cols;
   const int64_t frags = parts * (GATED ? 2 : 1) * a.N / 16;
   if (cols == 16) {
     if (frags < 4 * 512) return launch_rows_of<X, FP8, GATED, 1, 1, 8>(a, stream);
     return shorter ? launch_rows_of<X, FP8, GATED, 1, 2, 2>(a, stream) : launch_rows_of<X, FP8, GATED, 1, 4, 8>(a, stream);
   }
-  if (cols == 32) {
-    if (frags < 4 * 512) return launch_rows_of<X, FP8, GATED, 2, 1, 8>(a, stream);
-    return shorter ? launch_rows_of<X, FP8, GATED, 2, 2, 2>(a, stream) : launch_rows_of<X, FP8, GATED, 2, 2, 8>(a, stream);
-  }
-  return shorter ? launch_rows_of<X, FP8, GATED, 4, 2, 2>(a, stream) : launch_rows_of<X, FP8, GATED, 4, 2, 8>(a, stream);
+  if (frags < 4 * 512) return launch_rows_of<X, FP8, GATED, 2, 1, 8>(a, stream);
+  return shorter ? launch_rows_of<X, FP8, GATED, 2, 2, 2>(a, stream) : launch_rows_of<X, FP8, GATED, 2, 2, 8>(a, stream);
+}
+
+template <typename S, bool EXACT, bool DIRECT, int SIZE>
+int launch_fp8_tile_of(const Fp8TileArgs& a, hipStream_t stream) {
+  constexpr int BM = tile_m(SIZE), BN = tile_n(SIZE), THREADS = SIZE == TILE_LARGE ? 512 : 256;
+  const int64_t mt = a.seg.offsets ? a.M / BM + a.seg.E + 2 : (a.M + BM - 1) / BM;
+  const int64_t grid = (mt * ((a.N + BN - 1) / BN) * a.splits + 7) / 8 * 8;
+  KTMI_REQUIRE(grid < (int64_t)0xffffffff / THREADS, KTMI_EINVAL, "a grid of %lld blocks (below 2^32 threads)", (long long)grid);
+  if constexpr (SIZE == TILE_LARGE) fp8_tile<S, EXACT, DIRECT, 2, 4, 8, 4><<<(unsigned)grid, THREADS, 0, stream>>>(a);
+  else if constexpr (SIZE == TILE_LOW) fp8_tile<S, EXACT, DIRECT, 2, 2, 2, 4><<<(unsigned)grid, THREADS, 0, stream>>>(a);
+  else fp8_tile<S, EXACT, DIRECT, 2, 2, 4, 4><<<(unsigned)grid, THREADS, 0, stream>>>(a);
+  KTMI_HIP_TRY(hipGetLastError());
+  return KTMI_OK;
 }
 
 template <typename X>
-int launch_fp8_tile(const Fp8TileArgs& a, hipStream_t stream) {
+int launch_fp8_tile(const Fp8TileArgs& a, int size, hipStream_t stream) {
   using S = typename X::S;
   constexpr bool EXACT = std::is_same<X, F32>::value;
-  const bool direct = rows_direct(a.w, a.K, 256);
-  const int64_t mean = a.seg.offsets ? a.M / a.seg.E : a.M;
-  const bool large = direct && !EXACT && mean >= 192 && (mean + 255) / 256 * ((a.N + 255) / 256) * (a.seg.offsets ? a.seg.E : 1) >= 192;
-  const int64_t bm = large ? 256 : 128, bn = large ? 256 : 128, threads = large ? 512 : 256;
-  const int64_t mt = a.seg.offsets ? a.M / bm + a.seg.E + 2 : (a.M + bm - 1) / bm;
-  const int64_t grid = (mt * ((a.N + bn - 1) / bn) + 7) / 8 * 8;
-  KTMI_REQUIRE(grid < (int64_t)0xffffffff / threads, KTMI_EINVAL, "a grid of %lld blocks (below 2^32 threads)", (long long)grid);
-  if constexpr (!EXACT) {
-    if (large) fp8_tile<S, EXACT, true, 2, 4, 8, 4><<<(unsigned)grid, 512, 0, stream>>>(a);
+  const bool direct = a.K % 16 == 0 && rows_direct(a.w, a.K, 256);
+  if (size == TILE_LOW)
+    return direct ? launch_fp8_tile_of<S, EXACT, true, TILE_LOW>(a, stream) : launch_fp8_tile_of<S, EXACT, false, TILE_LOW>(a, stream);
+  if constexpr (!EXACT) {  // (whose operands as bf16 leave no registers for 256 rows)
+    if (direct && size == TILE_LARGE) return launch_fp8_tile_of<S, EXACT, true, TILE_LARGE>(a, stream);
   }
-  if (large) ;
-  else if (direct) fp8_tile<S, EXACT, true, 2, 2, 4, 4><<<(unsigned)grid, 256, 0, stream>>>(a);
-  else fp8_tile<S, EXACT, false, 2, 2, 4, 4><<<(unsigned)grid, 256, 0, stream>>>(a);
-  KTMI_HIP_TRY(hipGetLastError());
-  return KTMI_OK;
+  return direct ? launch_fp8_tile_of<S, EXACT, true, TILE_SMALL>(a, stream) : launch_fp8_tile_of<S, EXACT, false, TILE_SMALL>(a, stream);
 }
 
 // ---- one group of 16 lanes a group of 128 values: codes [rows, blocks * 128], scales [blocks, rows]
@@ -186,10 +241,15 @@ int launch_gated_grad(const float* gu, const void* dh, int64_t dh_stride, int64_
 
 template <typename T>
 struct ProdOps {
-  static int tile(int mode, bool gated, const TileArgs& a, hipStream_t s) {
-    if (mode == PROD_DX) return launch_tile<T, PROD_DX, false>(a, s);
-    if (mode == PROD_DW) return launch_tile<T, PROD_DW, false>(a, s);
-    return gated ? launch_tile<T, PROD_FWD, true>(a, s) : launch_tile<T, PROD_FWD, false>(a, s);
+  static int tile(int mode, bool gated, const TileArgs& a, int size, hipStream_t s) {
+    if (mode == PROD_DX) return launch_tile<T, PROD_DX, false>(a, size, s);
+    if (mode == PROD_DW) return launch_tile<T, PROD_DW, false>(a, size, s);
+    return gated ? launch_tile<T, PROD_FWD, true>(a, size, s) : launch_tile<T, PROD_FWD, false>(a, size, s);
+  }
+  static int sum(bool gated, const float* part, int splits, int64_t slice, int64_t rows, int64_t N, int act, void* out, float* gu,
+                 hipStream_t s) {
+    return gated ? launch_sum_parts<T, true>(part, splits, slice, rows, N, act, out, gu, s)
+                 : launch_sum_parts<T, false>(part, splits, slice, rows, N, act, out, gu, s);
   }
   static int rows(bool fp8, bool gated, const RowsArgs& a, int mean, hipStream_t s) {
     if (fp8) return launch_rows<T, true, false>(a, mean, s);

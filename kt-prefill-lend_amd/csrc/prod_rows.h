@@ -224,11 +224,19 @@ __global__ __launch_bounds__(64 * WK * WR) void prod_rows(RowsArgs a) {
   }
 }
 
+// Tiles of 256 x 256 by 8 waves (LARGE), of 128 x 256 by 8 waves with a step more of loads on their way (DEEP), of 128 x 128
+// (SMALL) and 64 x 128 (LOW) by 4 waves, of which two and three blocks share a CU.
+enum { TILE_SMALL = 0, TILE_DEEP = 1, TILE_LARGE = 2, TILE_LOW = 3 };
+constexpr int tile_m(int size) { return size == TILE_LARGE ? 256 : size == TILE_LOW ? 64 : 128; }
+constexpr int tile_n(int size) { return size == TILE_LARGE || size == TILE_DEEP ? 256 : 128; }
+
 // The launches of one element type.
 struct ProdTable {
-  int (*tile)(int mode, bool gated, const TileArgs& a, hipStream_t stream);
+  int (*tile)(int mode, bool gated, const TileArgs& a, int size, hipStream_t stream);
+  int (*sum)(bool gated, const float* part, int splits, int64_t slice, int64_t rows, int64_t N, int act, void* out, float* gu,
+             hipStream_t stream);
   int (*rows)(bool fp8, bool gated, const RowsArgs& a, int mean, hipStream_t stream);
-  int (*fp8_tile)(const Fp8TileArgs& a, hipStream_t stream);
+  int (*fp8_tile)(const Fp8TileArgs& a, int size, hipStream_t stream);
   int (*quantise)(const void* x, int64_t stride, int64_t K, int64_t rows, const int32_t* end, uint8_t* codes, float* scales,
                   hipStream_t stream);
   int (*gated_grad)(const float* gu, const void* dh, int64_t dh_stride, int64_t N, int64_t rows, int act, void* dgu,

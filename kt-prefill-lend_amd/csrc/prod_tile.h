@@ -22,6 +22,9 @@ struct TileArgs {
   Segments seg;                  // offsets NULL: one matrix for all rows
   float* gu;                     // gated: the sums, [M, 2 N] (NULL: not kept)
   int act;
+  int splits;                    // blocks that share a tile's k; more than one: their sums go to part, one slice
+  float* part;                   // of `slice` values each, in C's layout (gated: in gu's), and sum_parts adds them up
+  int64_t slice;
 };
 
 // s_waitcnt operands: until at most n vector memory operations are outstanding, or no LDS ones
@@ -49,7 +52,8 @@ __device__ __forceinline__ int row_slot(int row, int c) {
 
 // One operand's tile of W rows by 128 bytes of k, on its way from memory to LDS and from there to registers.
 // TR: k runs across the rows in memory, and the tile is 128 / ES rows of W elements. DIRECT: loads straight
-// into LDS, for rows that start at multiples of 16 bytes; otherwise through registers, at any alignment.
+// into LDS, for rows that start at multiples of 4 bytes (what a buffer load asks for); otherwise through registers, at
+// any alignment.
 template <typename T, bool TR, bool DIRECT, int W, int THREADS>
 struct TileOperand {
   static constexpr int ES = T::ES, EPC = T::EPC, BK = STEP_BYTES / ES;
@@ -91,8 +95,9 @@ struct TileOperand {
   }
 
   // Loads step `step` of the k up to kend into dst (DIRECT) or registers. base: row 0, k = 0; bytes: from there
-  // to the operand's end; width: elements of a row in memory (TR). Chunks past kend become zeros (ENDS: there are some).
-  template <bool ENDS = true>
+  // to the operand's end; width: elements of a row in memory (TR). DIRECT: whole chunks, of which ENDS puts zeros for
+  // those past kend; otherwise elements past it become zeros.
+  template <bool ENDS>
   __device__ __forceinline__ void load(const uint8_t* base, int64_t bytes, int64_t stride, int step, int kend, int width,
                                        uint8_t* dst, int tid) {
     const int k0 = step * BK;
@@ -101,15 +106,27 @@ struct TileOperand {
       const uint64_t left = (uint64_t)(bytes - at);  // at most 2^31 - 1 of them, in scalar instructions
       const uint32_t records = (uint32_t)(left >> 32) ? 0x7fffffffu : min((uint32_t)left, 0x7fffffffu);
       const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(base + at), (short)0, (int)records, 0x00020000);
-      const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-      const bool whole = k0 + BK <= kend;
+      uint8_t* to = dst + __builtin_amdgcn_readfirstlane(tid >> 6) * 1024;
+      auto issue = [&](auto ends) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          uint32_t o = off[j];
+          // past the operand's end, where a buffer load gives zeros
+          if (decltype(ends)::value && k0 + first + (TR ? j * ROWS : 0) >= kend) o = 0x80000000u;
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(to + j * THREADS * 16), 16,
+                                                   (int)o, 0, 0, 0);
+        }
+      };
+      if (!ENDS || k0 + BK <= kend) issue(std::false_type{});
+      else issue(std::true_type{});
+    } else if (k0 + BK <= kend && (!TR || (k0 + BK - 1) * stride + (int64_t)(width + EPC) * ES <= bytes)) {
+      // whole chunks, at any alignment: across the end of a row (TR) they run into the next one, in columns that C
+      // does not have, but never past the operand
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
-        uint32_t o = off[j];
-        // past the operand's end, where a buffer load gives zeros
-        if (ENDS && !whole && k0 + first + (TR ? j * ROWS : 0) >= kend) o = 0x80000000u;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            rsrc, (__attribute__((address_space(3))) void*)(dst + (j * THREADS + wave * 64) * 16), 16, (int)o, 0, 0, 0);
+        const uint8_t* p = TR ? base + (int64_t)(k0 + first + j * ROWS) * stride + min(col, width - 1) * ES
+                              : base + (int64_t)off[j] * stride + (int64_t)(k0 + first) * ES;
+        reg[j] = gload<u32x4_a1_t>(p);
       }
     } else {
 #pragma unroll
@@ -122,6 +139,23 @@ struct TileOperand {
           reg[j] = k < kend ? load_chunk<ES>(base + (int64_t)off[j] * stride, k, kend) : u32x4_t{0, 0, 0, 0};
         }
       }
+    }
+  }
+  // A DIRECT operand's step that ends inside a chunk: chunk by chunk through registers.
+  __device__ __forceinline__ void load_end(const uint8_t* base, int64_t stride, int step, int kend, int width, uint8_t* dst,
+                                           int tid) {
+    const int k0 = step * BK;
+#pragma unroll 1
+    for (int j = 0; j < NJ; ++j) {
+      u32x4_t v = {0, 0, 0, 0};
+      if constexpr (TR) {
+        const int k = k0 + first + j * ROWS;
+        if (k < kend && col < width) v = load_chunk<ES>(base + (int64_t)k * stride, col, width);
+      } else {
+        const int k = k0 + first;
+        if (k < kend) v = load_chunk<ES>(base + (off[j] - 16 * (uint32_t)(first / EPC)), k, kend);
+      }
+      *(u32x4_t*)(dst + (j * THREADS + tid) * 16) = v;
     }
   }
   // Puts what load() has in registers into dst.
@@ -177,6 +211,7 @@ struct Place {
   int m0, rows;  // rows of C (and of P unless PROD_DW), from m0 on
   int n0;
   int k0, k1;    // PROD_DW: the expert's rows
+  int split;
 };
 
 // The tile of this block. Blocks b, b + 8, .. run on one XCD: each XCD takes a run of neighbouring tiles, panels
@@ -194,9 +229,11 @@ __device__ __forceinline__ bool place_of(const TileArgs& a, Place& pl) {
     mt = a.seg.offsets ? count_tiles(a.seg, BM, mine) : (a.M + BM - 1) / BM;
     total = (int64_t)mt * nt;
   }
-  const int64_t per = (total + 7) / 8, at = blockIdx.x >> 3;
+  const int64_t per = (total * a.splits + 7) / 8, at = blockIdx.x >> 3;
   int64_t t = (blockIdx.x & 7) * per + at;
-  if (at >= per || t >= total) return false;
+  if (at >= per || t >= total * a.splits) return false;
+  pl.split = a.splits > 1 ? (int)(t / total) : 0;
+  t -= pl.split * total;
   int e = 0;
   if constexpr (MODE == PROD_DW) {
     e = (int)(t / ((int64_t)mt * nt));
@@ -221,20 +258,50 @@ __device__ __forceinline__ bool place_of(const TileArgs& a, Place& pl) {
   return true;
 }
 
-template <typename S>
-__device__ __forceinline__ void store4(S* c, int n, int width, bool vec, f32x4_t v) {
-  if (vec && n + 4 <= width) {
-    typename vec4_of<S>::type o = {(S)v[0], (S)v[1], (S)v[2], (S)v[3]};
-    *(typename vec4_of<S>::type*)(c + n) = o;
-  } else {
+// A wave's FR rows by NO fragments of FR columns of C, from the fragments' values v(i, r) to memory: through an LDS area of
+// its own, so that every store writes whole runs of FR NO values (stored from the fragments a lane had 8 bytes of each
+// row; rows by expert, 128 gradients of 1536 x 2048: 479 us instead of 364). A wave's LDS operations complete in order,
+// so only the compiler is kept from moving them. Fragment (i): lane l holds row l % FR, columns 4 (l / FR) + r % 4 of
+// every group of 256 / FR. C's rows start at(row) elements from c, for rows that are there; cols: columns that are. WIDE: 16 bytes
+// a lane, for rows that start and end at multiples of them; else a value a lane, a row an instruction.
+constexpr int STAGE_BYTES = 8192;
+template <typename O, int FR, int NO, typename F, typename A>
+__device__ __forceinline__ void store_rows(uint8_t* stage, F v, O* c, A at, int rows, int cols, bool wide, int lane) {
+  constexpr int ROW = FR * NO * sizeof(O), CH = ROW / 16, EPC = 16 / sizeof(O), VALUES = FR * FR / 64;
+  static_assert(FR * ROW <= STAGE_BYTES, "");
+  const int q = lane / FR, l = lane % FR;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (n + i < width) c[n + i] = (S)v[i];
+  for (int i = 0; i < NO; ++i)
+#pragma unroll
+    for (int r = 0; r < VALUES; r += 4) {
+      const typename vec4_of<O>::type o = {(O)v(i, r), (O)v(i, r + 1), (O)v(i, r + 2), (O)v(i, r + 3)};
+      const int b = (FR * i + 256 / FR * (r / 4) + 4 * q) * (int)sizeof(O);  // in the row
+      *(typename vec4_of<O>::type*)(stage + l * ROW + 16 * ((b / 16) ^ (l & (CH - 1))) + b % 16) = o;
+    }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  if (wide) {
+#pragma unroll
+    for (int t = 0; t < FR * CH / 64; ++t) {
+      const int row = (t * 64 + lane) / CH, ch = lane % CH;
+      const u32x4_t x = *(const u32x4_t*)(stage + row * ROW + 16 * (ch ^ (row & (CH - 1))));
+      if (row < rows && ch * EPC < cols) *(u32x4_t*)(c + at(row) + ch * EPC) = x;
+    }
+  } else {
+    constexpr int W = FR * NO < 64 ? FR * NO : 64;  // columns an instruction
+#pragma unroll 4
+    for (int t = 0; t < FR * FR * NO / 64; ++t) {
+      const int row = t * (64 / W) * W / (FR * NO) + lane / W, n = t * W % (FR * NO) + lane % W, b = n * (int)sizeof(O);
+      const O x = *(const O*)(stage + row * ROW + 16 * ((b / 16) ^ (row & (CH - 1))) + b % 16);
+      if (row < rows && n < cols) c[at(row) + n] = x;
+    }
   }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 // WM x WN waves, each MF x NF fragments of 32 x 32.
-template <typename T, int MODE, bool GATED, bool DIRECT, int WM, int WN, int MF, int NF>
+template <typename T, int MODE, bool GATED, bool DIRECT, bool TAIL, int WM, int WN, int MF, int NF, int NB>
 __global__ __launch_bounds__(64 * WM * WN, 2) void prod_tile(TileArgs a) {
   using S = typename T::S;
   constexpr int THREADS = 64 * WM * WN, BM = 32 * WM * MF, BN = 32 * WN * NF;
@@ -244,7 +311,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void prod_tile(TileArgs a) {
   using P = TileOperand<T, PTR, DIRECT, BM, THREADS>;
   using Q = TileOperand<T, QTR, DIRECT, BN, THREADS>;
   constexpr int BUF = P::BYTES + Q::BYTES, BK = P::BK, SUBS = 4;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * BUF];
+  constexpr int NLOAD = P::NJ + Q::NJ;  // of a thread a step
+  static_assert(DIRECT || NB == 2, "");
+  __shared__ __attribute__((aligned(16))) uint8_t lds[NB * BUF];
 
   Place pl;
   if (!place_of<MODE, BM, CN>(a, pl)) return;
@@ -289,10 +358,16 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void prod_tile(TileArgs a) {
     }
     // elements of a row in memory (operands with k across the rows)
     const int pw = a.M, qw = a.N;
-    const int steps = (kend + BK - 1) / BK;
+    const int all = (kend + BK - 1) / BK, share = (all + a.splits - 1) / a.splits;
+    const int begin = pl.split * share, stop = min(all, begin + share);  // the block's steps
+    // TAIL: k runs along rows and does not end with a whole step: the last one comes after the loop, whose loads need no
+    // masks. (A kernel of its own: with this code in one for whole steps its loop, itself unchanged, took up to 15% longer.)
+    static_assert(!TAIL || (DIRECT && MODE != PROD_DW), "");
+    const bool tail = TAIL && stop == all && begin < stop;
+    const int end = stop - tail;
     auto load = [&](int k, int buf) {
-      p.load(pb, pbytes, a.p_stride, k, kend, pw, lds + buf * BUF, tid);
-      q.load(qb, qbytes, a.q_stride, k, kend, qw, lds + buf * BUF + P::BYTES, tid);
+      p.template load<MODE != PROD_FWD>(pb, pbytes, a.p_stride, k, kend, pw, lds + buf * BUF, tid);
+      q.template load<MODE != PROD_FWD>(qb, qbytes, a.q_stride, k, kend, qw, lds + buf * BUF + P::BYTES, tid);
     };
     auto put = [&](int buf) {
       p.put(lds + buf * BUF, tid);
@@ -311,64 +386,86 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void prod_tile(TileArgs a) {
 #pragma unroll
         for (int i = 0; i < NF; ++i) acc[i][j] = T::mma32(qf[from][i], pf[from][j], acc[i][j]);
     };
-    if (steps > 0) {
-      // loads past the last step read that one again, into the buffer that is free: the loop has no branches
-      const int last = steps - 1;
-      load(0, 0);
+    if (begin < end) {
+      // loads past the last step read that one again, into a buffer that is free: the loop has no branches
+      const int last = end - 1;
+      load(begin, 0);
       put(0);
-      __builtin_amdgcn_s_waitcnt(WAIT_ALL);
+#pragma unroll
+      for (int i = 1; i < NB - 1; ++i) load(min(begin + i, last), i);
+      __builtin_amdgcn_s_waitcnt(wait_vm((NB - 2) * NLOAD));
+      if constexpr (!DIRECT) __builtin_amdgcn_s_waitcnt(WAIT_ALL);
       block_barrier();
-      load(min(1, last), 1);
+      load(min(begin + NB - 1, last), NB - 1);
       read(0, 0, 0);
-      for (int k = 0; k < steps; ++k) {
-        const int buf = k & 1;
+      int buf = 0;
+      for (int k = begin; k < end; ++k) {
+        const int next = buf + 1 == NB ? 0 : buf + 1;
 #pragma unroll
         for (int s = 0; s < SUBS - 1; ++s) {
           read(buf, s + 1, (s + 1) & 1);
           mma(s & 1);
         }
-        // this step's last operands are in registers: its buffer is free for step k + 2 once every wave
-        // is here, and step k + 1's loads, on their way since the last such place, have to be there
-        put(buf ^ 1);
-        __builtin_amdgcn_s_waitcnt(WAIT_ALL);
+        // This step's last operands are in registers: its buffer is free for step k + NB once every wave is here. Step
+        // k + 1's loads have to be there; those of the NB - 2 steps behind it stay on their way (counted: loads
+        // end in order, and a thread has no others).
+        put(next);
+        __builtin_amdgcn_s_waitcnt(DIRECT ? wait_vm((NB - 2) * NLOAD) & ~(15 << 8) : WAIT_ALL);
         block_barrier();
-        load(min(k + 2, last), buf);
-        read(buf ^ 1, 0, 0);
+        load(min(k + NB, last), buf);
+        read(next, 0, 0);
         mma((SUBS - 1) & 1);
+        buf = next;
       }
-      settle(acc);
     }
+    if (TAIL && tail) {
+      __builtin_amdgcn_s_waitcnt(WAIT_ALL);
+      block_barrier();
+      p.load_end(pb, a.p_stride, end, kend, pw, lds, tid);
+      q.load_end(qb, a.q_stride, end, kend, qw, lds + P::BYTES, tid);
+      __builtin_amdgcn_s_waitcnt(WAIT_ALL);
+      block_barrier();
+#pragma unroll
+      for (int s = 0; s < SUBS; ++s) {
+        read(0, s, 0);
+        mma(0);
+      }
+    }
+    settle(acc);
   }
 
   // fragment (i, j): the lane holds row 32 j + lane % 32 of P's, rows 8 r / 4 + 4 (lane / 32) + r % 4 of Q's
-  const int h = lane >> 5, l32 = lane & 31;
+  constexpr int NO = GATED ? NF / 2 : NF;  // fragments of C's columns
   S* c = (S*)a.c + (MODE == PROD_DW ? pl.expert * a.c_expert : 0);
-  const bool vec = (a.c_stride | a.c_expert) % 4 == 0 && (uintptr_t)a.c % (4 * sizeof(S)) == 0;
-  const bool gu_vec = a.N % 4 == 0;
+  const int n0 = pl.n0 + 32 * NO * wn;  // the wave's first column
+  const bool wide = ((uintptr_t)a.c | (a.c_stride * sizeof(S)) | (a.c_expert * sizeof(S)) | (a.N * sizeof(S))) % 16 == 0;
+  const bool gu_wide = a.N % 4 == 0;
+  float* const sums = a.splits > 1 ? a.part + pl.split * a.slice : a.gu;  // slices start at multiples of 16 bytes
+  __builtin_amdgcn_s_waitcnt(WAIT_ALL);  // the last steps' loads, into the buffers that the waves stage their rows in
+  block_barrier();
+  uint8_t* stage = lds + wave * STAGE_BYTES;
 #pragma unroll
   for (int j = 0; j < MF; ++j) {
-    const int m = 32 * (MF * wm + j) + l32;
-    if (m >= pl.rows) continue;
-    S* row = c + (int64_t)(pl.m0 + m) * a.c_stride;
-#pragma unroll
-    for (int i = 0; i < (GATED ? NF / 2 : NF); ++i) {
-#pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        const int n = pl.n0 + 32 * ((GATED ? NF / 2 : NF) * wn + i) + 2 * r + 4 * h;
-        f32x4_t v = {acc[i][j][r], acc[i][j][r + 1], acc[i][j][r + 2], acc[i][j][r + 3]};
-        if constexpr (GATED) {
-          const f32x16_t& u16 = acc[i + NF / 2][j];
-          const f32x4_t u = {u16[r], u16[r + 1], u16[r + 2], u16[r + 3]};
-          if (a.gu && n < a.N) {
-            float* gu = a.gu + (int64_t)(pl.m0 + m) * 2 * a.N;
-            store4(gu, n, a.N, gu_vec, v);
-            store4(gu + a.N, n, a.N, gu_vec, u);
-          }
-#pragma unroll
-          for (int x = 0; x < 4; ++x) v[x] = act_of(a.act, v[x]) * u[x];
-        }
-        if (n < a.N) store4(row, n, a.N, vec, v);
+    const int m = 32 * (MF * wm + j), rows = pl.rows - m;
+    if (rows <= 0) break;
+    S* row = c + (int64_t)(pl.m0 + m) * a.c_stride + n0;
+    const int cols = a.N - n0;
+    auto at = [&](int i) { return i * a.c_stride; };
+    if constexpr (GATED) {
+      if (sums) {
+        float* gu = sums + (int64_t)(pl.m0 + m) * 2 * a.N + n0;
+        auto gu_at = [&](int i) { return (int64_t)i * 2 * a.N; };
+        store_rows<float, 32, NO>(stage, [&](int i, int r) { return acc[i][j][r]; }, gu, gu_at, rows, cols, gu_wide, lane);
+        store_rows<float, 32, NO>(stage, [&](int i, int r) { return acc[i + NO][j][r]; }, gu + a.N, gu_at, rows, cols, gu_wide, lane);
       }
+      if (a.splits > 1) continue;
+      store_rows<S, 32, NO>(stage, [&](int i, int r) { return act_of(a.act, acc[i][j][r]) * acc[i + NO][j][r]; }, row, at, rows,
+                            cols, wide, lane);
+    } else if (a.splits > 1) {
+      store_rows<float, 32, NO>(stage, [&](int i, int r) { return acc[i][j][r]; }, sums + (row - (S*)a.c), at, rows, cols, gu_wide,
+                                lane);
+    } else {
+      store_rows<S, 32, NO>(stage, [&](int i, int r) { return acc[i][j][r]; }, row, at, rows, cols, wide, lane);
     }
   }
 }

@@ -55,7 +55,7 @@ def _launch_dense(stream, x, w, scales):
     T, K = x.shape
     N = w.shape[0]
     y = x.new_empty((T, N))
-    need = L.ktmi_fp8_linear_workspace(K, T)
+    need = L.ktmi_fp8_linear_workspace(N, K, T)
     ws = x.new_empty((need,), dtype=torch.uint8) if need else None
     rc = L.ktmi_fp8_linear(x.data_ptr(), _CODES[x.dtype], x.stride(0), K, w.data_ptr(), scales.data_ptr(), N, T, y.data_ptr(),
                            ws.data_ptr() if need else None, need, stream)
@@ -70,7 +70,7 @@ def _launch_routed(stream, x, w, scales, ids, top_k):
     T, K = x.shape
     E, N = w.shape[:2]
     y = x.new_empty((T * top_k, N))
-    need = L.ktmi_moe_fp8_vec_workspace(K, T, top_k, E)
+    need = L.ktmi_moe_fp8_vec_workspace(N, K, T, top_k, E)
     ws = x.new_empty((need,), dtype=torch.uint8) if need else None
     rc = L.ktmi_moe_fp8_vec(x.data_ptr(), _CODES[x.dtype], x.stride(0), K, w.data_ptr(), scales.data_ptr(), N, E,
                             ids.data_ptr(), top_k, T, y.data_ptr(), ws.data_ptr() if need else None, need, stream)
@@ -85,7 +85,7 @@ def _launch_sorted(stream, rows, w, scales, offsets):
     R, K = rows.shape
     E, N = w.shape[:2]
     y = rows.new_empty((R, N))
-    need = L.ktmi_moe_fp8_sorted_workspace(K, E, R)
+    need = L.ktmi_moe_fp8_sorted_workspace(N, K, E, R)
     ws = rows.new_empty((need,), dtype=torch.uint8) if need else None
     rc = L.ktmi_moe_fp8_sorted(rows.data_ptr(), _CODES[rows.dtype], rows.stride(0), K, w.data_ptr(), scales.data_ptr(), N, E,
                                offsets.data_ptr(), R, y.data_ptr(), ws.data_ptr() if need else None, need, stream)

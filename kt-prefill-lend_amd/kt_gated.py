@@ -60,6 +60,15 @@ def _experts(w):
     return w.shape[0] if w.dim() == 3 else 1
 
 
+def _workspace(what, x, rows, cols, n_experts):
+    """(the workspace of such a call or None, its address, its bytes)."""
+    need = _lib.lib().ktmi_linear_workspace(what, _CODES[x.dtype], rows, cols, n_experts, x.shape[0])
+    if not need:
+        return None, None, 0
+    ws = x.new_empty((need,), dtype=torch.uint8)
+    return ws, ws.data_ptr(), need
+
+
 def _launch_gated(stream, what, x, w13, offsets, act, keep):
     x, w13 = _rows_of(x), w13.contiguous()
     if offsets is not None:
@@ -67,9 +76,10 @@ def _launch_gated(stream, what, x, w13, offsets, act, keep):
     R, inter = x.shape[0], w13.shape[-2] // 2
     h = x.new_empty((R, inter))
     sums = x.new_empty((R, 2 * inter), dtype=torch.float32) if keep else None
+    ws, at, need = _workspace(_lib.PROD_GATED, x, inter, x.shape[1], _experts(w13))
     rc = _lib.lib().ktmi_gated(x.data_ptr(), _CODES[x.dtype], x.stride(0), x.shape[1], w13.data_ptr(), inter, _experts(w13),
                                None if offsets is None else _address(what, offsets), R, act, h.data_ptr(),
-                               sums.data_ptr() if keep else None, stream)
+                               sums.data_ptr() if keep else None, at, need, stream)
     if rc:
         _lib.check(rc, what)
     return h, sums
@@ -78,8 +88,9 @@ def _launch_gated(stream, what, x, w13, offsets, act, keep):
 def _launch_linear(stream, what, x, w, offsets):
     x, w, offsets = _rows_of(x), w.contiguous(), offsets.contiguous()
     y = x.new_empty((x.shape[0], w.shape[1]))
+    ws, at, need = _workspace(_lib.PROD_LINEAR, x, w.shape[1], w.shape[2], w.shape[0])
     rc = _lib.lib().ktmi_linear(x.data_ptr(), _CODES[x.dtype], x.stride(0), x.shape[1], w.data_ptr(), w.shape[1], w.shape[0],
-                                _address(what, offsets), x.shape[0], y.data_ptr(), stream)
+                                _address(what, offsets), x.shape[0], y.data_ptr(), at, need, stream)
     if rc:
         _lib.check(rc, what)
     return y
@@ -98,10 +109,13 @@ def _launch_grads(stream, what, dy, x, w, offsets, want_x, want_w):
     dw = w.new_empty(w.shape) if want_w else None
     rc = 0
     if want_x:
-        rc = L.ktmi_linear_grad_x(_address(what, dy), code, dy.stride(0), N, w.data_ptr(), K, E, at, R, dx.data_ptr(), stream)
+        ws, ws_at, need = _workspace(_lib.PROD_GRAD_X, x, N, K, E)
+        rc = L.ktmi_linear_grad_x(_address(what, dy), code, dy.stride(0), N, w.data_ptr(), K, E, at, R, dx.data_ptr(), ws_at,
+                                  need, stream)
     if want_w and not rc:
+        ws, ws_at, need = _workspace(_lib.PROD_GRAD_W, x, N, K, E)
         rc = L.ktmi_linear_grad_w(_address(what, dy), code, dy.stride(0), N, x.data_ptr(), x.stride(0), K, E, at, R,
-                                  dw.data_ptr(), stream)
+                                  dw.data_ptr(), ws_at, need, stream)
     if rc:
         _lib.check(rc, what)
     return dx, dw

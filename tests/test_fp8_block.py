@@ -385,16 +385,16 @@ def test_c_refusals():
     for kw in [dict(dt=3), dict(K=0), dict(N=0), dict(T=-1), dict(x=0), dict(w=0), dict(s=0), dict(y=0), dict(x=p + 1), dict(s=p + 1),
                dict(y=p + 1), dict(xs=63), dict(K=1 << 25, xs=1 << 25), dict(T=1 << 31)]:
         assert dense(**kw) == -1 and b"fp8_linear" in L.ktmi_last_error(), kw
-    need = L.ktmi_fp8_linear_workspace(64, 1000)
+    need = L.ktmi_fp8_linear_workspace(8, 64, 1000)
     assert need >= 1000 * 128 and dense(T=1000, n=need - 1) == -4 and dense(T=1000, ws=0) == -4 and dense(T=1000, ws=p + 4) == -4
-    assert dense(T=0) == 0 and L.ktmi_fp8_linear_workspace(0, 5) == 0 and L.ktmi_fp8_linear_workspace(64, -1) == 0
+    assert dense(T=0) == 0 and L.ktmi_fp8_linear_workspace(8, 0, 5) == 0 and L.ktmi_fp8_linear_workspace(8, 64, -1) == 0
 
     def routed_(E=4, ids=p, k=2, T=2, ws=p, n=1 << 40, x=p, N=8):
         return L.ktmi_moe_fp8_vec(x, 2, 64, 64, p, p, N, E, ids, k, T, p, ws, n, 0)
 
     for kw in [dict(E=0), dict(E=F.MAX_EXPERTS + 1), dict(ids=0), dict(k=0), dict(k=65536), dict(T=-1), dict(T=1 << 31), dict(x=0)]:
         assert routed_(**kw) == -1 and b"moe_fp8_vec" in L.ktmi_last_error(), kw
-    need = L.ktmi_moe_fp8_vec_workspace(64, 100, 8, 4)
+    need = L.ktmi_moe_fp8_vec_workspace(8, 64, 100, 8, 4)
     assert need > 0 and routed_(T=100, k=8, n=need - 1) == -4 and routed_(T=100, k=8, ws=0) == -4
     assert routed_(T=0) == 0
 
@@ -403,7 +403,7 @@ def test_c_refusals():
 
     for kw in [dict(E=0), dict(off=0), dict(R=-1), dict(N=0), dict(R=1 << 31)]:
         assert sorted_(**kw) == -1 and b"moe_fp8_sorted" in L.ktmi_last_error(), kw
-    need = L.ktmi_moe_fp8_sorted_workspace(64, 4, 1000)
+    need = L.ktmi_moe_fp8_sorted_workspace(8, 64, 4, 1000)
     assert need > 0 and sorted_(R=1000, n=need - 1) == -4
     assert sorted_(R=0) == 0
     # a grid past 2^32 threads

@@ -283,6 +283,15 @@ def test_strides_and_alignment(dev, rows, dtype):
                 xx, ww = xx.detach().requires_grad_(True), ww.detach().requires_grad_(True)
                 got = grads(lambda x, w: G.moe_linear_sorted(x, w, strided[::2]), [xx, ww], dd)
                 assert all(torch.equal(a, b) for a, b in zip(got, want))
+    # rows that end inside a word or a chunk, at strides that are multiples of 16 bytes; what lies behind them is not read
+    for n in (K - 1, K - 3):
+        xx, ww, dd = [torch.full((t.shape[0], t.shape[1] + 24), float("nan"), dtype=dtype, device=dev)[:, :m]
+                      for t, m in ((x, n), (w.reshape(2 * N, K), n), (dy, N - 1))]
+        xx.copy_(x[:, :n]), dd.copy_(dy[:, :N - 1])
+        wp = w[:, :N - 1, :n].contiguous()
+        got = grads(lambda x, w: G.moe_linear_sorted(x, w, offsets), [xx.requires_grad_(True), wp.requires_grad_(True)], dd)
+        for a, b in zip(got, linear64(x[:, :n], wp.detach(), offsets, dy[:, :N - 1])):
+            same(a, b)
     # the gate's gradient from a strided dh
     dh = dwide[:, 3:N // 2 + 3]
     fn = lambda x, w: G.moe_gated_sorted(x, w, offsets)  # noqa: E731
@@ -518,8 +527,8 @@ def test_c_refusals():
     L = _lib.lib()
     p = 4096
 
-    def gated(x=p, dt=2, xs=64, K=64, w=p, N=8, E=4, off=p, R=2, act=0, h=p, sums=0):
-        return L.ktmi_gated(x, dt, xs, K, w, N, E, off, R, act, h, sums, 0)
+    def gated(x=p, dt=2, xs=64, K=64, w=p, N=8, E=4, off=p, R=2, act=0, h=p, sums=0, ws=p, n=1 << 50):
+        return L.ktmi_gated(x, dt, xs, K, w, N, E, off, R, act, h, sums, ws, n, 0)
 
     for kw in [dict(dt=3), dict(K=0), dict(N=0), dict(R=-1), dict(x=0), dict(w=0), dict(h=0), dict(x=p + 1), dict(w=p + 1), dict(h=p + 1),
                dict(sums=p + 4), dict(xs=63), dict(K=1 << 25, xs=1 << 25), dict(R=1 << 31), dict(E=0), dict(E=2049), dict(off=0),
@@ -534,14 +543,14 @@ def test_c_refusals():
         assert grad(**kw) == -1 and b"gated_grad" in L.ktmi_last_error(), kw
     assert grad(R=0) == 0
 
-    def linear(x=p, dt=2, xs=64, K=64, w=p, N=8, E=4, off=p, R=2, y=p):
-        return L.ktmi_linear(x, dt, xs, K, w, N, E, off, R, y, 0)
+    def linear(x=p, dt=2, xs=64, K=64, w=p, N=8, E=4, off=p, R=2, y=p, ws=p, n=1 << 50):
+        return L.ktmi_linear(x, dt, xs, K, w, N, E, off, R, y, ws, n, 0)
 
-    def grad_x(x=p, dt=2, xs=64, K=8, w=p, N=64, E=4, off=p, R=2, y=p):
-        return L.ktmi_linear_grad_x(x, dt, xs, N, w, K, E, off, R, y, 0)
+    def grad_x(x=p, dt=2, xs=64, K=8, w=p, N=64, E=4, off=p, R=2, y=p, ws=p, n=1 << 50):
+        return L.ktmi_linear_grad_x(x, dt, xs, N, w, K, E, off, R, y, ws, n, 0)
 
-    def grad_w(x=p, dt=2, xs=64, K=64, N=64, E=4, off=p, R=2, y=p, dy=p, ds=64):
-        return L.ktmi_linear_grad_w(dy, dt, ds, N, x, xs, K, E, off, R, y, 0)
+    def grad_w(x=p, dt=2, xs=64, K=64, N=64, E=4, off=p, R=2, y=p, dy=p, ds=64, ws=p, n=1 << 50):
+        return L.ktmi_linear_grad_w(dy, dt, ds, N, x, xs, K, E, off, R, y, ws, n, 0)
 
     for fn, name in ((linear, b"linear"), (grad_x, b"linear_grad_x"), (grad_w, b"linear_grad_w")):
         for kw in [dict(dt=3), dict(K=0), dict(N=0), dict(R=-1), dict(x=0), dict(y=0), dict(x=p + 1), dict(y=p + 1), dict(xs=63),
