@@ -34,7 +34,7 @@ struct TilePlan {
 // with three splits 46; by 7168 x 2048: 25 us, with two 40.)
 TilePlan split_tiles(int size, int es, int64_t tiles, int64_t steps, int64_t values, double* us) {
   const bool four = size == TILE_LOW || size == TILE_SMALL;
-  const int64_t slots = size == TILE_LOW ? 768 : size == TILE_SMALL ? 512 : 256;
+  const int64_t slots = size == TILE_LOW && es != 2 ? 768 : four ? 512 : 256;
   TilePlan best = {size, 1};
   for (int64_t s = 1; s <= 16 && (s == 1 || (tiles * s <= slots && steps >= 8 * s)); ++s) {
     const int64_t blocks = tiles * s, rounds = (blocks + slots - 1) / slots, shared = (blocks + 255) / 256;

@@ -13,6 +13,9 @@ typedef uint32_t u32x4_a1_t __attribute__((ext_vector_type(4))) __attribute__((a
 
 namespace ktmi {
 
+// and stores
+__device__ __forceinline__ void gstore(void* p, u32x4_t v) { *(__attribute__((address_space(1))) u32x4_a1_t*)p = v; }
+
 // An element type: its bytes (ES), elements of a 16-byte chunk (EPC), the fp32 value of one and back, and
 // the products of 32 rows by 32 rows (mma32) and 16 by 16 (mma16) over the k of one chunk a lane: lane half
 // (quarter) q holds chunk q of its row, so that the sum runs over 2 (4) chunks. fp32 chunks take four

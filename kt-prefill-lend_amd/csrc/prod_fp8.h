@@ -92,8 +92,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile(Fp8TileArgs a) {
   constexpr int THREADS = 64 * WM * WN, BM = 16 * WM * MF, BN = 16 * WN * NF;
   using P = TileOperand<E4M3, false, true, BM, THREADS>;
   using Q = TileOperand<E4M3, false, DIRECT, BN, THREADS>;
-  constexpr int BUF = P::BYTES + Q::BYTES + BM * 4 + 256;  // rows, their scales, those of the columns' blocks
-
+  constexpr int SCALES = P::BYTES + Q::BYTES, BUF = SCALES + THREADS * 4;  // rows, and a scale for each thread
+  constexpr int NLOAD = P::NJ + Q::NJ + 1;  // of a thread a step
+  static_assert(MF % 2 == 0, "");
   static_assert(BM % 64 == 0 && BM <= THREADS && 128 % (16 * NF) == 0 && BN % 128 == 0, "a wave's columns lie in one block");
   __shared__ __attribute__((aligned(16))) uint8_t lds[2 * BUF];
 
@@ -124,33 +125,31 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile(Fp8TileArgs a) {
     const int64_t qbytes = (int64_t)(a.N - pl.n0) * a.K;
     const int end = a.N - 1 - pl.n0;
     q.init(tid, a.K, 0, [&](int i) { return min(i, end); });
-    // The scales of a step go to LDS too: wave i < BM / 64 takes those of 64 rows, the next one those of the columns'
-    // blocks (by scalar loads, which count with the LDS reads, every step waited for them)
+    // The scales of a step go to LDS too, a value a thread: wave i < BM / 64 takes those of 64 rows, the next one those of
+    // the columns' blocks, any other loads that one's again, which nobody reads (by scalar loads, which count with the
+    // LDS reads, every step waited for them).
     constexpr int SW = BM / 64;
     static_assert(SW < WM * WN, "");
     const int col_blocks = (a.N + 127) / 128;
-    const float* sp = wave < SW ? a.xs + sbase + row_of(tid)
-                                : a.ws + ((int64_t)pl.expert * col_blocks + min(pl.n0 / 128 + (lane & (BN / 128 - 1)), col_blocks - 1)) * blocks;
-    const int64_t sp_step = wave < SW ? a.xs_stride : 1;
-    float s_reg = 0;
+    const bool of_rows = wave < SW;
+    const int col = min(pl.n0 / 128 + (lane & (BN / 128 - 1)), col_blocks - 1);
+    const float* sb = of_rows ? a.xs + sbase : a.ws + ((int64_t)pl.expert * col_blocks + col) * blocks;
+    const float* sp = sb + (of_rows ? row_of(tid) : 0);
+    const int64_t s_step = of_rows ? a.xs_stride : 1;
     auto load = [&](int k, int buf) {
       uint8_t* b = lds + buf * BUF;
-      if (wave <= SW) s_reg = gload<float>(sp + k * sp_step);
-      p.template load<false>(pb, pbytes, a.x_stride, k, blocks * 128, 0, b, tid);
-      q.template load<true>(qb, qbytes, a.K, k, a.K, 0, b + P::BYTES, tid);
+      __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)(sp + k * s_step),
+                                       (__attribute__((address_space(3))) void*)(b + SCALES + wave * 256), 4, 0, 0);
+      p.template load<false>(pb, pbytes, a.x_stride, k, true, blocks * 128, 0, b, tid);
+      q.template load<true>(qb, qbytes, a.K, k, true, a.K, 0, b + P::BYTES, tid);
     };
-    auto put = [&](int buf) {
-      uint8_t* b = lds + buf * BUF;
-      if (wave <= SW) *(float*)(b + P::BYTES + Q::BYTES + 4 * tid) = s_reg;
-      q.put(b + P::BYTES, tid);
-    };
+    auto put = [&](int buf) { q.put(lds + buf * BUF + P::BYTES, tid); };
     u32x4_t pf[2][2], qf[NF][2];
     float sx[2];
     // a lane's chunks of fragment 0 of x's and w's rows (fragment j is 16 rows on, with the same slots), its scale
     const int slot[2] = {16 * row_slot<1>(l16, q4), 16 * row_slot<1>(l16, 4 + q4)};
     const int p_at = (16 * MF * wm + l16) * STEP_BYTES, q_at = P::BYTES + (16 * NF * wn + l16) * STEP_BYTES;
-    const int s_at = P::BYTES + Q::BYTES + 4 * (16 * MF * wm + l16);
-    const int sw_at = P::BYTES + Q::BYTES + 4 * BM + 4 * (16 * NF * wn / 128);
+    const int s_at = SCALES + 4 * (16 * MF * wm + l16), sw_at = SCALES + 4 * BM + 4 * (16 * NF * wn / 128);
     auto read_p = [&](int buf, int j, int to) {
       const uint8_t* b = lds + buf * BUF;
 #pragma unroll
@@ -161,12 +160,18 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile(Fp8TileArgs a) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) qf[i][c] = *(const u32x4_t*)(lds + buf * BUF + q_at + slot[c] + 16 * i * STEP_BYTES);
     };
-    load(begin, 0);
-    put(0);
-    __builtin_amdgcn_s_waitcnt(WAIT_ALL);
-    block_barrier();
     // loads past the last step read that one again, into the buffer that is free: the loop has no branches
-    load(min(begin + 1, end_k), 1);
+    load(begin, 0);
+    if constexpr (DIRECT) {
+      load(min(begin + 1, end_k), 1);
+      __builtin_amdgcn_s_waitcnt(wait_vm(NLOAD));
+      block_barrier();
+    } else {
+      put(0);
+      __builtin_amdgcn_s_waitcnt(WAIT_ALL);
+      block_barrier();
+      load(min(begin + 1, end_k), 1);
+    }
 #pragma unroll
     for (int i = 0; i < NF; ++i) read_q(0, i);
     read_p(0, 0, 0);
@@ -197,21 +202,21 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile(Fp8TileArgs a) {
       asm volatile("" : "+v"(acc[NF - 1][jp]));
     };
     for (int k = begin; k <= end_k; ++k) {
-      const int buf = (k - begin) & 1;
+      const int buf = (k - begin) & 1, next = buf ^ 1;
 #pragma unroll
       for (int j = 0; j + 1 < MF; ++j) {
         read_p(buf, j + 1, (j + 1) & 1);
         products(j, [](int) {});
       }
-      // the step's last rows are in registers, and its columns too: the buffer is free for step k + 2 once
-      // every wave is here, and step k + 1's loads, on their way since the last such place, have to be there
-      put(buf ^ 1);
+      // The step's last rows are in registers, and its columns too: the buffer is free for step k + 2 once every wave is
+      // here, and step k + 1's loads, on their way since the last such place, have to be there.
+      put(next);
       __builtin_amdgcn_s_waitcnt(WAIT_ALL);
       block_barrier();
       load(min(k + 2, end_k), buf);
-      products(MF - 1, [&](int i) { read_q(buf ^ 1, i); });
-      read_p(buf ^ 1, 0, 0);
-      sw = *(const float*)(lds + (buf ^ 1) * BUF + sw_at);
+      products(MF - 1, [&](int i) { read_q(next, i); });
+      read_p(next, 0, 0);
+      sw = *(const float*)(lds + next * BUF + sw_at);
     }
     settle(c);
 #pragma unroll
@@ -226,7 +231,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile(Fp8TileArgs a) {
     const int p = pl.m0 + m;
     return a.perm ? (pl.expert >= 0 ? a.perm[p] : ~a.perm[p]) : p;
   };
-  const bool wide = ((uintptr_t)a.y | (a.N * sizeof(S))) % 16 == 0;
   __builtin_amdgcn_s_waitcnt(WAIT_ALL);  // the last steps' loads, into the buffers that the waves stage their rows in
   block_barrier();
   uint8_t* stage = lds + wave * STAGE_BYTES;
@@ -236,11 +240,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile(Fp8TileArgs a) {
     if (m >= pl.rows) break;
     if (a.splits > 1) {  // (its rows in the order of y already)
       store_rows<float, 16, NF>(stage, [&](int i, int r) { return acc[i][j][r]; }, a.part + pl.split * a.slice + n0,
-                                [&](int i) { return (int64_t)place(m + i) * a.N; }, pl.rows - m, a.N - n0, a.N % 4 == 0, lane);
+                                [&](int i) { return (int64_t)place(m + i) * a.N; }, pl.rows - m, a.N - n0, lane);
       continue;
     }
     store_rows<S, 16, NF>(stage, [&](int i, int r) { return acc[i][j][r]; }, (S*)a.y + n0,
-                          [&](int i) { return (int64_t)place(m + i) * a.N; }, pl.rows - m, a.N - n0, wide, lane);
+                          [&](int i) { return (int64_t)place(m + i) * a.N; }, pl.rows - m, a.N - n0, lane);
   }
 }
 

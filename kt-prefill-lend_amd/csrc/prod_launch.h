@@ -15,7 +15,7 @@ int launch_tile_of(const TileArgs& a, hipStream_t stream) {
   KTMI_REQUIRE(grid < (int64_t)0xffffffff / THREADS, KTMI_EINVAL, "a grid of %lld blocks (below 2^32 threads)", (long long)grid);
   if constexpr (SIZE == TILE_LARGE) prod_tile<T, MODE, GATED, DIRECT, TAIL, 2, 4, 4, 2, 2><<<(unsigned)grid, THREADS, 0, stream>>>(a);
   else if constexpr (SIZE == TILE_DEEP) prod_tile<T, MODE, GATED, DIRECT, TAIL, 2, 4, 2, 2, 3><<<(unsigned)grid, THREADS, 0, stream>>>(a);
-  else if constexpr (SIZE == TILE_LOW) prod_tile<T, MODE, GATED, DIRECT, TAIL, 2, 2, 1, 2, 2><<<(unsigned)grid, THREADS, 0, stream>>>(a);
+  else if constexpr (SIZE == TILE_LOW) prod_tile<T, MODE, GATED, DIRECT, TAIL, 2, 2, 1, 2, (DIRECT && T::ES == 2 ? 3 : 2)><<<(unsigned)grid, THREADS, 0, stream>>>(a);
   else prod_tile<T, MODE, GATED, DIRECT, TAIL, 2, 2, 2, 2, 2><<<(unsigned)grid, THREADS, 0, stream>>>(a);
   KTMI_HIP_TRY(hipGetLastError());
   return KTMI_OK;

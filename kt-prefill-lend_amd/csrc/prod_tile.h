@@ -96,15 +96,16 @@ struct TileOperand {
 
   // Loads step `step` of the k up to kend into dst (DIRECT) or registers. base: row 0, k = 0; bytes: from there
   // to the operand's end; width: elements of a row in memory (TR). DIRECT: whole chunks, of which ENDS puts zeros for
-  // those past kend; otherwise elements past it become zeros.
+  // those past kend; otherwise elements past it become zeros. A step that is not `there` is past every operand's end: its
+  // loads are counted as the others and fetch nothing.
   template <bool ENDS>
-  __device__ __forceinline__ void load(const uint8_t* base, int64_t bytes, int64_t stride, int step, int kend, int width,
+  __device__ __forceinline__ void load(const uint8_t* base, int64_t bytes, int64_t stride, int step, bool there, int kend, int width,
                                        uint8_t* dst, int tid) {
     const int k0 = step * BK;
     if constexpr (DIRECT) {
       const int64_t at = TR ? (int64_t)k0 * stride : (int64_t)k0 * ES;
       const uint64_t left = (uint64_t)(bytes - at);  // at most 2^31 - 1 of them, in scalar instructions
-      const uint32_t records = (uint32_t)(left >> 32) ? 0x7fffffffu : min((uint32_t)left, 0x7fffffffu);
+      const uint32_t records = !there ? 0u : (uint32_t)(left >> 32) ? 0x7fffffffu : min((uint32_t)left, 0x7fffffffu);
       const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(base + at), (short)0, (int)records, 0x00020000);
       uint8_t* to = dst + __builtin_amdgcn_readfirstlane(tid >> 6) * 1024;
       auto issue = [&](auto ends) {
@@ -262,11 +263,11 @@ __device__ __forceinline__ bool place_of(const TileArgs& a, Place& pl) {
 // its own, so that every store writes whole runs of FR NO values (stored from the fragments a lane had 8 bytes of each
 // row; rows by expert, 128 gradients of 1536 x 2048: 479 us instead of 364). A wave's LDS operations complete in order,
 // so only the compiler is kept from moving them. Fragment (i): lane l holds row l % FR, columns 4 (l / FR) + r % 4 of
-// every group of 256 / FR. C's rows start at(row) elements from c, for rows that are there; cols: columns that are. WIDE: 16 bytes
-// a lane, for rows that start and end at multiples of them; else a value a lane, a row an instruction.
+// every group of 256 / FR. C's rows start at(row) elements from c, at any address, for rows that are there; cols: columns that
+// are.
 constexpr int STAGE_BYTES = 8192;
 template <typename O, int FR, int NO, typename F, typename A>
-__device__ __forceinline__ void store_rows(uint8_t* stage, F v, O* c, A at, int rows, int cols, bool wide, int lane) {
+__device__ __forceinline__ void store_rows(uint8_t* stage, F v, O* c, A at, int rows, int cols, int lane) {
   constexpr int ROW = FR * NO * sizeof(O), CH = ROW / 16, EPC = 16 / sizeof(O), VALUES = FR * FR / 64;
   static_assert(FR * ROW <= STAGE_BYTES, "");
   const int q = lane / FR, l = lane % FR;
@@ -280,20 +281,16 @@ __device__ __forceinline__ void store_rows(uint8_t* stage, F v, O* c, A at, int 
     }
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-  if (wide) {
 #pragma unroll
-    for (int t = 0; t < FR * CH / 64; ++t) {
-      const int row = (t * 64 + lane) / CH, ch = lane % CH;
-      const u32x4_t x = *(const u32x4_t*)(stage + row * ROW + 16 * (ch ^ (row & (CH - 1))));
-      if (row < rows && ch * EPC < cols) *(u32x4_t*)(c + at(row) + ch * EPC) = x;
-    }
-  } else {
-    constexpr int W = FR * NO < 64 ? FR * NO : 64;  // columns an instruction
-#pragma unroll 4
-    for (int t = 0; t < FR * FR * NO / 64; ++t) {
-      const int row = t * (64 / W) * W / (FR * NO) + lane / W, n = t * W % (FR * NO) + lane % W, b = n * (int)sizeof(O);
-      const O x = *(const O*)(stage + row * ROW + 16 * ((b / 16) ^ (row & (CH - 1))) + b % 16);
-      if (row < rows && n < cols) c[at(row) + n] = x;
+  for (int t = 0; t < FR * CH / 64; ++t) {
+    const int row = (t * 64 + lane) / CH, ch = lane % CH, left = cols - ch * EPC;
+    const uint8_t* from = stage + row * ROW + 16 * (ch ^ (row & (CH - 1)));
+    O* to = c + at(row) + ch * EPC;
+    if (row >= rows || left <= 0) continue;
+    if (left >= EPC) {
+      gstore(to, *(const u32x4_t*)from);
+    } else {
+      for (int i = 0; i < left; ++i) to[i] = ((const O*)from)[i];
     }
   }
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -366,8 +363,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void prod_tile(TileArgs a) {
     const bool tail = TAIL && stop == all && begin < stop;
     const int end = stop - tail;
     auto load = [&](int k, int buf) {
-      p.template load<MODE != PROD_FWD>(pb, pbytes, a.p_stride, k, kend, pw, lds + buf * BUF, tid);
-      q.template load<MODE != PROD_FWD>(qb, qbytes, a.q_stride, k, kend, qw, lds + buf * BUF + P::BYTES, tid);
+      const bool there = k < end;
+      const int step = there ? k : end - 1;
+      p.template load<MODE != PROD_FWD>(pb, pbytes, a.p_stride, step, there, kend, pw, lds + buf * BUF, tid);
+      q.template load<MODE != PROD_FWD>(qb, qbytes, a.q_stride, step, there, kend, qw, lds + buf * BUF + P::BYTES, tid);
     };
     auto put = [&](int buf) {
       p.put(lds + buf * BUF, tid);
@@ -387,16 +386,19 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void prod_tile(TileArgs a) {
         for (int i = 0; i < NF; ++i) acc[i][j] = T::mma32(qf[from][i], pf[from][j], acc[i][j]);
     };
     if (begin < end) {
-      // loads past the last step read that one again, into a buffer that is free: the loop has no branches
-      const int last = end - 1;
-      load(begin, 0);
-      put(0);
+      // loads past the last step are issued too, and fetch nothing: the loop has no branches
+      if constexpr (DIRECT) {
 #pragma unroll
-      for (int i = 1; i < NB - 1; ++i) load(min(begin + i, last), i);
-      __builtin_amdgcn_s_waitcnt(wait_vm((NB - 2) * NLOAD));
-      if constexpr (!DIRECT) __builtin_amdgcn_s_waitcnt(WAIT_ALL);
-      block_barrier();
-      load(min(begin + NB - 1, last), NB - 1);
+        for (int i = 0; i < NB; ++i) load(begin + i, i);
+        __builtin_amdgcn_s_waitcnt(wait_vm((NB - 1) * NLOAD));
+        block_barrier();
+      } else {
+        load(begin, 0);
+        put(0);
+        __builtin_amdgcn_s_waitcnt(WAIT_ALL);
+        block_barrier();
+        load(begin + 1, 1);
+      }
       read(0, 0, 0);
       int buf = 0;
       for (int k = begin; k < end; ++k) {
@@ -412,7 +414,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void prod_tile(TileArgs a) {
         put(next);
         __builtin_amdgcn_s_waitcnt(DIRECT ? wait_vm((NB - 2) * NLOAD) & ~(15 << 8) : WAIT_ALL);
         block_barrier();
-        load(min(k + NB, last), buf);
+        load(k + NB, buf);
         read(next, 0, 0);
         mma((SUBS - 1) & 1);
         buf = next;
@@ -438,9 +440,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void prod_tile(TileArgs a) {
   constexpr int NO = GATED ? NF / 2 : NF;  // fragments of C's columns
   S* c = (S*)a.c + (MODE == PROD_DW ? pl.expert * a.c_expert : 0);
   const int n0 = pl.n0 + 32 * NO * wn;  // the wave's first column
-  const bool wide = ((uintptr_t)a.c | (a.c_stride * sizeof(S)) | (a.c_expert * sizeof(S)) | (a.N * sizeof(S))) % 16 == 0;
-  const bool gu_wide = a.N % 4 == 0;
-  float* const sums = a.splits > 1 ? a.part + pl.split * a.slice : a.gu;  // slices start at multiples of 16 bytes
+  float* const sums = a.splits > 1 ? a.part + pl.split * a.slice : a.gu;
   __builtin_amdgcn_s_waitcnt(WAIT_ALL);  // the last steps' loads, into the buffers that the waves stage their rows in
   block_barrier();
   uint8_t* stage = lds + wave * STAGE_BYTES;
@@ -455,17 +455,16 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void prod_tile(TileArgs a) {
       if (sums) {
         float* gu = sums + (int64_t)(pl.m0 + m) * 2 * a.N + n0;
         auto gu_at = [&](int i) { return (int64_t)i * 2 * a.N; };
-        store_rows<float, 32, NO>(stage, [&](int i, int r) { return acc[i][j][r]; }, gu, gu_at, rows, cols, gu_wide, lane);
-        store_rows<float, 32, NO>(stage, [&](int i, int r) { return acc[i + NO][j][r]; }, gu + a.N, gu_at, rows, cols, gu_wide, lane);
+        store_rows<float, 32, NO>(stage, [&](int i, int r) { return acc[i][j][r]; }, gu, gu_at, rows, cols, lane);
+        store_rows<float, 32, NO>(stage, [&](int i, int r) { return acc[i + NO][j][r]; }, gu + a.N, gu_at, rows, cols, lane);
       }
       if (a.splits > 1) continue;
       store_rows<S, 32, NO>(stage, [&](int i, int r) { return act_of(a.act, acc[i][j][r]) * acc[i + NO][j][r]; }, row, at, rows,
-                            cols, wide, lane);
+                            cols, lane);
     } else if (a.splits > 1) {
-      store_rows<float, 32, NO>(stage, [&](int i, int r) { return acc[i][j][r]; }, sums + (row - (S*)a.c), at, rows, cols, gu_wide,
-                                lane);
+      store_rows<float, 32, NO>(stage, [&](int i, int r) { return acc[i][j][r]; }, sums + (row - (S*)a.c), at, rows, cols, lane);
     } else {
-      store_rows<S, 32, NO>(stage, [&](int i, int r) { return acc[i][j][r]; }, row, at, rows, cols, wide, lane);
+      store_rows<S, 32, NO>(stage, [&](int i, int r) { return acc[i][j][r]; }, row, at, rows, cols, lane);
     }
   }
 }
