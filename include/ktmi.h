@@ -201,6 +201,11 @@ int ktmi_moe_fp8_sorted(const void* x, int x_dtype, int64_t x_stride, int64_t co
                         int64_t rows, int64_t n_experts, const int32_t* offsets, int64_t n_rows, void* y, void* workspace,
                         int64_t ws_bytes, void* stream);
 
+/* The kernel that such a call takes, as ktmi_linear_kernel_of tells; routed: 1 for ktmi_moe_fp8_vec's. */
+struct ktmi_prod_kernel;
+int ktmi_fp8_kernel_of(int routed, int64_t rows, int64_t cols, int64_t n_experts, int64_t top_k, int64_t x_rows,
+                       struct ktmi_prod_kernel* kernel);
+
 /* ---- gated and linear products with gradients --------------------------------------
  * Rows of x [n_rows, cols] by the matrix of their expert, in bf16, f16 or fp32 (x, w, y and gradients of one type), sums in
  * fp32, rounded once. offsets: the experts' segments as ktmi_moe_sort gives them (rows in no segment give zeros, clamped
@@ -212,6 +217,14 @@ int ktmi_moe_fp8_sorted(const void* x, int x_dtype, int64_t x_stride, int64_t co
  * = inter). */
 enum { KTMI_PROD_GATED = 0, KTMI_PROD_LINEAR = 1, KTMI_PROD_GRAD_X = 2, KTMI_PROD_GRAD_W = 3 };
 int64_t ktmi_linear_workspace(int what, int dtype, int64_t rows, int64_t cols, int64_t n_experts, int64_t n_rows);
+/* The kernel that such a call takes (as w4_kernel_of). */
+typedef struct ktmi_prod_kernel {
+  int32_t tile_rows;  /* rows of x a tile (gradient of w: of w); 0: the kernel of few rows */
+  int32_t tile_cols;  /* columns of y a tile (GATED: of both projections together) */
+  int32_t splits;     /* blocks that share a tile's k */
+} ktmi_prod_kernel;
+int ktmi_linear_kernel_of(int what, int dtype, int64_t rows, int64_t cols, int64_t n_experts, int64_t n_rows,
+                          ktmi_prod_kernel* kernel);
 /* h = act(x Wg^T) * (x Wu^T), w13 [n_experts, 2 inter, cols] = rows [gate; up], h [n_rows, inter]. sums fp32 [n_rows, 2 inter]
  * takes both projections before the activation, which the gradient needs (NULL: not kept). */
 int ktmi_gated(const void* x, int dtype, int64_t x_stride, int64_t cols, const void* w13, int64_t inter, int64_t n_experts,

@@ -60,6 +60,14 @@ class ktmi_w4_kernel(C.Structure):
     ]
 
 
+class ktmi_prod_kernel(C.Structure):
+    _fields_ = [
+        ("tile_rows", C.c_int32),
+        ("tile_cols", C.c_int32),
+        ("splits", C.c_int32),
+    ]
+
+
 # name -> (restype, argtypes); every symbol declared in include/ktmi.h
 SIGNATURES = {
     "ktmi_last_error": (C.c_char_p, []),
@@ -90,6 +98,8 @@ SIGNATURES = {
     "ktmi_moe_fp8_vec": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _vp]),
     "ktmi_moe_fp8_sorted_workspace": (_i64, [_i64, _i64, _i64, _i64]),
     "ktmi_moe_fp8_sorted": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp]),
+    "ktmi_fp8_kernel_of": (_i32, [_i32, _i64, _i64, _i64, _i64, _i64, C.POINTER(ktmi_prod_kernel)]),
+    "ktmi_linear_kernel_of": (_i32, [_i32, _i32, _i64, _i64, _i64, _i64, C.POINTER(ktmi_prod_kernel)]),
     "ktmi_linear_workspace": (_i64, [_i32, _i32, _i64, _i64, _i64, _i64]),
     "ktmi_gated": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i32, _vp, _vp, _vp, _i64, _vp]),
     "ktmi_gated_grad": (_i32, [_vp, _vp, _i32, _i64, _i64, _i64, _i32, _vp, _vp]),

@@ -384,6 +384,14 @@ int ktmi_moe_fp8_sorted(const void* x, int x_dtype, int64_t x_stride, int64_t co
   return launch_fp8(a, (hipStream_t)stream);
 }
 
+int ktmi_fp8_kernel_of(int routed, int64_t rows, int64_t cols, int64_t n_experts, int64_t top_k, int64_t x_rows,
+                       ktmi_prod_kernel* kernel) {
+  g_err[0] = 0;
+  KTMI_REQUIRE(fp8_shape(rows, cols, x_rows, n_experts, top_k) && kernel, KTMI_EINVAL, "fp8_kernel_of: a shape, or a null pointer");
+  *kernel = fp8_kernel_of(rows, cols, x_rows, n_experts, top_k, routed != 0);
+  return KTMI_OK;
+}
+
 // ---- gated and linear products with gradients
 
 static int check_prod(const char* what, const ProdArgs& a) {
@@ -411,6 +419,16 @@ int64_t ktmi_linear_workspace(int what, int dtype, int64_t rows, int64_t cols, i
       cols > (1 << 24) || n_experts <= 0 || n_experts > SORT_MAX_EXPERTS || n_rows <= 0 || n_rows > MAX_ROWS)
     return 0;
   return prod_workspace(what, dtype, rows, cols, n_experts, n_rows);
+}
+
+int ktmi_linear_kernel_of(int what, int dtype, int64_t rows, int64_t cols, int64_t n_experts, int64_t n_rows,
+                          ktmi_prod_kernel* kernel) {
+  g_err[0] = 0;
+  KTMI_REQUIRE(what >= KTMI_PROD_GATED && what <= KTMI_PROD_GRAD_W && dtype_ok(dtype) && rows > 0 && rows <= (1 << 24) && cols > 0 &&
+                   cols <= (1 << 24) && n_experts > 0 && n_experts <= SORT_MAX_EXPERTS && n_rows > 0 && n_rows <= MAX_ROWS && kernel,
+               KTMI_EINVAL, "linear_kernel_of: a shape, or a null pointer");
+  *kernel = prod_kernel_of(what, dtype, rows, cols, n_experts, n_rows);
+  return KTMI_OK;
 }
 
 // the call's workspace is there; then it runs

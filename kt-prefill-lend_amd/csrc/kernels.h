@@ -73,6 +73,7 @@ struct ProdArgs {
   float* part;  // workspace
 };
 int64_t prod_workspace(int what, int dtype, int64_t rows, int64_t cols, int64_t n_experts, int64_t n_rows);
+ktmi_prod_kernel prod_kernel_of(int what, int dtype, int64_t rows, int64_t cols, int64_t n_experts, int64_t n_rows);
 int launch_prod(int what, const ProdArgs& a, hipStream_t stream);
 int launch_gated_grad(const float* sums, const void* dh, int dtype, int64_t dh_stride, int64_t inter, int64_t n_rows, int act,
                       void* dsums, hipStream_t stream);
@@ -92,6 +93,7 @@ struct Fp8Args {
   uint8_t* ws;
 };
 int64_t fp8_workspace(int64_t rows, int64_t cols, int64_t x_rows, int64_t n_experts, int64_t top_k, bool ids);
+ktmi_prod_kernel fp8_kernel_of(int64_t rows, int64_t cols, int64_t x_rows, int64_t n_experts, int64_t top_k, bool ids);
 int launch_fp8(const Fp8Args& a, hipStream_t stream);
 
 // GEMV over raw GGUF rows against q8_1 activations (the decode-window kernel).

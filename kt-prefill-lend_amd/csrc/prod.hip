@@ -100,6 +100,16 @@ int64_t prod_workspace(int what, int dtype, int64_t rows, int64_t cols, int64_t 
   return p.tiles.splits > 1 ? 4 * p.tiles.splits * slice_of(p.rows * p.width) : 0;
 }
 
+static ktmi_prod_kernel told(bool few, const TilePlan& p) {
+  if (few) return {0, 0, 1};
+  return {tile_m(p.size), tile_n(p.size), p.splits};
+}
+
+ktmi_prod_kernel prod_kernel_of(int what, int dtype, int64_t rows, int64_t cols, int64_t n_experts, int64_t n_rows) {
+  const ProdPlan p = plan_prod(what, dtype, rows, cols, n_experts, n_rows);
+  return told(p.few, p.tiles);
+}
+
 int launch_prod(int what, const ProdArgs& a, hipStream_t stream) {
   const int es = size_of(a.dtype);
   const Segments seg = {a.offsets, (int)a.n_experts, (int)a.n_rows};
@@ -164,6 +174,11 @@ Fp8Plan plan_fp8(int64_t rows, int64_t cols, int64_t x_rows, int64_t n_experts, 
   return p;
 }
 }  // namespace
+
+ktmi_prod_kernel fp8_kernel_of(int64_t rows, int64_t cols, int64_t x_rows, int64_t n_experts, int64_t top_k, bool ids) {
+  const Fp8Plan p = plan_fp8(rows, cols, x_rows, n_experts, top_k, ids);
+  return told(p.few, p.tiles);
+}
 
 static int64_t fp8_slice_workspace(int64_t rows, int64_t cols, int64_t x_rows, int64_t n_experts, int64_t top_k, bool ids) {
   const int64_t blocks = (cols + 127) / 128;

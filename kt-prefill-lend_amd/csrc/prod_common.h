@@ -14,7 +14,12 @@ typedef uint32_t u32x4_a1_t __attribute__((ext_vector_type(4))) __attribute__((a
 namespace ktmi {
 
 // and stores
-__device__ __forceinline__ void gstore(void* p, u32x4_t v) { *(__attribute__((address_space(1))) u32x4_a1_t*)p = v; }
+template <bool STREAM>
+__device__ __forceinline__ void gstore(void* p, u32x4_t v) {
+  auto* g = (__attribute__((address_space(1))) u32x4_a1_t*)p;
+  if constexpr (STREAM) __builtin_nontemporal_store(v, g);
+  else *g = v;
+}
 
 // An element type: its bytes (ES), elements of a 16-byte chunk (EPC), the fp32 value of one and back, and
 // the products of 32 rows by 32 rows (mma32) and 16 by 16 (mma16) over the k of one chunk a lane: lane half

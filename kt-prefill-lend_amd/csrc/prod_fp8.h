@@ -239,11 +239,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile(Fp8TileArgs a) {
     const int m = 16 * (MF * wm + j);
     if (m >= pl.rows) break;
     if (a.splits > 1) {  // (its rows in the order of y already)
-      store_rows<float, 16, NF>(stage, [&](int i, int r) { return acc[i][j][r]; }, a.part + pl.split * a.slice + n0,
+      store_rows<float, 16, NF, false>(stage, [&](int i, int r) { return acc[i][j][r]; }, a.part + pl.split * a.slice + n0,
                                 [&](int i) { return (int64_t)place(m + i) * a.N; }, pl.rows - m, a.N - n0, lane);
       continue;
     }
-    store_rows<S, 16, NF>(stage, [&](int i, int r) { return acc[i][j][r]; }, (S*)a.y + n0,
+    store_rows<S, 16, NF, false>(stage, [&](int i, int r) { return acc[i][j][r]; }, (S*)a.y + n0,
                           [&](int i) { return (int64_t)place(m + i) * a.N; }, pl.rows - m, a.N - n0, lane);
   }
 }

@@ -4,6 +4,7 @@ Most cases use integers for x with one 448 (times a power of two) in each row's 
 codes are x itself, small integers for w and powers of two for the scales: every product and partial sum is
 exact in fp32 whatever the order of the sums, and no term is more than 2^13 times another, so the
 outputs have to be equal bit for bit. Others use general values against 64 bits."""
+import ctypes
 import math
 
 import pytest
@@ -100,6 +101,37 @@ def test_dense_exact(dev, T, N, K, dtype):
     x = make_x(T, K, dtype, T, dev)
     assert torch.equal(quantised(x), x.double())
     same(F.fp8_linear(x, w, s), x.double() @ matrix(w, s).t())
+
+
+# routed or not, rows of x, top_k, experts, N, K -> the tile, and whether blocks share its k
+SHAPES = [(0, 20, 1, 1, 40, 200, (0, 0), False), (1, 20, 2, 3, 40, 200, (0, 0), False), (0, 100, 1, 1, 300, 256, (64, 128), False),
+          (0, 256, 1, 1, 12300, 256, (128, 128), False), (0, 256, 1, 1, 12300, 200, (128, 128), False),
+          (0, 1000, 1, 1, 12300, 256, (256, 256), False), (0, 1000, 1, 1, 12300, 144, (256, 256), False),
+          (0, 100, 1, 1, 130, 8192, (64, 128), True), (0, 90, 1, 1, 131, 8197, (64, 128), True),
+          (1, 90, 2, 2, 70, 8192, (64, 128), True), (1, 300, 4, 2, 12300, 128, (256, 256), False)]
+
+
+def test_kernel_shapes_are_all_reached():
+    k = _lib.ktmi_prod_kernel()
+    for ids, T, top_k, E, N, K, tile, split in SHAPES:
+        assert _lib.lib().ktmi_fp8_kernel_of(ids, N, K, E, top_k, T, ctypes.byref(k)) == 0
+        assert ((k.tile_rows, k.tile_cols), k.splits > 1) == (tile, split), (ids, T, top_k, E, N, K, k.tile_rows, k.tile_cols, k.splits)
+    for args in [(0, 0, 8, 1, 1, 1), (0, 8, 0, 1, 1, 1), (0, 8, 8, 0, 1, 1), (0, 8, 8, 1, 0, 1), (0, 8, 8, 1, 1, 0)]:
+        assert _lib.lib().ktmi_fp8_kernel_of(*args, ctypes.byref(k)) == -1
+    assert _lib.lib().ktmi_fp8_kernel_of(0, 8, 8, 1, 1, 1, None) == -1
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("ids,T,top_k,E,N,K,tile,split", SHAPES)
+def test_shapes_exact(dev, ids, T, top_k, E, N, K, tile, split, dtype):
+    w, s = make_w((E,), N, K, N + K, dev)
+    x = make_x(T, K, dtype, T, dev)
+    if ids:
+        r = routes(T, top_k, E, 0.1, T, dev)
+        same(F.moe_fp8_vec(x, w, s, r, top_k), routed(x, w, s, r, top_k)[0])
+    else:
+        same(F.fp8_linear(x, w[0], s[0]), x.double() @ matrix(w[0], s[0]).t())
 
 
 def routes(T, k, E, cold, seed, dev):
@@ -312,6 +344,22 @@ def test_codes_past_32_bits(dev):
     w = torch.full((2048, 128), one, dtype=torch.uint8, device=dev)
     y = F.fp8_linear(x, w, torch.ones((16, 1), device=dev))
     assert (y[-1] == 448).all() and (y[:-1] == 0).all()
+
+
+@gpu
+def test_routed_tokens_past_32_bits_of_codes(dev):
+    """More than 2 GiB of quantised tokens: slices of them, the last one short."""
+    K, N, E, T = 1 << 17, 16, 2, (1 << 14) + 70
+    w = torch.zeros((E, N, K), device=dev).to(E4M3)
+    w[0, :, 5], w[1, :, K - 1] = 1, 2
+    x = torch.zeros((T, K), dtype=torch.bfloat16, device=dev)
+    x[:, 5], x[:, K - 1] = 448, 448
+    x[-3:] *= -1
+    ids = (torch.arange(T, device=dev) % 3 - 1).to(torch.int32)
+    y = F.moe_fp8_vec(x, w, torch.ones((E, 1, K // 128), device=dev), ids, 1)
+    want = torch.where(ids < 0, 0, 448 * (ids + 1)).to(torch.bfloat16)
+    want[-3:] *= -1
+    assert torch.equal(y, want[:, None].expand(T, N))
 
 
 @gpu

@@ -3,6 +3,7 @@
 The linear products are tested with small integers: every product and partial sum is exact in fp32 whatever the
 order of the sums, so outputs and gradients have to be equal bit for bit. The gate is not exact: its values
 are tested against 64 bits, with the roundings counted, and its gradients against the formula and against differences."""
+import ctypes
 import math
 
 import pytest
@@ -158,6 +159,68 @@ def check_gated(x, w, offsets, act, dh):
     if offsets is not None:
         end = int(offsets[-1])
         assert (got[0][end:] == 0).all() and (got[1][end:] == 0).all()
+
+
+def kernel_of(what, dtype, N, K, E, R):
+    k = _lib.ktmi_prod_kernel()
+    assert _lib.lib().ktmi_linear_kernel_of(what, _lib.dtype_code(dtype), N, K, E, R, ctypes.byref(k)) == 0
+    return k.tile_rows, k.tile_cols, k.splits
+
+
+# what, rows of each expert, N, K -> the tile of 16-bit and of fp32 rows and whether blocks share its k; K with whole steps,
+# with a last chunk, with a word in it
+FWD, DX, DW = _lib.PROD_LINEAR, _lib.PROD_GRAD_X, _lib.PROD_GRAD_W
+SHAPES = [(FWD, [30, 3], 40, 192, (0, 0), (0, 0), False), (FWD, [40, 70], 300, 128, (64, 128), (64, 128), False),
+          (FWD, [40, 70], 300, 136, (64, 128), (64, 128), False), (FWD, [40, 70], 300, 134, (64, 128), (64, 128), False),
+          (FWD, [250], 12300, 128, (128, 128), (64, 128), False), (FWD, [250], 12300, 138, (128, 128), (64, 128), False),
+          (FWD, [250, 252], 12300, 128, (128, 256), (64, 128), False), (FWD, [250, 252], 12300, 130, (128, 256), (64, 128), False),
+          (FWD, [1000], 12300, 128, (256, 256), (256, 256), False), (FWD, [1000], 12300, 150, (256, 256), (256, 256), False),
+          (FWD, [40, 70], 130, 4096, (64, 128), (64, 128), True), (FWD, [600], 200, 4100, (64, 128), (64, 128), True),
+          (DX, [40, 70], 128, 300, (64, 128), (64, 128), False), (DX, [250], 128, 12300, (128, 128), (64, 128), False),
+          (DX, [250], 138, 12300, (128, 128), (64, 128), False), (DX, [1000], 128, 12300, (256, 256), (256, 256), False),
+          (DX, [1000], 150, 12300, (256, 256), (256, 256), False), (DX, [70, 90], 4100, 130, (64, 128), (64, 128), True),
+          (DW, [40, 70], 200, 300, (128, 128), (128, 128), False), (DW, [60], 3300, 4100, (256, 256), (128, 128), False),
+          (DW, [5000], 200, 300, (128, 128), (128, 128), True), (DW, [2500, 2400], 100, 90, (128, 128), (128, 128), True)]
+
+
+def test_kernel_shapes_are_all_reached():
+    reached = set()
+    for what, counts, N, K, narrow, wide, split in SHAPES:
+        for dtype in DTYPES:
+            *tile, splits = kernel_of(what, dtype, N, K, len(counts), sum(counts) + 5)
+            assert tuple(tile) == (wide if dtype == torch.float32 else narrow) and (splits > 1) == split, (what, counts, N, K, dtype, tile, splits)
+            reached.add((what, *tile, splits > 1))
+    tiles = {(64, 128), (128, 128), (256, 256)}
+    assert {(w, *t, False) for w in (FWD, DX) for t in tiles} | {(FWD, 128, 256, False), (FWD, 0, 0, False), (DW, 256, 256, False),
+                                                                 (DW, 128, 128, False)} <= reached
+    k = ctypes.byref(_lib.ktmi_prod_kernel())
+    for args in [(4, 2, 8, 8, 1, 1, k), (-1, 2, 8, 8, 1, 1, k), (0, 3, 8, 8, 1, 1, k), (0, 2, 0, 8, 1, 1, k), (0, 2, 8, 0, 1, 1, k),
+                 (0, 2, 8, 8, 0, 1, k), (0, 2, 8, 8, 1, 0, k), (0, 2, 8, 8, 1, 1, None)]:
+        assert _lib.lib().ktmi_linear_kernel_of(*args) == -1
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("what,counts,N,K,narrow,wide,split", SHAPES)
+def test_shapes_exact(dev, what, counts, N, K, narrow, wide, split, dtype):
+    offsets, R = segments(counts, 5, dev)
+    x, w, dy = ints((R, K), dtype, 1, dev, 2), ints((len(counts), N, K), dtype, 2, dev, 2), ints((R, N), dtype, 3, dev, 2)
+    want = linear64(x, w, offsets, dy)
+    got = grads(lambda x, w: G.moe_linear_sorted(x, w, offsets), [x.requires_grad_(True), w.requires_grad_(True)], dy)
+    for a, b in zip(got, want):
+        same(a, b)
+
+
+# rows, I, K: the gate's tiles, with splits and without
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,N,K,tile,split", [(256, 6150, 128, (128, 128), False), (300, 12300, 192, (128, 256), False),
+                                              (1000, 6150, 130, (256, 256), False), (100, 90, 4100, (64, 128), True),
+                                              (70, 3, 8192, (64, 128), True)])
+def test_gated_shapes(dev, T, N, K, tile, split, dtype):
+    *got, splits = kernel_of(_lib.PROD_GATED, dtype, N, K, 1, T)
+    assert (dtype == torch.float32 or tuple(got) == tile) and (splits > 1) == split
+    check_gated(randn((T, K), dtype, 1, dev), randn((2 * N, K), dtype, 2, dev, 1 / math.sqrt(K)), None, "silu", randn((T, N), dtype, 3, dev))
 
 
 @gpu
@@ -559,6 +622,11 @@ def test_c_refusals():
         if fn is not grad_w:  # an expert without rows has a gradient too
             assert fn(R=0) == 0
     assert grad_w(dy=0) == -1 and grad_w(ds=63) == -1 and grad_w(R=0, y=0) == -1
+    # workspaces: what splits of a long k ask for
+    need = L.ktmi_linear_workspace(_lib.PROD_LINEAR, 2, 64, 8192, 1, 70)
+    assert need > 0 and linear(K=8192, xs=8192, N=64, E=1, R=70, n=need - 1) == -4 and linear(K=8192, xs=8192, N=64, E=1, R=70, ws=0) == -4
+    assert linear(K=8192, xs=8192, N=64, E=1, R=70, ws=p + 4) == -4
+    assert L.ktmi_linear_workspace(_lib.PROD_LINEAR, 2, 64, 64, 1, 70) == 0 and L.ktmi_linear_workspace(9, 2, 64, 8192, 1, 70) == 0
     # grids past 2^32 threads
     assert linear(E=2048, R=1 << 30, N=1 << 24) == -1 and b"grid" in L.ktmi_last_error()
     assert grad_x(E=2048, R=1 << 30, K=1 << 24) == -1 and b"grid" in L.ktmi_last_error()
