@@ -217,7 +217,8 @@ int ktmi_fp8_kernel_of(int routed, int64_t rows, int64_t cols, int64_t n_experts
  * = inter). */
 enum { KTMI_PROD_GATED = 0, KTMI_PROD_LINEAR = 1, KTMI_PROD_GRAD_X = 2, KTMI_PROD_GRAD_W = 3 };
 int64_t ktmi_linear_workspace(int what, int dtype, int64_t rows, int64_t cols, int64_t n_experts, int64_t n_rows);
-/* The kernel that such a call takes (as w4_kernel_of). */
+/* The kernel that such a call takes, if its rows start at multiples of 4 bytes: others, and a k that does not end with a
+ * step of 128 bytes, take 128 x 128 in place of 128 x 256, others also of 256 x 256 (as does fp32 x of the 8-bit products). */
 typedef struct ktmi_prod_kernel {
   int32_t tile_rows;  /* rows of x a tile (gradient of w: of w); 0: the kernel of few rows */
   int32_t tile_cols;  /* columns of y a tile (GATED: of both projections together) */

@@ -48,7 +48,8 @@ int launch_tile(const TileArgs& a, int size, hipStream_t stream) {
   return launch_tile_of<T, MODE, GATED, true, false, TILE_SMALL>(a, stream);
 }
 
-// ---- the sums of a tile's k shared by `splits` blocks, in the blocks' order: four values a thread where rows
+// ---- the sums of a tile's k shared by `splits` blocks, in the blocks' order (the same bits from run to run; 512 x 4096 in three slices 5
+// us, bound by the caches and its launch): four values a thread where rows
 // hold multiples of four (VEC), else one. gated: rows [g; u] of 2 N, h = act(g) u.
 template <typename T, bool GATED, bool VEC>
 __global__ __launch_bounds__(256) void sum_parts(const float* part, int splits, int64_t slice, int64_t rows, int N, int act,
@@ -150,7 +151,8 @@ int launch_fp8_tile(const Fp8TileArgs& a, int size, hipStream_t stream) {
   return direct ? launch_fp8_tile_of<S, EXACT, true, TILE_SMALL>(a, stream) : launch_fp8_tile_of<S, EXACT, false, TILE_SMALL>(a, stream);
 }
 
-// ---- one group of 16 lanes a group of 128 values: codes [rows, blocks * 128], scales [blocks, rows]
+// ---- one group of 16 lanes a group of 128 values: codes [rows, blocks * 128], scales [blocks, rows] (a tile takes the scales of
+// its rows for a block at a time). Bound by HBM: 91750 of 131072 rows of 2048 bf16 126 us, 4.5 TB/s.
 template <typename X>
 __global__ __launch_bounds__(256) void fp8_quantise(const uint8_t* x, int64_t stride, int K, int64_t rows, const int32_t* end,
                                                     uint8_t* codes, float* scales) {
@@ -192,7 +194,8 @@ int launch_quantise(const void* x, int64_t stride, int64_t K, int64_t rows, cons
   return KTMI_OK;
 }
 
-// ---- the gradients of the sums from that of h = act(g) u: dg = dh u act'(g), du = dh act(g)
+// ---- the gradients of the sums from that of h = act(g) u: dg = dh u act'(g), du = dh act(g), from the fp32 sums, rounded once to
+// the type that the products take. Bound by HBM: 4096 x 2048 bf16 20 us, 5 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void gated_grad(const float* gu, const uint8_t* dh, int64_t dh_stride, int N, int64_t rows,
                                                   int act, uint8_t* dgu) {

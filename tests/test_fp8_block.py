@@ -347,6 +347,19 @@ def test_codes_past_32_bits(dev):
 
 
 @gpu
+@pytest.mark.parametrize("K", [(1 << 23) + 128, 1 << 24])
+def test_longest_rows(dev, K):
+    """Tiles of rows whose codes lie up to 2 GiB apart."""
+    T, N = 140, 3
+    x = torch.zeros((T, K), dtype=torch.bfloat16, device=dev)
+    w = torch.zeros((N, K), dtype=torch.uint8, device=dev)
+    w[:, K - 1] = w[:, 3] = int(torch.tensor(1.0).to(E4M3).view(torch.uint8))
+    x[:, K - 1], x[::2, 3] = 448, 448
+    y = F.fp8_linear(x, w, torch.ones((1, K // 128), device=dev))
+    assert (y[::2] == 896).all() and (y[1::2] == 448).all()
+
+
+@gpu
 def test_routed_tokens_past_32_bits_of_codes(dev):
     """More than 2 GiB of quantised tokens: slices of them, the last one short."""
     K, N, E, T = 1 << 17, 16, 2, (1 << 14) + 70
