@@ -18,10 +18,13 @@ int64_t mean_rows(int64_t rows, int64_t n_experts) { return (rows + n_experts - 
 
 int64_t ints(int64_t n) { return (n + 3) / 4 * 4; }
 
-// Whether the kernels for few rows run: up to 32 a matrix, where tiles of 128 of its rows would be too few blocks to keep
-// the CUs' loads on their way. (128 experts of 1536 x 2048 bf16, 8 rows each: 155 us, in tiles of 64 rows 149; 32 rows: 259 and 155; one
-// of 4096 x 7168, 32 rows: 21 us, in tiles 60.)
-bool few_rows(int64_t mean, int64_t parts, int64_t n) { return mean <= 32 && parts * ((n + 127) / 128) < 512; }
+// Whether the kernel for few rows runs: up to 32 a matrix, where tiles of 128 of its rows would be too few blocks to keep
+// the CUs' loads on their way, the fewer the more rows of x there are to read for each. (bf16, then e4m3: one row by
+// 65280 x 4096 104 and 48 us, in tiles 101 and 43; 16 rows 107 and 64, in tiles 102 and 45; 32 rows 130 and 132, in tiles 105 and 45; 32 rows by
+// 7168 x 2048 13 and 16, in tiles 11 and 17.)
+bool few_rows(int64_t mean, int64_t parts, int64_t n) {
+  return mean <= 32 && parts * ((n + 127) / 128) < (mean <= 4 ? 512 : mean <= 16 ? 256 : 64);
+}
 
 // A product's tiles and the blocks that share a tile's k.
 struct TilePlan {

@@ -107,9 +107,9 @@ int launch_rows_of(RowsArgs a, hipStream_t stream) {
   return KTMI_OK;
 }
 
-// mean: rows of a matrix. Rows of w a wave: 16 where more would leave CUs without a block, else 64 (32 against 32 rows of
-// x), which share the rows of x and, of e4m3, their quantisation. Rows of w below 16 units are too short for eight
-// waves: two share one.
+// mean: rows of a matrix. Rows of w a wave: 16 where more would leave CUs without a block, else 32 or 64, which share the rows of
+// x and, of e4m3, their quantisation (one row by 16384 x 4096 e4m3: 25 us with 16). Rows of w below 16 units are too
+// short for eight waves: two share one.
 template <typename X, bool FP8, bool GATED>
 int launch_rows(const RowsArgs& a, int mean, hipStream_t stream) {
   constexpr int UE = 128 / (FP8 ? 1 : X::ES);
@@ -118,11 +118,18 @@ int launch_rows(const RowsArgs& a, int mean, hipStream_t stream) {
   const int64_t parts = a.ids || a.seg.offsets ? min((int64_t)a.seg.E, (int64_t)a.R) : (a.R + cols - 1) / cols;
   const int64_t frags = parts * (GATED ? 2 : 1) * a.N / 16;
   if (cols == 16) {
-    if (frags < 4 * 512) return launch_rows_of<X, FP8, GATED, 1, 1, 8>(a, stream);
-    return shorter ? launch_rows_of<X, FP8, GATED, 1, 2, 2>(a, stream) : launch_rows_of<X, FP8, GATED, 1, 4, 8>(a, stream);
+    if (frags < (FP8 ? 512 : 4 * 512)) return launch_rows_of<X, FP8, GATED, 1, 1, 8>(a, stream);
+    if (shorter) return launch_rows_of<X, FP8, GATED, 1, 2, 2>(a, stream);
+    if constexpr (FP8) {
+      if (frags < 1024) return launch_rows_of<X, FP8, GATED, 1, 2, 8>(a, stream);
+    }
+    return launch_rows_of<X, FP8, GATED, 1, 4, 8>(a, stream);
   }
-  if (frags < 4 * 512) return launch_rows_of<X, FP8, GATED, 2, 1, 8>(a, stream);
-  return shorter ? launch_rows_of<X, FP8, GATED, 2, 2, 2>(a, stream) : launch_rows_of<X, FP8, GATED, 2, 2, 8>(a, stream);
+  if constexpr (FP8) {  // (without ids few_rows() ends below)
+    if (frags >= 4 * 512)
+      return shorter ? launch_rows_of<X, FP8, GATED, 2, 2, 2>(a, stream) : launch_rows_of<X, FP8, GATED, 2, 2, 8>(a, stream);
+  }
+  return launch_rows_of<X, FP8, GATED, 2, 1, 8>(a, stream);
 }
 
 template <typename S, bool EXACT, bool DIRECT, int SIZE>

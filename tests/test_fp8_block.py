@@ -90,7 +90,9 @@ def same(got, want64):
 # tokens, N, K: few rows, then tiles; rows of w at any alignment; ends inside a block, a chunk, a tile
 DENSE = [(1, 1, 1), (1, 5, 127), (2, 17, 128), (3, 130, 129), (1, 515, 1111), (7, 64, 1000), (16, 128, 256), (17, 96, 384),
          (33, 20, 2080), (64, 300, 130), (65, 1, 1), (65, 129, 128), (66, 515, 1111), (100, 260, 1000), (129, 128, 144),
-         (255, 257, 640), (300, 600, 272), (1100, 4200, 256), (1000, 4097, 400), (513, 8192, 130)]
+         (255, 257, 640), (300, 600, 272), (1100, 4200, 256), (1000, 4097, 400), (513, 8192, 130),
+         # few rows by many: more rows of w a wave, short rows
+         (3, 8200, 2100), (16, 16500, 2050), (2, 8200, 256), (1, 33000, 2176)]
 
 
 @gpu
@@ -143,7 +145,8 @@ def routes(T, k, E, cold, seed, dev):
 
 ROUTED = [(1, 1, 1, 5, 64, 0.0), (1, 8, 40, 64, 256, 0.3), (5, 3, 7, 72, 130, 0.2), (64, 1, 1, 33, 160, 0.0), (21, 3, 2, 48, 384, 0.1),
           (40, 8, 300, 16, 96, 0.0), (6, 2, 4, 20, 77, 1.0), (64, 8, 3, 130, 288, 0.1), (70, 4, 2, 200, 1000, 0.2),
-          (600, 2, 3, 300, 272, 0.3), (300, 4, 64, 40, 144, 0.0), (90, 1, 1, 140, 515, 0.5)]
+          (600, 2, 3, 300, 272, 0.3), (300, 4, 64, 40, 144, 0.0), (90, 1, 1, 140, 515, 0.5),
+          (60, 1, 2, 17000, 300, 0.1), (20, 3, 2, 17000, 2100, 0.1)]
 
 
 @gpu

@@ -94,7 +94,7 @@ def grads(fn, leaves, d):
 LINEAR = [([1], 0, 1, 1), ([2], 0, 5, 7), ([0, 3, 0, 0, 17, 1, 0], 4, 72, 384), ([0, 0, 0], 7, 9, 96), ([70, 0, 33], 0, 40, 130),
           ([5] * 60, 3, 16, 96), ([300, 2], 1, 24, 256), ([0] * 500 + [2, 1], 2, 33, 64), ([1] * 2048, 5, 3, 8),
           ([129, 0, 257, 64], 130, 300, 144), ([90, 400], 3, 129, 515), ([700, 500], 300, 1030, 520), ([1111], 0, 515, 1111),
-          ([260, 230, 200, 250], 9, 2048, 1536)]
+          ([260, 230, 200, 250], 9, 2048, 1536), ([3], 0, 33000, 1100), ([2], 1, 33000, 200), ([25, 20], 1, 200, 600)]
 
 
 @gpu
@@ -111,7 +111,8 @@ def test_linear_exact(dev, counts, tail, N, K, dtype):
 
 
 # the gate and up of whole tiles, of parts of them, of few rows
-GATED = [(1, 1, 1), (3, 5, 7), (16, 8, 64), (17, 33, 130), (64, 20, 515), (65, 1, 8), (100, 130, 256), (200, 257, 1000), (1000, 1100, 144)]
+GATED = [(1, 1, 1), (3, 5, 7), (16, 8, 64), (17, 33, 130), (64, 20, 515), (65, 1, 8), (100, 130, 256), (200, 257, 1000), (1000, 1100, 144),
+         (2, 17000, 1100), (3, 17000, 130), (30, 300, 500)]
 
 
 @gpu
