@@ -184,7 +184,7 @@ int ktmi_w4_kernel_of(int by, int x_dtype, int64_t cols, int64_t group, int64_t 
  * codes (OCP, no infinities) [n_experts, rows, cols], scales fp32 [n_experts, ceil(rows / 128), ceil(cols / 128)]. x is
  * quantised on the way: a = max(|x|, 2^-116) over the block's values of the row, xq = e4m3(f32(x * f32(448 / a))),
  * xs = f32(a / 448); a value that is not finite makes its row NaN. Sums in fp32, rounded once to x's type. Any cols and
- * rows (to 2^24), any alignment of the codes; rows of x that start at multiples of 16 bytes and cols that are multiples of 16 are
+ * rows (to 2^24), any alignment of the codes; codes at a multiple of 4 bytes and cols that are a multiple of 16 are
  * the fast case. No counterpart in the reference. */
 int64_t ktmi_fp8_linear_workspace(int64_t rows, int64_t cols, int64_t tokens);
 int ktmi_fp8_linear(const void* x, int x_dtype, int64_t x_stride, int64_t cols, const void* w, const float* scales,
@@ -210,7 +210,7 @@ int ktmi_fp8_kernel_of(int routed, int64_t rows, int64_t cols, int64_t n_experts
  * Rows of x [n_rows, cols] by the matrix of their expert, in bf16, f16 or fp32 (x, w, y and gradients of one type), sums in
  * fp32, rounded once. offsets: the experts' segments as ktmi_moe_sort gives them (rows in no segment give zeros, clamped
  * as above), or NULL for one matrix (n_experts 1). No atomics: the same bits from run to run. Any sizes (to 2^24) and
- * alignment; rows at multiples of 16 bytes are the fast case. No counterpart in the reference. */
+ * alignment; rows at multiples of 4 bytes are the fast case. No counterpart in the reference. */
 #define KTMI_ACT_SILU 0
 #define KTMI_ACT_GELU_TANH 1
 /* Workspace of a call (0: none is needed), for sums of a long k shared by several blocks. rows, cols: those of w (GATED: rows
