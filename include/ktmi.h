@@ -183,9 +183,10 @@ int ktmi_w4_kernel_of(int by, int x_dtype, int64_t cols, int64_t group, int64_t 
  * y[r, n] = sum_g xs[r, g] * scales[e, n / 128, g] * sum_{c in block g} xq[r, c] * w[e, n, c], blocks of 128 columns. w: e4m3
  * codes (OCP, no infinities) [n_experts, rows, cols], scales fp32 [n_experts, ceil(rows / 128), ceil(cols / 128)]. x is
  * quantised on the way: a = max(|x|, 2^-116) over the block's values of the row, xq = e4m3(f32(x * f32(448 / a))),
- * xs = f32(a / 448); a value that is not finite makes its row NaN. Sums in fp32, rounded once to x's type. Any cols and
- * rows (to 2^24), any alignment of the codes; codes at a multiple of 4 bytes and cols that are a multiple of 16 are
- * the fast case. No counterpart in the reference. */
+ * xs = f32(a / 448); a value that is not finite makes its row NaN. Sums in fp32, rounded once to x's type; xs * scales is an
+ * fp32 number, the largest one where it is past it (a scale that is not finite aside). Any cols and rows (to 2^24), any
+ * alignment of the codes; codes at a multiple of 4 bytes and cols that are a multiple of 16 are the fast case. No
+ * counterpart in the reference. */
 int64_t ktmi_fp8_linear_workspace(int64_t rows, int64_t cols, int64_t tokens);
 int ktmi_fp8_linear(const void* x, int x_dtype, int64_t x_stride, int64_t cols, const void* w, const float* scales,
                     int64_t rows, int64_t tokens, void* y, void* workspace, int64_t ws_bytes, void* stream);

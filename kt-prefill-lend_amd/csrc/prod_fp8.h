@@ -71,6 +71,12 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, u, true);
 }
 
+// The product of a scale of x and one of w, held at fp32's largest number where it is past it: with an infinite one a block whose
+// codes sum to 0 would add NaN in place of 0. most = most_product(ws), which for an infinite or NaN ws leaves the product as it
+// is. (x that is not finite has NaN codes, whatever the scales.)
+__device__ __forceinline__ float most_product(float ws) { return __builtin_isfinite(ws) ? 0x1.fffffep127f : fabsf(ws); }
+__device__ __forceinline__ float scales_product(float xs, float ws, float most) { return __builtin_amdgcn_fmed3f(xs * ws, -most, most); }
+
 struct Fp8TileArgs {
   const uint8_t* x;         // codes [rows, x_stride], quantised rows padded with zeros to whole blocks
   const float* xs;          // scales [blocks, xs_stride]
@@ -178,7 +184,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile(Fp8TileArgs a) {
 #pragma unroll
     for (int i = 0; i < NF; ++i) read_q(0, i);
     read_p(0, 0, 0);
-    float sw = *(const float*)(lds + sw_at);
+    float sw = *(const float*)(lds + sw_at), most = most_product(sw);
     // The products of 16 rows of x go to c[0] and c[1] in turn: while the matrix cores work on one, the other's are
     // scaled and added, four instructions behind each of theirs. The asm keeps the compiler from moving that past
     // the branches below, with every block's sums in registers till then. A c is read behind the four products of the other,
@@ -187,7 +193,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile(Fp8TileArgs a) {
     float s[2] = {0, 0};
     auto products = [&](int j, auto between) {
       const int cur = j & 1, prev = cur ^ 1, jp = (j + MF - 1) % MF;  // jp of the step before at first
-      s[cur] = sx[cur] * sw;
+      s[cur] = scales_product(sx[cur], sw, most);
 #pragma unroll
       for (int i = 0; i < NF; ++i) {
         c[cur][i] = mma_block<EXACT>(qf[i], pf[cur]);
@@ -219,7 +225,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile(Fp8TileArgs a) {
       load(min(k + 2, end_k), buf);
       products(MF - 1, [&](int i) { read_q(next, i); });
       read_p(next, 0, 0);
-      sw = *(const float*)(lds + next * BUF + sw_at);
+      sw = *(const float*)(lds + next * BUF + sw_at), most = most_product(sw);
     }
     settle(c);
 #pragma unroll

@@ -152,6 +152,11 @@ __global__ __launch_bounds__(64 * WK * WR) void prod_rows(RowsArgs a) {
       }
     };
     auto compute = [&](const Unit& v) {
+      float most[NRF];
+      if constexpr (FP8) {
+#pragma unroll
+        for (int f = 0; f < NRF; ++f) most[f] = most_product(v.s[f]);
+      }
 #pragma unroll
       for (int t = 0; t < CT; ++t) {
         if constexpr (FP8) {
@@ -163,7 +168,7 @@ __global__ __launch_bounds__(64 * WK * WR) void prod_rows(RowsArgs a) {
 #pragma unroll
           for (int f = 0; f < NRF; ++f) {
             asm volatile("" : "+v"(c[f]));  // read in the products' block: see settle()
-            const float sc = s * v.s[f];
+            const float sc = scales_product(s, v.s[f], most[f]);
 #pragma unroll
             for (int r = 0; r < 4; ++r) acc[f][t][r] = __builtin_fmaf(c[f][r], sc, acc[f][t][r]);
           }

@@ -11,7 +11,7 @@ each row and block of 128 columns: a = max(|x|, 2^-116), xq = e4m3(f32(x * f32(4
 to nearest, ties to even; a value that is not finite makes its row of y NaN. Sums are in fp32 (of y in 16
 bits a block's sum by the matrix cores' 8-bit products, which keep about 16 bits below the largest product)
 and rounded once to x's type; the two scales' product is an fp32 number (below 2^-126 in its subnormal
-steps). Any K and N (to 2^24).
+steps, past fp32's largest number that one, unless the scale of w is not finite). Any K and N (to 2^24).
 They run on the current stream of x's device, allocate from torch's caching allocator, never
 synchronise and can be captured into a HIP graph. No gradient: inputs that require one are refused
 while gradients are recorded (RuntimeError), inputs with a forward-mode tangent always

@@ -254,6 +254,41 @@ def test_ends_of_the_range(dev, T, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [3, 90])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_scales_whose_product_is_past_the_range(dev, T, sign, dtype):
+    """A block of the type's largest values by a scale of 2^125: their product is no fp32 number, and a row of w with zeros there
+    adds 0 all the same, so that the other blocks' sums are left, bit for bit. One with codes there is infinite; a scale
+    that is not finite makes its rows so."""
+    N, K = 300, 640
+    w, s = make_w((), N, K, 3, dev)
+    x = make_x(T, K, dtype, 4, dev)
+    want = x.double()
+    want[:, 128:256] = 0
+    want = want @ matrix(w, s).t()
+    x[:, 128:256] = 0
+    x[:, 130] = torch.finfo(dtype).max
+    s[:, 1] = sign * 2.0 ** 125
+    w = w.view(torch.uint8)
+    w[:, 130] = 0
+    got = F.fp8_linear(x, w, s)
+    same(got, want)
+    ids = (torch.arange(T, device=dev) % 2).to(torch.int32)
+    assert torch.equal(F.moe_fp8_vec(x, torch.stack([w, w]), torch.stack([s, s]), ids, 1), got)
+    w[7, 130] = torch.tensor(448.0).to(E4M3).view(torch.uint8)
+    y = F.fp8_linear(x, w, s)
+    assert (y[:, 7] == sign * math.inf).all()
+    rest = torch.arange(N, device=dev) != 7
+    assert torch.equal(y[:, rest], got[:, rest])
+    w[:, 130] = w[7, 130]
+    for bad in (math.inf, -math.inf, math.nan):
+        s[1, 1] = bad
+        y = F.fp8_linear(x, w, s)
+        assert y[:, 128:256].isnan().all() if math.isnan(bad) else (y[:, 128:256] == bad).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T", [5, 90])
 @pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
 def test_not_finite(dev, T, dtype, bad):
