@@ -286,8 +286,8 @@ __device__ __forceinline__ void store_rows(uint8_t* stage, F v, O* c, A at, int 
   for (int t = 0; t < FR * CH / 64; ++t) {
     const int row = (t * 64 + lane) / CH, ch = lane % CH, left = cols - ch * EPC;
     const uint8_t* from = stage + row * ROW + 16 * (ch ^ (row & (CH - 1)));
-    O* to = c + at(row) + ch * EPC;
     if (row >= rows || left <= 0) continue;
+    O* to = c + at(row) + ch * EPC;  // (at(row) may read memory, which ends with the last row)
     if (left >= EPC) {
       gstore<STREAM>(to, *(const u32x4_t*)from);
     } else {
