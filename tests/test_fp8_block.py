@@ -228,6 +228,32 @@ def test_every_code(dev, T, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("T", [1, 17, 100])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_every_pair_of_codes(dev, T, dtype):
+    """All 254 finite codes of x, by their bytes, against all of w: one product an output, exact, the last rounding aside. (The
+    walk of test_every_code finds its place by value: at -0 it finds 0, and starts over.)"""
+    K = 128
+    codes = torch.arange(256, dtype=torch.uint8)
+    value = codes.view(E4M3).float()
+    finite = ~value.isnan()
+    of_x = codes[finite]
+    w = torch.zeros((256, K), dtype=torch.uint8)
+    w[:, 1] = codes
+    w, scales, done = w.to(dev), torch.ones((2, 1), device=dev), []
+    for i in range(-(-of_x.numel() // T)):
+        c = of_x[(torch.arange(T) * 53 + i * T * 53) % of_x.numel()]
+        x = torch.zeros((T, K))
+        x[:, 0], x[:, 1] = 448, c.view(E4M3).float()
+        y = F.fp8_linear(x.to(dtype).to(dev), w, scales).cpu()
+        want = c.view(E4M3).double()[:, None] * value.double()
+        assert torch.equal(y[:, finite], want[:, finite].float().to(dtype))
+        assert y[:, ~finite].isnan().all()
+        done.append(c)
+    assert torch.cat(done).unique().numel() == 254
+
+
+@gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T", [3, 100])
 def test_ends_of_the_range(dev, T, dtype):
