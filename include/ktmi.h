@@ -202,7 +202,8 @@ int ktmi_moe_fp8_sorted(const void* x, int x_dtype, int64_t x_stride, int64_t co
                         int64_t rows, int64_t n_experts, const int32_t* offsets, int64_t n_rows, void* y, void* workspace,
                         int64_t ws_bytes, void* stream);
 
-/* The kernel that such a call takes, as ktmi_linear_kernel_of tells; routed: 1 for ktmi_moe_fp8_vec's. */
+/* The kernel that such a call takes; routed: 1 for ktmi_moe_fp8_vec's. For 16-bit x and codes at a multiple of 4 bytes: fp32 x and
+ * other codes take 128 x 128 in place of 256 x 256. */
 struct ktmi_prod_kernel;
 int ktmi_fp8_kernel_of(int routed, int64_t rows, int64_t cols, int64_t n_experts, int64_t top_k, int64_t x_rows,
                        struct ktmi_prod_kernel* kernel);
@@ -218,8 +219,9 @@ int ktmi_fp8_kernel_of(int routed, int64_t rows, int64_t cols, int64_t n_experts
  * = inter). */
 enum { KTMI_PROD_GATED = 0, KTMI_PROD_LINEAR = 1, KTMI_PROD_GRAD_X = 2, KTMI_PROD_GRAD_W = 3 };
 int64_t ktmi_linear_workspace(int what, int dtype, int64_t rows, int64_t cols, int64_t n_experts, int64_t n_rows);
-/* The kernel that such a call takes, if its rows start at multiples of 4 bytes: others, and a k that does not end with a
- * step of 128 bytes, take 128 x 128 in place of 128 x 256, others also of 256 x 256 (as does fp32 x of the 8-bit products). */
+/* The kernel that such a call takes, if its rows start at multiples of 4 bytes and 256 of them (GATED: also all 2 inter rows of a
+ * matrix) span less than 2^31 bytes: others, and a k that does not end with a step of 128 bytes, take 128 x 128 in place of
+ * 128 x 256, others also of 256 x 256. */
 typedef struct ktmi_prod_kernel {
   int32_t tile_rows;  /* rows of x a tile (gradient of w: of w); 0: the kernel of few rows */
   int32_t tile_cols;  /* columns of y a tile (GATED: of both projections together) */

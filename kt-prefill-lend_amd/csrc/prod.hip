@@ -173,6 +173,7 @@ Fp8Plan plan_fp8(int64_t rows, int64_t cols, int64_t x_rows, int64_t n_experts, 
   Fp8Plan p = {};
   p.few = (ids && R <= 64) || few_rows(mean, parts, rows);
   p.tiles = plan_tiles(PROD_FWD, 1, mean, rows, (cols + 127) / 128, parts);
+  if (cols % 16 && p.tiles.size == TILE_LARGE) p.tiles.size = TILE_SMALL;  // codes through registers: no tiles of 256 rows
   if (cols > (1 << 22)) p.tiles.size = TILE_LOW;  // 32-bit offsets reach the codes of 64 rows of 2^24, of 256 of 2^22
   if (p.few) p.tiles.splits = 1;
   return p;

@@ -136,6 +136,25 @@ def test_shapes_exact(dev, ids, T, top_k, E, N, K, tile, split, dtype):
         same(F.fp8_linear(x, w[0], s[0]), x.double() @ matrix(w[0], s[0]).t())
 
 
+# columns that are no multiple of 16, whose codes go through registers: no tiles of 256 rows there
+RAGGED = [(0, 1000, 1, 1, 12300, 132, (128, 128)), (0, 1000, 1, 1, 12300, 130, (128, 128)), (0, 256, 1, 1, 12300, 137, (128, 128)),
+          (1, 300, 4, 2, 12300, 132, (128, 128)), (0, 100, 1, 1, 300, 132, (64, 128)), (0, 20, 1, 1, 300, 132, (0, 0))]
+
+
+def test_kernels_of_ragged_columns():
+    k = _lib.ktmi_prod_kernel()
+    for ids, T, top_k, E, N, K, tile in RAGGED:
+        assert _lib.lib().ktmi_fp8_kernel_of(ids, N, K, E, top_k, T, ctypes.byref(k)) == 0
+        assert (k.tile_rows, k.tile_cols, k.splits) == (*tile, 1), (ids, T, top_k, E, N, K, k.tile_rows, k.tile_cols, k.splits)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("ids,T,top_k,E,N,K,tile", RAGGED)
+def test_ragged_columns_exact(dev, ids, T, top_k, E, N, K, tile, dtype):
+    test_shapes_exact(dev, ids, T, top_k, E, N, K, tile, False, dtype)
+
+
 def routes(T, k, E, cold, seed, dev):
     g = torch.Generator().manual_seed(seed)
     ids = torch.randint(0, E, (T * k,), generator=g, dtype=torch.int32)
