@@ -90,17 +90,25 @@ __device__ __forceinline__ u32x4_t load_chunk(const uint8_t* row, int64_t k, int
 // (g + 0.044715 g^3), which is the tanh form g (1 + tanh z) / 2: both are g times a sigmoid. Past |g| = 16
 // the second's sigmoid is 0 or 1 in fp32, so the cube takes a clamped g, which cannot overflow.
 constexpr float GELU_2C = 1.5957691216057308f, GELU_A = 0.044715f;
-__device__ __forceinline__ float sigmoid(float v) { return 1.0f / (1.0f + __expf(-v)); }
-__device__ __forceinline__ float clamp16(float g) { return g > 16.0f ? 16.0f : g < -16.0f ? -16.0f : g; }
-__device__ __forceinline__ float gate_sigmoid(int act, float g) {
-  if (act == KTMI_ACT_SILU) return sigmoid(g);
-  const float c = clamp16(g);
-  return sigmoid(GELU_2C * (c + GELU_A * c * c * c));
+// S: the type that the values are rounded to. In 16 bits the power is that of v_exp_f32 with the argument's product with log2 e
+// rounded (2^-24 |v| of it), far below their rounding; in fp32 it is right to a step.
+template <typename S>
+__device__ __forceinline__ float sigmoid(float v) {
+  return 1.0f / (1.0f + (std::is_same<S, float>::value ? expf(-v) : __expf(-v)));
 }
-__device__ __forceinline__ float act_of(int act, float g) { return g * gate_sigmoid(act, g); }
+__device__ __forceinline__ float clamp16(float g) { return g > 16.0f ? 16.0f : g < -16.0f ? -16.0f : g; }
+template <typename S>
+__device__ __forceinline__ float gate_sigmoid(int act, float g) {
+  if (act == KTMI_ACT_SILU) return sigmoid<S>(g);
+  const float c = clamp16(g);
+  return sigmoid<S>(GELU_2C * (c + GELU_A * c * c * c));
+}
+template <typename S>
+__device__ __forceinline__ float act_of(int act, float g) { return g * gate_sigmoid<S>(act, g); }
 // act(g) and its derivative
+template <typename S>
 __device__ __forceinline__ void act_grad(int act, float g, float& f, float& d) {
-  const float s = gate_sigmoid(act, g), c = clamp16(g);
+  const float s = gate_sigmoid<S>(act, g), c = clamp16(g);
   f = g * s;
   d = act == KTMI_ACT_SILU ? s + f * (1.0f - s) : s + c * s * (1.0f - s) * GELU_2C * (1.0f + 3.0f * GELU_A * c * c);
 }

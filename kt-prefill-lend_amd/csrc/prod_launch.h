@@ -72,7 +72,7 @@ __global__ __launch_bounds__(256) void sum_parts(const float* part, int splits, 
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     if constexpr (GATED) {
-      o[v] = (S)(act_of(act, g[v]) * u[v]);
+      o[v] = (S)(act_of<S>(act, g[v]) * u[v]);
       if (gu) gu[row * 2 * N + col + v] = g[v], gu[row * 2 * N + N + col + v] = u[v];
     } else {
       o[v] = (S)g[v];
@@ -223,7 +223,7 @@ __global__ __launch_bounds__(256) void gated_grad(const float* gu, const uint8_t
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float f, df;
-      act_grad(act, gv[i], f, df);
+      act_grad<S>(act, gv[i], f, df);
       a[i] = (S)((float)dv[i] * uv[i] * df);
       b[i] = (S)((float)dv[i] * f);
     }
@@ -232,7 +232,7 @@ __global__ __launch_bounds__(256) void gated_grad(const float* gu, const uint8_t
   } else {
     for (int i = 0; i < 4 && n + i < N; ++i) {
       float f, df;
-      act_grad(act, g[i], f, df);
+      act_grad<S>(act, g[i], f, df);
       dg[i] = (S)((float)d[i] * u[i] * df);
       du[i] = (S)((float)d[i] * f);
     }

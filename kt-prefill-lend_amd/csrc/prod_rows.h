@@ -219,7 +219,7 @@ __global__ __launch_bounds__(64 * WK * WR) void prod_rows(RowsArgs a) {
     float v = 0;
     if constexpr (GATED) {
       float g = 0, u = 0;
-      if (expert >= 0) g = sum(n >> 3, n & 7, c), u = sum(n >> 3, 8 + (n & 7), c), v = act_of(a.act, g) * u;
+      if (expert >= 0) g = sum(n >> 3, n & 7, c), u = sum(n >> 3, 8 + (n & 7), c), v = act_of<S>(a.act, g) * u;
       if (a.gu) {
         a.gu[at * 2 * a.N + n0 + n] = g;
         a.gu[at * 2 * a.N + a.N + n0 + n] = u;

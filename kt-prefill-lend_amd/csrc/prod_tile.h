@@ -465,7 +465,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void prod_tile(TileArgs a) {
         store_rows<float, 32, NO, true>(stage, [&](int i, int r) { return acc[i + NO][j][r]; }, gu + a.N, gu_at, rows, cols, lane);
       }
       if (a.splits > 1) continue;
-      store_rows<S, 32, NO, MODE == PROD_DW>(stage, [&](int i, int r) { return act_of(a.act, acc[i][j][r]) * acc[i + NO][j][r]; }, row, at, rows,
+      store_rows<S, 32, NO, MODE == PROD_DW>(stage, [&](int i, int r) { return act_of<S>(a.act, acc[i][j][r]) * acc[i + NO][j][r]; }, row, at, rows,
                             cols, lane);
     } else if (a.splits > 1) {
       store_rows<float, 32, NO, false>(stage, [&](int i, int r) { return acc[i][j][r]; }, sums + (row - (S*)a.c), at, rows, cols, lane);

@@ -248,6 +248,35 @@ def test_gate_over_its_range(dev, act):
 
 
 @gpu
+@pytest.mark.parametrize("rows,cols,tile,split", [(20, 2, (0, 0), False), (400, 2, (64, 128), False), (100, 4096, (64, 128), True)])
+def test_silu_keeps_fp32(dev, rows, cols, tile, split):
+    """h, dg and du in fp32 for g from -87, where the sigmoid is a normal number yet, to 87, and u = 1: in units of 2^-24 of their values
+    the power is off by 2 at most (a step), the sum and the quotient by 1 each, so the sigmoid s by 4, f = g s by 5, h = f u
+    by 6 and du = dh f too. 1 - s is off by 4 s and its own rounding; act' = s + f (1 - s) by 4 s + |f| (4 s + 7 (1 - s))
+    and the sum's rounding, dg by one more. The products with w are by 1 and 0. Terms of second order are below 2^-20 of these."""
+    N = 90
+    *got, splits = kernel_of(_lib.PROD_GATED, torch.float32, N, cols, 1, rows)
+    assert tuple(got) == tile and (splits > 1) == split
+    u = 2.0 ** -24 * (1 + 2.0 ** -18)
+    g = torch.linspace(-87, 87, 400 * 3, device=dev)
+    w = torch.zeros((2 * N, cols), device=dev)
+    w[:N, 0], w[N:, cols - 1] = 1, 1
+    for part in torch.cat([g, torch.linspace(-6, 6, 400, device=dev)]).split(rows):
+        x = torch.zeros((rows, cols), device=dev)
+        x[:, cols - 1] = 1
+        x[:part.numel(), 0] = part
+        dh = torch.zeros((rows, N), device=dev)
+        dh[:, N - 1] = 1
+        h, dx = grads(lambda x: G.gated(x, w), [x.requires_grad_(True)], dh)
+        v = x.detach()[:, 0].double()
+        s, r = torch.sigmoid(v), torch.sigmoid(-v)  # r = 1 - s
+        f, df = v * s, s * (1 + v * r)
+        assert ((h.double() - f[:, None]).abs() <= 6 * u * f.abs()[:, None]).all()
+        assert ((dx[:, cols - 1].double() - f).abs() <= 6 * u * f.abs()).all()
+        assert ((dx[:, 0].double() - df).abs() <= u * (4 * s + f.abs() * (4 * s + 7 * r) + 2 * df.abs())).all()
+
+
+@gpu
 @pytest.mark.parametrize("act", ACTS)
 def test_gradients_against_differences(dev, act):
     """Central differences of the forward pass itself, in fp32: of a sum over h weighted with dh, along random
