@@ -19,9 +19,11 @@ int64_t mean_rows(int64_t rows, int64_t n_experts) { return (rows + n_experts - 
 int64_t ints(int64_t n) { return (n + 3) / 4 * 4; }
 
 // Whether the kernel for few rows runs: up to 32 a matrix, where tiles of 128 of its rows would be too few blocks to keep
-// the CUs' loads on their way, the fewer the more rows of x there are to read for each. (bf16, then e4m3: one row by
-// 65280 x 4096 104 and 48 us, in tiles 101 and 43; 16 rows 107 and 64, in tiles 102 and 45; 32 rows 130 and 132, in tiles 105 and 45; 32 rows by
-// 7168 x 2048 13 and 16, in tiles 11 and 17.)
+// the CUs' loads on their way, the fewer the more rows of x there are to read for each. One limit for all types. us by 4096
+// columns, weights from HBM, in this kernel and in tiles: e4m3 one row by 16384 17 / 21, 65280 59 / 67, 131072 111 / 128; 16 rows by
+// 8192 13 / 17, 16384 20 / 21, 32768 38 / 31; 32 rows by 4096 15 / 16, 7168 27 / 18. bf16 one row by 16384 27 / 30, 65280 104 / 99,
+// 131072 195 / 174; 16 rows by 8192 21 / 21, 16384 40 / 30, 32768 60 / 65; 32 rows by 4096 15 / 15, 7168 26 / 20. So at
+// 32 rows the limit is late: from about 6000 rows of w on tiles take less.
 bool few_rows(int64_t mean, int64_t parts, int64_t n) {
   return mean <= 32 && parts * ((n + 127) / 128) < (mean <= 4 ? 512 : mean <= 16 ? 256 : 64);
 }
@@ -58,6 +60,8 @@ TilePlan plan_tiles(int mode, int es, int64_t m, int64_t n, int64_t steps, int64
     return es == 2 && (tiles(TILE_LARGE) >= 192 || other < us) ? large : small;
   }
   if (m <= (es == 4 ? 256 : 64) || tiles(TILE_SMALL) < 192) return split(TILE_LOW, &us);
+  // (8-bit, 64 experts of 1024 x 2048, us in tiles of 128 / 256 rows: each 256 rows 67 / 62, 300 94 / 99, 400 125 / 108, 512 143 / 124; uneven
+  // ones of such a mean 86 / 93, 101 / 103, 125 / 139, 155 / 153, of 600 183 / 169)
   if (m >= 512 && tiles(TILE_LARGE) >= 192) return {TILE_LARGE, 1};
   if (mode == PROD_FWD && es != 1 && tiles(TILE_DEEP) >= 192) return {TILE_DEEP, 1};
   return split(TILE_SMALL, &us);
@@ -171,6 +175,9 @@ struct Fp8Plan {
 Fp8Plan plan_fp8(int64_t rows, int64_t cols, int64_t x_rows, int64_t n_experts, int64_t top_k, bool ids) {
   const int64_t R = x_rows * top_k, mean = mean_rows(R, n_experts), parts = n_experts < R ? n_experts : R;
   Fp8Plan p = {};
+  // Up to 64 routes are taken as they come, without the order's and the quantisation's launches. (64 routes by 4096 x 7168 of 4
+  // experts 33 us, in tiles, that is of 65 routes, 35; of 8 experts 53 / 53. Where many of them share an expert tiles take less: of one
+  // or two experts 58 / 25, by 65280 x 2048 338 / 41.)
   p.few = (ids && R <= 64) || few_rows(mean, parts, rows);
   p.tiles = plan_tiles(PROD_FWD, 1, mean, rows, (cols + 127) / 128, parts);
   if (cols % 16 && p.tiles.size == TILE_LARGE) p.tiles.size = TILE_SMALL;  // codes through registers: no tiles of 256 rows

@@ -94,8 +94,9 @@ struct Fp8TileArgs {
 };
 
 // A tile of y: WM x WN waves, each MF x NF fragments of 16 x 16, two buffers in LDS; see prod_tile, whose step of 128 bytes is a
-// block here. Bound by the matrix cores and the clock that they leave (4096 x 4096 x 7168: 136 us with the quantisation, 1.77 PFLOP/s,
-// busy 52% of the cycles), of few rows a matrix by HBM (128 experts of 2048 x 2048, up to 16 rows each: 120 us, 4.5 TB/s).
+// block here. Bound by the matrix cores and the vector instructions that scale their sums, which the waves of a SIMD overlap
+// only in part (8192 cubed: 52 and 35% of the cycles, at 1.96 GHz; 4096 x 4096 x 7168: 130 us with the quantisation, 1.85 PFLOP/s); of
+// few rows a matrix by HBM (128 experts of 2048 x 2048, up to 16 rows each: 109 us, 4.9 TB/s).
 template <typename S, bool EXACT, bool DIRECT, int WM, int WN, int MF, int NF>
 __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile(Fp8TileArgs a) {
   constexpr int THREADS = 64 * WM * WN, BM = 16 * WM * MF, BN = 16 * WN * NF;

@@ -4,8 +4,9 @@
 // x, which are the columns of the matrix cores' tiles. WK waves of a block share the k: wave i takes the 128-byte units
 // i, i + WK, .. of the rows, so that they read neighbouring bytes, and each unit of x is read by one of them
 // only, straight into the operands' registers; their sums meet in LDS. The block's other waves take the rows behind.
-// One row by 4096 x 7168: e4m3 9.3 us (the weights' bytes take 6.0), bf16 gate and up 11.0 (12.0 from HBM; the last-level cache
-// holds them); 16 rows 15 us, 32 rows 21 in both, where the rows of x from L2 take as long as w: tiles go on from there.
+// One row by 4096 x 7168, calls in a graph: e4m3 10.6 us with weights from HBM, which their bytes take 6.0 of, and 9.0 from the
+// last-level cache; bf16 gate and up 12.9 (12.0) and 11.3; an empty kernel of that grid 1.6. 16 rows 15 us, 32 rows 21 in both,
+// where the rows of x from L2 take as long as w: tiles go on from there.
 #pragma once
 #include "prod_fp8.h"
 

@@ -15,10 +15,11 @@ expert's segment (behind offsets[E]) give zero rows and have zero gradients, wha
 
 The gradients, with respect to the rows and the weights: the forward pass keeps x, w13 and both
 projections in fp32 (they are not rounded before the activation's derivative takes them); the gradients of the
-projections are rounded once to x's type, which is the matrix cores' operand (in f16 one past 65504 is infinite, and with it
-its row of dx). In fp32 silu and its derivative are right to a few roundings; gelu's sigmoid is off by up to 2^-15 of itself where
-it is below 1e-30. No atomics: outputs and gradients are the same from run to run. They are not differentiable a second time. Forward-mode tangents
-(NotImplementedError) and traces by torch.jit.trace or make_fx (RuntimeError) are refused.
+projections are rounded once to x's type, which is the matrix cores' operand (in f16 one past 65504 is infinite,
+and so are the gradients that it enters). No atomics: outputs and gradients are the same from run to run. They are not
+differentiable a second time. In fp32 silu and its derivative are right to a few roundings; gelu's sigmoid, whose
+argument takes five, is off by up to 2^-15 of itself in its far tail. Forward-mode tangents (NotImplementedError) and
+traces by torch.jit.trace or make_fx (RuntimeError) are refused.
 All run on the current stream of the tensors' device, allocate from torch's caching allocator, never
 synchronise and can be captured into a HIP graph; a captured backward pass needs, as any in torch, that no
 graph of the same leaves built outside the capture is alive.
